@@ -16,3 +16,15 @@ __all__ = [
     "read_logits", "weight_count", "weight_info",
     "CQ35Error", "LIBRARY", "load", "SPLIT_KEYS_DEFAULT",
 ]
+
+# the operators over torch tensors (paged.py), loaded on first use: the rest of
+# the package runs without torch
+_PAGED = ("PLAN_STATUS", "PagePlan", "page_plan", "paged_prepare", "paged_attention", "paged_attention_workspace")
+__all__ += _PAGED
+
+
+def __getattr__(name):
+    if name in _PAGED:
+        from . import paged
+        return getattr(paged, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

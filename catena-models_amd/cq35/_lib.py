@@ -24,6 +24,18 @@ class TensorInfo(ctypes.Structure):
                 ("bytes", ctypes.c_int64)]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of ``cq35_paged_cache``."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Heads(ctypes.Structure):
+    """Mirror of ``cq35_heads``."""
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 def load():
     """Load the in-tree library; raise loudly when it has not been built."""
     global _lib
@@ -36,6 +48,7 @@ def load():
     l = ctypes.CDLL(LIBRARY)
     P, I64, I32, U64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint64
     PC = ctypes.POINTER(CConfig)
+    PG, PH = ctypes.POINTER(PagedCache), ctypes.POINTER(Heads)
     sig = {
         "cq35_last_error": ([], ctypes.c_char_p),
         "cq35_abi_version": ([], ctypes.c_int),
@@ -87,6 +100,12 @@ def load():
         "cq35_step_static": ([P, P, I64, U64, I64, P, ctypes.POINTER(U64), P], ctypes.c_int),
         "cq35_session_set_attention_split": ([P, I64], ctypes.c_int),
         "cq35_session_attention_split": ([P, ctypes.POINTER(I64)], ctypes.c_int),
+        "cq35_page_plan": ([P, I64, I64, I64, P, P, P, I64, P, I32, I64, P, P, P, P, P, P], ctypes.c_int),
+        "cq35_paged_prepare": ([PG, PH, PH, PH, I64, I32, P, P, ctypes.c_float, P, I32, P, I64, I32, P, P, PH, P],
+                               ctypes.c_int),
+        "cq35_paged_attention_workspace": ([I64, I64, I32, I32, I32, I64, I64, ctypes.POINTER(I64)], ctypes.c_int),
+        "cq35_paged_attention": ([PG, PH, PH, PH, I64, I32, P, I64, I64, I64, P, P, ctypes.c_float, I64, I64, P, I64, P],
+                                 ctypes.c_int),
         "cq35_session_phase_trace": ([P, P, I64, ctypes.POINTER(I64), ctypes.POINTER(I64)], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
@@ -118,4 +137,5 @@ EXPORTED = [
     "cq35_gguf_config", "cq35_gguf_validate", "cq35_model_load_gguf", "cq35_gguf_tensor_name",
     "cq35_step_batch", "cq35_step_static", "cq35_session_set_attention_split",
     "cq35_session_attention_split", "cq35_session_phase_trace",
+    "cq35_page_plan", "cq35_paged_prepare", "cq35_paged_attention_workspace", "cq35_paged_attention",
 ]

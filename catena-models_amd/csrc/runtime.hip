@@ -3174,3 +3174,4 @@ extern "C" int cq35_device_matrix_attention(const uint16_t* q, const uint16_t* g
 }
 
 #include "static_step.h"
+#include "paged_ops.h"

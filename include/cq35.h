@@ -322,6 +322,127 @@ int cq35_device_matrix_attention(const uint16_t* q, const uint16_t* gate, const 
                                  const uint16_t* v, int64_t n, int64_t start, int heads, int kv_heads,
                                  int head_dim, uint16_t* out);
 
+/* ---------------------------------------------------------- paged KV cache
+ * Operators over device memory for callers that serve many requests from one
+ * pool of cache pages beside their own projections: pages and slots of a
+ * round (cq35_page_plan), head norm + rotation + append (cq35_paged_prepare)
+ * and attention (cq35_paged_attention). No reference counterpart (its cache
+ * is one contiguous block per session, state_layout.hex:26-27).
+ *
+ * Every pointer is device memory (of one device, which need not be the
+ * calling thread's current one) unless its comment says host. A call checks
+ * its arguments, enqueues its kernels on `stream` (a hipStream_t of that
+ * device; NULL: its default stream) and returns; it allocates and waits for
+ * nothing, so it may be captured into a graph. Buffers stay valid until the
+ * work has run. Numbers in device memory (lengths, tables, slots) are read by
+ * the kernels, which never leave the buffers whatever they hold: what a wrong
+ * number does is said with each operator. */
+
+/* Keys and values of `pages` pages of `page_size` rows (a power of two, 16 to
+ * 65536), BF16. Row o of page p, head h starts at p * page_stride +
+ * o * row_stride + h * head_stride elements of `keys` and `values` (both laid
+ * out alike) and holds head_dim (64, 128 or 256) elements. Strides are
+ * multiples of 8, the bases 16-byte addresses; pages, rows and heads may
+ * follow each other in any order but not overlap. pages * page_size is below
+ * 2^31. */
+typedef struct cq35_paged_cache {
+  void* keys;
+  void* values;
+  int64_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int64_t page_stride;
+  int64_t row_stride;
+  int64_t head_stride;
+} cq35_paged_cache;
+
+/* Rows of heads, BF16: head h of row t starts at t * row_stride +
+ * h * head_stride elements. Strides are multiples of 8 (0 repeats a row of an
+ * input), the base a 16-byte address. */
+typedef struct cq35_heads {
+  void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} cq35_heads;
+
+/* The pages, positions and slots of a round: request r holds cached[r] tokens
+ * and is to hold lengths[r]. A longer one gets lengths[r] - cached[r] rows and
+ * the pages they need; a shorter one (0: finished) gives back the pages it no
+ * longer needs. Tables hold `width` page numbers, row r at r * table_stride;
+ * those of the first ceil(cached[r] / page_size) entries are read.
+ * `free_pages` is a stack of `pages` entries, the first *free_count of them
+ * free pages. Pages given back are pushed first, in request and table order,
+ * then the needed ones are popped in request and table order.
+ * Written: the tables' new entries; free_pages; row_start[requests + 1] (the
+ * exclusive sums of the requests' rows); positions and slots of `rows` rows (a
+ * row's slot is page * page_size + position % page_size; rows behind the last
+ * request's get position 0 and slot -1, also a row of an entry outside the
+ * pages); *free_left (the count after; not free_count itself); status[2]: 0, or
+ * 1 pages are missing (status[1] of them), 2 `rows` is too small (by
+ * status[1]), 3 a length is negative or longer than a table, 4 the stack's
+ * count is negative or above `pages`. Unless status[0] is 0 the tables and
+ * the stack are left as they were, row_start is 0 and every slot -1: later
+ * operators of the round then do nothing. Outputs overlap neither each other
+ * nor inputs, the tables and free_pages apart. requests: 1 to 8192. With the
+ * same free_count the call can be repeated with the same results. */
+int cq35_page_plan(int32_t* table, int64_t table_stride, int64_t requests, int64_t width,
+                   const int32_t* cached, const int32_t* lengths, int32_t* free_pages, int64_t pages,
+                   const int32_t* free_count, int32_t page_size, int64_t rows, int32_t* row_start,
+                   int32_t* positions, int32_t* slots, int32_t* free_left, int32_t* status,
+                   void* stream);
+
+/* Head norm, rotation and append of `rows` rows of projections: queries
+ * q_out = rotate(norm(q, q_weight)), keys rotate(norm(k, k_weight)) into cache
+ * row slots[t], values copied there. norm(x, w) = x w / sqrt(mean(x^2) + eps)
+ * over a head's channels (w: F32, head_dim entries at a 16-byte address);
+ * rotate turns channels i and i + rope_dim / 2 by position * inv_freq[i]
+ * (inv_freq: F32, rope_dim / 2 entries; rope_dim a multiple of 16), the
+ * position that of axis pair_axis[i] (host, rope_dim / 2 entries below `axes`;
+ * NULL with one axis): positions[axis * position_stride + t], up to 4 axes
+ * (time, height and width of images). F32 inside, the angle modulo a turn in
+ * 64 bits, each result rounded to BF16 once. q_out may be q itself, laid out
+ * alike. A row whose slot is negative or past the cache is left alone: neither
+ * its query nor the cache is written. Slots of one call differ; of two equal
+ * ones either row may end up in the cache, piece by piece. */
+int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const cq35_heads* k,
+                       const cq35_heads* v, int64_t rows, int32_t q_heads, const float* q_weight,
+                       const float* k_weight, float eps, const float* inv_freq, int32_t rope_dim,
+                       const int32_t* positions, int64_t position_stride, int32_t axes,
+                       const uint8_t* pair_axis, const int32_t* slots, const cq35_heads* q_out,
+                       void* stream);
+
+/* Attention of new tokens over the cache: rows row_start[r] up to
+ * row_start[r + 1] of q are the last tokens of request r, which holds
+ * lengths[r] tokens (theirs included) in the pages of table row r (`width`
+ * entries at r * table_stride). Row i of n is at position p = lengths[r] - n
+ * + i and sees the keys at positions 0 .. p:
+ *   out = sum_j softmax_j(scale q . k_j) v_j, times sigmoid(gate) where gate
+ * is not NULL; query head h reads key/value head h * kv_heads / q_heads.
+ * Products on the matrix cores with F32 sums; the weights e^(s - max) enter
+ * the second product as BF16 (relative error 2^-9 each, as the values they
+ * meet), the sums and the running maximum stay F32, the result is rounded to
+ * BF16 once. The same call gives the same bits.
+ * A row that sees no key (p < 0) gets zeros. Keys in pages whose number is
+ * outside the cache are not seen; lengths are cut to what the table holds.
+ * Rows outside every request are left alone. out may be q itself, laid out
+ * alike; it overlaps no other operand.
+ * max_rows and max_keys are what the caller knows of the most rows and keys
+ * of any request, 0 for nothing: they steer how the work is cut and the
+ * launches spared, results hold whatever they say.
+ * workspace: cq35_paged_attention_workspace bytes (of the same arguments) at
+ * a 16-byte address, used during the call's work only and by no other work at
+ * that time; NULL where 0 bytes are needed. */
+int cq35_paged_attention_workspace(int64_t rows, int64_t requests, int32_t q_heads, int32_t kv_heads,
+                                   int32_t head_dim, int64_t max_rows, int64_t max_keys,
+                                   int64_t* bytes);
+int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_heads* q, const cq35_heads* gate,
+                         const cq35_heads* out, int64_t rows, int32_t q_heads, const int32_t* table,
+                         int64_t table_stride, int64_t requests, int64_t width,
+                         const int32_t* row_start, const int32_t* lengths, float scale,
+                         int64_t max_rows, int64_t max_keys, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
