@@ -1,5 +1,35 @@
-// Attention of new tokens over a paged KV cache.
+// Attention of new tokens over a paged KV cache, on the matrix cores: scores
+// S^T = K Q^T of 32 keys and 32 packed rows (row * group + query head), the
+// running maximum and sum of a softmax per row, O^T += V^T P^T.
+//
+// v_mfma_f32_32x32x16_bf16 (operand layouts: mfma.h) leaves the 16 scores of a
+// lane all in one row's column, so that maxima and sums are in-lane but for
+// one exchange of the two half-waves, and the weights, rounded to BF16, lie
+// where the second product takes them: register 8 s + i of half h is key
+// 16 s + 8 (i / 4) + 4 h + i % 4. V^T's operand for those keys is two
+// ds_read_b64_tr_b16, each of which hands lane j of 16 the 4 keys x 1 channel
+// that lanes 4 e .. 4 e + 3 point at as 4 channels of key e.
+//
+// Key and value tiles go straight to LDS (16 bytes a lane, no registers held)
+// in rows of head_dim, their 16-byte pieces swizzled by the row so that the 32
+// rows of a key operand and the 8 rows of a value operand spread over the
+// banks.
+//
+// The weights' rounding to BF16 (relative error 2^-9 on average half that) is
+// of the size of the values' own and an eighth of the work of F32 products;
+// the sum of the weights takes them unrounded, in F32. A row's maximum moves
+// only when it grows by more than 8 (in units of a factor 2; the first tile
+// aside): weights stay below 2^8, exact to scale in BF16 and F32, and the
+// sums are not rescaled at every tile.
+//
+// Zero weights do not hide a non-finite value of a later token from the rows
+// in front of it (0 * inf). A row whose result is NaN is therefore done again
+// with the keys behind its position left out of the tiles: only calls with
+// such values, or with NaN results, pay for it. Rows behind a request's end
+// and those of pages outside the cache are never read: zeros take their place.
 #pragma once
+
+#include <type_traits>
 
 #include "mfma.h"
 #include "paged_index.h"
@@ -14,60 +44,689 @@ struct AttendArgs {
   int64_t pages, page_stride, row_stride, head_stride;
   int shift;
   const int32_t* table;
-  int64_t table_stride, width;
+  int64_t table_stride;
   const int32_t *row_start, *lengths;
   int requests;
-  int64_t rows;
-  int q_heads, kv_heads, group;
-  float scale;
+  int64_t most_keys;  // that a table row holds
+  // |scale| log2(e): scores in units of a factor 2. The scale's sign goes into
+  // the queries' (a scale of 0: queries of 0, scaled by 1), so that masked
+  // scores of -inf stay that.
+  float scale2;
+  uint32_t q_and, q_xor;
+  CutRule cut;
+  float* part;   // slots of [group of 32 rows]: weighted sums in fragment order, then maxima, then sums
 };
 
-// One block per (row, query head); each wave every fourth key.
-constexpr int kSimpleThreads = 256;
-template <int HD>
-__global__ __launch_bounds__(kSimpleThreads) void k_paged_simple(AttendArgs a) {
-  constexpr int E = HD / 64;
-  __shared__ float ms[4], ds[4], os[4][HD];
-  const int64_t t = blockIdx.x;
-  const int head = blockIdx.y, kvh = head / a.group, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (a.row_start[0] > t) return;
-  const int r = request_of(a.row_start, a.requests, t);
-  const int64_t begin = a.row_start[r], end = a.row_start[r + 1];
-  if (t >= end) return;
-  const int64_t length = max((int64_t)0, min((int64_t)a.lengths[r], a.width << a.shift));
-  const int64_t pos = length - (end - begin) + (t - begin);
-  float q[E], o[E] = {}, m = -INFINITY, d = 0.0f;
-  for (int e = 0; e < E; ++e) q[e] = bf2f(a.q[t * a.q_row + head * a.q_head + lane + 64 * e]);
-  for (int64_t j = wave; j <= pos; j += 4) {
-    const int32_t page = a.table[r * a.table_stride + (j >> a.shift)];
-    if (page < 0 || page >= a.pages) continue;
-    const int64_t at = page * a.page_stride + (j & ((1 << a.shift) - 1)) * a.row_stride + kvh * a.head_stride + lane;
-    float s = 0.0f;
-    for (int e = 0; e < E; ++e) s = __builtin_fmaf(q[e], bf2f(a.keys[at + 64 * e]), s);
-    for (int x = 32; x; x >>= 1) s += __shfl_xor(s, x, 64);
-    s *= a.scale;
-    const float mn = fmaxf(m, s), keep = m == mn ? 1.0f : expf(m - mn), p = expf(s - mn);
-    d = d * keep + p;
-    for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(p, bf2f(a.values[at + 64 * e]), o[e] * keep);
-    m = mn;
+constexpr float kRescale = 8.0f;
+
+// ------------------------------------------------------------ finding work
+
+struct Found {
+  int32_t request, index;  // the request and the item (or row tile) inside it
+  int64_t parts_before;    // partial results of earlier requests
+  int32_t chunk;
+};
+
+// The request that holds item `at` (kTiles: row tile `at`) of the launch. Every
+// block makes the sums over all requests itself: a few KB from L2 instead of a
+// launch in front of this one.
+template <bool kTiles, int kThreads>
+__device__ bool find_work(const AttendArgs& a, uint32_t at, Found* found, CutRequest* req) {
+  constexpr int W = kThreads / 64;
+  __shared__ int64_t sums[3][W];
+  __shared__ Found hit;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = a.requests;
+  const int per = (R + kThreads - 1) / kThreads;
+  const int first = min(tid * per, R), last = min(first + per, R);
+  auto read = [&](int r) { return cut_request(a.cut, a.row_start[r], a.row_start[r + 1], a.lengths[r]); };
+  CutRequest front = {};
+  if (first < last) front = read(first);
+  auto shape = [&](int r) { return r == first ? front : read(r); };
+  int64_t pairs = 0;
+  for (int r = first; r < last; ++r) {
+    const CutRequest q = shape(r);
+    pairs += (int64_t)q.tiles * q.key_tiles;
   }
-  if (lane == 0) ms[wave] = m, ds[wave] = d;
-  for (int e = 0; e < E; ++e) os[wave][lane + 64 * e] = o[e];
+  for (int d = 1; d < 64; d <<= 1) pairs += __shfl_xor(pairs, d, 64);
+  if (lane == 0) sums[0][wave] = pairs;
+  if (tid == 0) hit.request = -1;
   __syncthreads();
-  float M = -INFINITY, D = 0.0f;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, ms[w]);
-  for (int c = threadIdx.x; c < HD; c += kSimpleThreads) {
-    float x = 0.0f;
-    D = 0.0f;
-    for (int w = 0; w < 4; ++w) {
-      if (ds[w] == 0.0f) continue;
-      const float f = expf(ms[w] - M);
-      D += ds[w] * f, x += os[w][c] * f;
-    }
-    x = D == 0.0f ? 0.0f : x / D;
-    if (a.gate) x *= 1.0f / (1.0f + expf(-bf2f(a.gate[t * a.gate_row + head * a.gate_head + c])));
-    a.out[t * a.out_row + head * a.out_head + c] = f2bf(x);
+  pairs = 0;
+  for (int w = 0; w < W; ++w) pairs += sums[0][w];
+  const int32_t chunk = cut_chunk(a.cut, pairs);
+  int64_t own[2] = {0, 0};  // items (row tiles), partial results
+  for (int r = first; r < last; ++r) {
+    const CutRequest q = shape(r);
+    const int32_t n = cut_splits(a.cut, q, chunk);
+    own[0] += kTiles ? q.tiles : (int64_t)q.tiles * n;
+    own[1] += n > 1 ? (int64_t)q.tiles * n : 0;
   }
+  int64_t upto[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int64_t x = own[i];
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(x, d, 64);
+      if (lane >= d) x += y;
+    }
+    if (lane == 63) sums[1 + i][wave] = x;
+    upto[i] = x - own[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    for (int w = 0; w < wave; ++w) upto[i] += sums[1 + i][w];
+  if (at >= upto[0] && at < upto[0] + own[0]) {
+    for (int r = first; r < last; ++r) {
+      const CutRequest q = shape(r);
+      const int32_t n = cut_splits(a.cut, q, chunk);
+      const int64_t items = kTiles ? q.tiles : (int64_t)q.tiles * n;
+      if (at < upto[0] + items) {
+        hit = {r, (int32_t)(at - upto[0]), upto[1], chunk};
+        break;
+      }
+      upto[0] += items;
+      upto[1] += n > 1 ? (int64_t)q.tiles * n : 0;
+    }
+  }
+  __syncthreads();
+  *found = hit;
+  if (found->request < 0) return false;
+  *req = read(found->request);
+  return true;
+}
+
+// ------------------------------------------------------------ tiles in LDS
+
+template <int HD>
+struct KvTile {
+  static constexpr int kRow = 2 * HD;               // bytes of a row
+  static constexpr int kBytes = kKeyTile * kRow;    // of a tile of keys, or of values
+  static constexpr int kPieces = HD / 8;            // 16-byte pieces of a row
+  static constexpr int kLoads = kBytes / 1024;      // wave-wide requests of a tile
+  static constexpr int kPer = 1024 / kRow;          // rows of a request
+  static __device__ __forceinline__ int key_swizzle(int row) { return row & (kPieces < 16 ? kPieces - 1 : 15); }
+  static __device__ __forceinline__ int value_swizzle(int row) {
+    return HD == 64 ? (row >> 1 & 1) << 2 : (row & (kPieces / 4 - 1)) << 2;
+  }
+};
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// 16 bytes per lane from `from` to LDS `to` + 16 lane. Written out because the
+// compiler would make every later LDS read wait for all of them.
+__device__ __forceinline__ void request_lds(uint32_t to, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+
+// The same from a uniform base and a lane's offset in bytes.
+__device__ __forceinline__ void request_lds(uint32_t to, const void* base, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(to), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+
+// All but the newest `n` requests of this wave have arrived.
+template <int n>
+__device__ __forceinline__ void arrived_but() {
+  static_assert(n >= 0 && n < 64, "the counter's range");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (n & 15) | ((n >> 4) << 14));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Where the 32 keys of a tile lie: two runs of 16 rows (pages hold a multiple
+// of 16), each in one page.
+struct TilePlace {
+  int64_t half[2];  // elements
+  int bad;          // bit per half: a page number outside the cache
+};
+
+__device__ __forceinline__ TilePlace place_tile(const AttendArgs& a, int request, int64_t kv_offset, int tile, int last_key) {
+  // uniform: through the scalar cache
+  typedef const __attribute__((address_space(4))) int32_t* Entry;
+  TilePlace p;
+  p.bad = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    // the second run may lie behind the last key, where the table may end
+    int key = kKeyTile * tile + 16 * h;
+    if (key > last_key) key = kKeyTile * tile;
+    const Entry e = (Entry)(uintptr_t)(a.table + request * a.table_stride + (key >> a.shift));
+    int32_t page = __builtin_amdgcn_readfirstlane(*e);
+    if (page < 0 || page >= a.pages) page = 0, p.bad |= 1 << h;
+    p.half[h] = page * a.page_stride + (key & ((1 << a.shift) - 1)) * a.row_stride + kv_offset;
+  }
+  return p;
+}
+
+// Zeros in place of rows that must not be read.
+__device__ __align__(16) uint32_t attend_zeros[4];
+
+// Requests i0 .. i0 + count - 1 of a tile of keys (or of values), zeros for
+// rows behind `last_row` of the tile and those of bad pages.
+template <int HD, bool kKeys>
+__device__ __forceinline__ void request_tile(const AttendArgs& a, const TilePlace& p, int last_row, uint32_t to, int i0,
+                                             int count) {
+  typedef KvTile<HD> T;
+  const int lane = threadIdx.x & 63, lr = lane / T::kPieces, piece = lane % T::kPieces;
+  const uint16_t* base = kKeys ? a.keys : a.values;
+  if (last_row >= 31 && !p.bad) {
+#pragma unroll
+    for (int n = 0; n < count; ++n) {
+      const int i = i0 + n, row = i * T::kPer + lr;
+      const int in = (i * T::kPer) & 15;  // the request's first row in its run of 16
+      const uint32_t off = lr * (uint32_t)a.row_stride * 2 + 16 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row)));
+      request_lds(to + 1024 * i, base + (i * T::kPer < 16 ? p.half[0] : p.half[1]) + in * a.row_stride, off);
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < count; ++n) {
+      const int i = i0 + n, row = i * T::kPer + lr;
+      const int off = 8 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row)));
+      const uint16_t* from = base + (i * T::kPer < 16 ? p.half[0] : p.half[1]) + (row & 15) * a.row_stride + off;
+      if (row > last_row || (p.bad >> (row >> 4) & 1)) from = reinterpret_cast<const uint16_t*>(attend_zeros);
+      request_lds(to + 1024 * i, from);
+    }
+  }
+}
+
+// ------------------------------------------------------------ one tile
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The other half-wave's value of the same column.
+__device__ __forceinline__ float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, x), __builtin_bit_cast(int, x), false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+  const bf16x2_t v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 read_transposed(uint32_t at) {
+  const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)at);
+  return __builtin_bit_cast(uint2, v);
+}
+
+// The state of a wave's 32 packed rows; lane l holds column l % 32, half l / 32.
+template <int HD>
+struct Rows {
+  typedef KvTile<HD> T;
+  static constexpr int kSteps = HD / 16, kChannelTiles = HD / 32, kAhead = 4;
+  u32x4 q[kSteps];
+  f32x16_t o[kChannelTiles];
+  float max, sum;  // sum: this half's keys
+  int pos;         // last key that the column sees, -1: none
+
+  // the columns are packed rows m0 ..
+  __device__ __forceinline__ void load(const AttendArgs& a, const CutRequest& r, int kvh, int m0) {
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int m = m0 + c, in = min(m, r.packed - 1);
+    const int token = (int)((uint32_t)in / (uint32_t)a.cut.group);
+    const int64_t row = r.begin + token;
+    const uint16_t* from = a.q + row * a.q_row + (kvh * a.cut.group + in - token * a.cut.group) * a.q_head + 8 * h;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) q[s] = (*reinterpret_cast<const u32x4*>(from + 16 * s) & a.q_and) ^ a.q_xor;
+    pos = m < r.packed ? visible_keys(r.lead + row, r.length) - 1 : -1;
+  }
+  __device__ __forceinline__ void clear() {
+    max = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int ct = 0; ct < kChannelTiles; ++ct) o[ct] = f32x16_t{};
+  }
+
+  __device__ __forceinline__ void scores(uint32_t keys, f32x16_t& sc) const {
+    const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+    const uint32_t at = keys + row * T::kRow + 16 * (h ^ T::key_swizzle(row));
+    auto read = [&](int s) { return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(at ^ (32 * s)); };
+    // four operands on their way: more would not fit the registers beside q and o
+    u32x4 k[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) k[s] = read(s);
+    sc = f32x16_t{};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      sc = mfma32(k[s % kAhead], q[s], sc);
+      if (s + kAhead < kSteps) k[s % kAhead] = read(s + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // Scores to weights; `first` is the tile's first key, `mask` where some of
+  // its keys are not seen by some column.
+  __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t& t, bool mask, int first, int bad, u32x4 (&w)[2]) {
+    const int h = (threadIdx.x & 63) >> 5;
+    if (mask) {
+      const int past = pos - first - 4 * h;  // keys beyond it are not seen
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) > past || (bad >> (r >> 3) & 1)) t[r] = -INFINITY;
+    }
+    float most = t[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) most = fmaxf(most, t[r]);
+    most = fmaxf(most, other_half(most)) * a.scale2;
+    if (__any(most > max + kRescale)) {
+      const float grown = fmaxf(max, most), keep = exp2_fast(max - (grown == -INFINITY ? 0.0f : grown));
+      max = grown;
+      sum *= keep;
+#pragma unroll
+      for (int ct = 0; ct < kChannelTiles; ++ct)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[ct][r] *= keep;
+    }
+    const float base = max == -INFINITY ? 0.0f : max;
+    float total = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      t[r] = exp2_fast(__builtin_fmaf(t[r], a.scale2, -base));
+      total += t[r];
+    }
+    sum += total;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[s][i] = pack_weights(t[8 * s + 2 * i], t[8 * s + 2 * i + 1]);
+  }
+
+  // o += V^T P^T.
+  __device__ __forceinline__ void context(uint32_t values, const u32x4 (&w)[2]) {
+    const int lane = threadIdx.x & 63, j = lane & 15, h = lane >> 5, upper = lane >> 4 & 1;
+    const int row = 4 * h + (j >> 2);
+    const uint32_t at = values + row * T::kRow + 16 * ((2 * upper + (j >> 1 & 1)) ^ T::value_swizzle(row)) + 8 * (j & 1);
+    // step n: channel tile n / 2, keys 16 (n % 2) ..
+    auto read = [&](int n) {
+      const uint2 x0 = read_transposed((at ^ (32 * (n & ~1))) + (16 * (n & 1)) * T::kRow);
+      const uint2 x1 = read_transposed((at ^ (32 * (n & ~1))) + (16 * (n & 1) + 8) * T::kRow);
+      return u32x4{x0.x, x0.y, x1.x, x1.y};
+    };
+    u32x4 v[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) v[n] = read(n);
+#pragma unroll
+    for (int n = 0; n < 2 * kChannelTiles; ++n) {
+      o[n >> 1] = mfma32(v[n % kAhead], w[n & 1], o[n >> 1]);
+      if (n + kAhead < 2 * kChannelTiles) v[n % kAhead] = read(n + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // Whether a result of a column that sees anything is NaN (or infinite).
+  __device__ __forceinline__ bool any_nan() const {
+    float x = 0.0f;
+#pragma unroll
+    for (int ct = 0; ct < kChannelTiles; ++ct)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x = __builtin_fmaf(o[ct][r], 0.0f, x);
+    return x != x && pos >= 0;
+  }
+};
+
+// Packed row m's results: divided by its sum, gated, rounded once.
+struct RowWriter {
+  uint16_t* out;
+  const uint16_t* gate;
+  float inverse;
+
+  __device__ __forceinline__ RowWriter(const AttendArgs& a, const CutRequest& r, int kvh, int m, float sum) {
+    const int token = (int)((uint32_t)m / (uint32_t)a.cut.group);
+    const int64_t row = r.begin + token, head = kvh * a.cut.group + m - token * a.cut.group;
+    out = a.out + row * a.out_row + head * a.out_head;
+    gate = a.gate ? a.gate + row * a.gate_row + head * a.gate_head : nullptr;
+    inverse = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+  }
+  // four channels from `ch`
+  template <bool kGate>
+  __device__ __forceinline__ void write(int ch, float x0, float x1, float x2, float x3) const {
+    float x[4] = {x0 * inverse, x1 * inverse, x2 * inverse, x3 * inverse};
+    if (kGate) {
+      const uint2 g = *reinterpret_cast<const uint2*>(gate + ch);
+      const float gv[4] = {lo2f(g.x), hi2f(g.x), lo2f(g.y), hi2f(g.y)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] *= __builtin_amdgcn_rcpf(1.0f + exp2_fast(gv[i] * -1.44269504f));
+    }
+    *reinterpret_cast<uint2*>(out + ch) = make_uint2(pack_weights(x[0], x[1]), pack_weights(x[2], x[3]));
+  }
+};
+
+// A partial result of 32 rows: o[channel tile][4 registers][lane] as float4,
+// then 32 maxima, then 32 sums.
+template <int HD>
+struct PartSlot {
+  static constexpr int kFloats = 32 * HD + 64;
+};
+
+// A block's item: a row tile of one KV head over one split of the keys.
+struct Item {
+  int request, row_tile;
+  int64_t slot;
+  int t0, t1;      // its key tiles
+  int last_key;    // that any of its rows sees
+  bool parts;      // its row tile has other splits
+};
+
+template <int kThreads>
+__device__ __forceinline__ bool find_item(const AttendArgs& a, int kvh, Item* item, CutRequest* req) {
+  Found f;
+  if (!find_work<false, kThreads>(a, blockIdx.x / (uint32_t)a.cut.kv_heads, &f, req)) return false;
+  const int splits = cut_splits(a.cut, *req, f.chunk), chunk = split_tiles(*req, splits);
+  const int nth = (int)((uint32_t)f.index / (uint32_t)splits), split = f.index - nth * splits;
+  item->request = f.request;
+  item->row_tile = req->tiles - 1 - nth;  // the last rows, which see the most keys, first
+  item->last_key = tile_keys(a.cut, *req, item->row_tile) - 1;
+  const int seen = key_tiles_of(item->last_key + 1);
+  item->parts = seen > chunk;
+  item->t0 = split * chunk;
+  item->t1 = min(item->t0 + chunk, seen);
+  if (split > 0 && item->t0 >= seen) return false;
+  item->slot = (f.parts_before + f.index) * a.cut.kv_heads + kvh;
+  return !item->parts || item->slot < a.cut.slots;
+}
+
+// Where an item's rows came out NaN it is done again up to the least position
+// among them, for the rows of that position, until none is left: a row whose
+// own pass is NaN is so from what it sees. The first pass, up to the item's
+// last key, writes every row that is not NaN.
+
+// The least position among the columns of the block for which `open` holds, or
+// INT32_MAX.
+template <int kThreads>
+__device__ __forceinline__ int least_open(bool open, int pos, int* shared) {
+  int least = open ? pos : INT32_MAX;
+  for (int d = 1; d < 64; d <<= 1) least = min(least, __shfl_xor(least, d, 64));
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = least;
+  __syncthreads();
+  for (int w = 0; w < kThreads / 64; ++w) least = min(least, shared[w]);
+  return __builtin_amdgcn_readfirstlane(least);
+}
+
+// ------------------------------------------------- few rows: keys over waves
+//
+// One item is 32 packed rows over one split of the keys; its key tiles go
+// round the four waves, each with tiles of its own in LDS and no barrier until
+// the end, where the waves' results are joined through LDS.
+constexpr int kFewThreads = 256;
+constexpr int kFewRows = 32;
+
+template <int HD>
+constexpr size_t few_lds_bytes() { return 4 * 2 * KvTile<HD>::kBytes; }
+
+template <int HD>
+__global__ __launch_bounds__(kFewThreads, 2) void k_paged_few(AttendArgs a) {
+  typedef KvTile<HD> T;
+  typedef Rows<HD> R;
+  extern __shared__ __align__(1024) uint8_t attend_lds[];
+  __shared__ float stat[2][4][32];
+  __shared__ int open_at[4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
+  Item item;
+  CutRequest req;
+  if (!find_item<kFewThreads>(a, kvh, &item, &req)) return;
+  const int m0 = kFewRows * item.row_tile;
+  const int64_t kv_offset = kvh * a.head_stride;
+  R rows;
+  rows.load(a, req, kvh, m0);
+  // up to this key every column sees all: none where a column is no row
+  const int least = m0 + kFewRows > req.packed ? -1 : visible_keys(packed_position(a.cut, req, m0), req.length) - 1;
+  const uint32_t keys = lds_address(attend_lds) + wave * 2 * T::kBytes, values = keys + T::kBytes;
+  bool open = m0 + c < req.packed;  // this column's result is not written yet
+  for (int limit = item.last_key;;) {
+    rows.clear();
+    const int t1 = min(item.t1, key_tiles_of(limit + 1)), mine = item.t0 + wave;
+    TilePlace at = {}, next = {};
+    if (mine < t1) {
+      at = place_tile(a, item.request, kv_offset, mine, limit);
+      request_tile<HD, true>(a, at, limit - kKeyTile * mine, keys, 0, T::kLoads);
+      request_tile<HD, false>(a, at, limit - kKeyTile * mine, values, 0, T::kLoads);
+    }
+#pragma unroll 1
+    for (int t = mine; t < t1; t += 4) {
+      const bool more = t + 4 < t1;
+      if (more) next = place_tile(a, item.request, kv_offset, t + 4, limit);
+      arrived_but<T::kLoads>();
+      f32x16_t sc;
+      rows.scores(keys, sc);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) request_tile<HD, true>(a, next, limit - kKeyTile * (t + 4), keys, 0, T::kLoads);
+      u32x4 w[2];
+      rows.weights(a, sc, kKeyTile * t + kKeyTile - 1 > least || at.bad, kKeyTile * t, at.bad, w);
+      if (more) arrived_but<T::kLoads>();
+      else arrived_but<0>();
+      rows.context(values, w);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) request_tile<HD, false>(a, next, limit - kKeyTile * (t + 4), values, 0, T::kLoads);
+      at = next;
+    }
+    // join the waves
+    const float total = rows.sum + other_half(rows.sum);
+    if (h == 0) stat[0][wave][c] = rows.max, stat[1][wave][c] = total;
+    __syncthreads();
+    float most = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) most = fmaxf(most, stat[0][w][c]);
+    const float base = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum += stat[1][w][c] * exp2_fast(stat[0][w][c] - base);
+    const float keep = exp2_fast(rows.max - base);
+    float4* red = reinterpret_cast<float4*>(attend_lds);  // [wave][channel tile][4 registers][lane]
+    constexpr int kQuads = R::kChannelTiles * 4;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const f32x16_t& o = rows.o[i >> 2];
+      const int r = 4 * (i & 3);
+      red[(wave * kQuads + i) * 64 + lane] = make_float4(o[r] * keep, o[r + 1] * keep, o[r + 2] * keep, o[r + 3] * keep);
+    }
+    __syncthreads();
+    float joined[kQuads / 4][4];
+    bool nan = false;
+#pragma unroll
+    for (int n = 0; n < kQuads / 4; ++n) {
+      const int i = wave + 4 * n;
+      float4 v = red[i * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        const float4 x = red[(w * kQuads + i) * 64 + lane];
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      joined[n][0] = v.x, joined[n][1] = v.y, joined[n][2] = v.z, joined[n][3] = v.w;
+      nan |= v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
+    }
+    // a column is written by all its lanes at once or not yet
+    __syncthreads();
+    if (lane < 32) stat[0][wave][c] = 0.0f;
+    if (nan) stat[0][wave][c] = 1.0f;
+    __syncthreads();
+    nan = stat[0][0][c] + stat[0][1][c] + stat[0][2][c] + stat[0][3][c] != 0.0f;
+    if (open && ((!nan && limit == item.last_key) || rows.pos == limit)) {
+      open = false;
+      if (!item.parts) {
+        const RowWriter to(a, req, kvh, m0 + c, sum);
+        auto write = [&](auto gate) {
+#pragma unroll
+          for (int n = 0; n < kQuads / 4; ++n) {
+            const int i = wave + 4 * n;
+            to.template write<decltype(gate)::value>(8 * i + 4 * h, joined[n][0], joined[n][1], joined[n][2], joined[n][3]);
+          }
+        };
+        if (a.gate) write(std::true_type{});
+        else write(std::false_type{});
+      } else {
+        float* part = a.part + item.slot * PartSlot<HD>::kFloats;
+#pragma unroll
+        for (int n = 0; n < kQuads / 4; ++n)
+          reinterpret_cast<float4*>(part)[(wave + 4 * n) * 64 + lane] = make_float4(joined[n][0], joined[n][1], joined[n][2], joined[n][3]);
+        if (wave == 0 && h == 0) part[32 * HD + c] = most, part[32 * HD + 32 + c] = sum;
+      }
+    }
+    limit = least_open<kFewThreads>(open, rows.pos, open_at);
+    if (limit == INT32_MAX) break;
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------- many rows: rows over waves
+//
+// One item is 256 packed rows over one split of the keys, 32 rows a wave, two
+// waves a SIMD: one's products run beside the other's softmax. The eight waves
+// share a ring of tiles, each wave requesting an eighth, three tiles ahead;
+// one barrier a tile.
+constexpr int kManyThreads = 512;
+constexpr int kManyRows = 256;
+constexpr int kManyStages = 4;
+
+template <int HD>
+constexpr size_t many_lds_bytes() { return kManyStages * 2 * KvTile<HD>::kBytes; }
+
+template <int HD>
+__global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
+  typedef KvTile<HD> T;
+  typedef Rows<HD> R;
+  extern __shared__ __align__(1024) uint8_t attend_lds[];
+  __shared__ int open_at[8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
+  Item item;
+  CutRequest req;
+  if (!find_item<kManyThreads>(a, kvh, &item, &req)) return;
+  const int m0 = kManyRows * item.row_tile + 32 * wave;
+  const int64_t kv_offset = kvh * a.head_stride;
+  R rows;
+  rows.load(a, req, kvh, m0);
+  const int least = m0 + 32 > req.packed ? -1 : visible_keys(packed_position(a.cut, req, m0), req.length) - 1;
+  const uint32_t ring = lds_address(attend_lds);
+  // a wave's share of a tile of keys and of values: an eighth of each, or (64
+  // channels: four requests each) a quarter of one of them
+  constexpr int kOwn = T::kLoads >= 8 ? T::kLoads / 8 : 1, kAll = T::kLoads >= 8 ? 2 * kOwn : 1;
+  bool open = m0 + c < req.packed;
+  for (int limit = item.last_key;;) {
+    rows.clear();
+    const int t1 = min(item.t1, key_tiles_of(limit + 1));
+    auto request = [&](const TilePlace& p, int t) {
+      const uint32_t to = ring + (uint32_t)((t - item.t0) % kManyStages) * 2 * T::kBytes;
+      const int last = limit - kKeyTile * t;
+      if (T::kLoads >= 8) {
+        request_tile<HD, true>(a, p, last, to, wave * kOwn, kOwn);
+        request_tile<HD, false>(a, p, last, to + T::kBytes, wave * kOwn, kOwn);
+      } else if (wave < 4) {
+        request_tile<HD, true>(a, p, last, to, wave, 1);
+      } else {
+        request_tile<HD, false>(a, p, last, to + T::kBytes, wave - 4, 1);
+      }
+    };
+    int bad = 0;  // the halves of the ring's tiles, two bits a stage
+    TilePlace next = {};
+    for (int s = 0; s < kManyStages - 1; ++s)
+      if (item.t0 + s < t1) {
+        next = place_tile(a, item.request, kv_offset, item.t0 + s, limit);
+        bad |= next.bad << (2 * s);
+        request(next, item.t0 + s);
+      }
+    if (item.t0 + kManyStages - 1 < t1) next = place_tile(a, item.request, kv_offset, item.t0 + kManyStages - 1, limit);
+#pragma unroll 1
+    for (int t = item.t0; t < t1; ++t) {
+      if (t + 2 < t1) arrived_but<2 * kAll>();
+      else if (t + 1 < t1) arrived_but<kAll>();
+      else arrived_but<0>();
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      const int stage = (t - item.t0) % kManyStages;
+      if (t + kManyStages - 1 < t1) {
+        const int ahead = (stage + kManyStages - 1) % kManyStages;
+        bad = (bad & ~(3 << (2 * ahead))) | next.bad << (2 * ahead);
+        request(next, t + kManyStages - 1);
+        if (t + kManyStages < t1) next = place_tile(a, item.request, kv_offset, t + kManyStages, limit);
+      }
+      const uint32_t keys = ring + (uint32_t)stage * 2 * T::kBytes, values = keys + T::kBytes;
+      const int gone = bad >> (2 * stage) & 3;
+      f32x16_t sc;
+      rows.scores(keys, sc);
+      u32x4 w[2];
+      rows.weights(a, sc, kKeyTile * t + kKeyTile - 1 > least || gone, kKeyTile * t, gone, w);
+      rows.context(values, w);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    bool nan = rows.any_nan();
+    nan |= __shfl_xor((int)nan, 32, 64) != 0;
+    const float sum = rows.sum + other_half(rows.sum);
+    if (open && ((!nan && limit == item.last_key) || rows.pos == limit)) {
+      open = false;
+      if (!item.parts) {
+        const RowWriter to(a, req, kvh, m0 + c, sum);
+        auto write = [&](auto gate) {
+#pragma unroll
+          for (int i = 0; i < R::kChannelTiles * 4; ++i) {
+            const f32x16_t& o = rows.o[i >> 2];
+            const int r = 4 * (i & 3);
+            to.template write<decltype(gate)::value>(8 * i + 4 * h, o[r], o[r + 1], o[r + 2], o[r + 3]);
+          }
+        };
+        if (a.gate) write(std::true_type{});
+        else write(std::false_type{});
+      } else {
+        float* part = a.part + (item.slot * (kManyRows / 32) + wave) * PartSlot<HD>::kFloats;
+#pragma unroll
+        for (int i = 0; i < R::kChannelTiles * 4; ++i) {
+          const f32x16_t& o = rows.o[i >> 2];
+          const int r = 4 * (i & 3);
+          reinterpret_cast<float4*>(part)[i * 64 + lane] = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+        }
+        if (h == 0) part[32 * HD + c] = rows.max, part[32 * HD + 32 + c] = sum;
+      }
+    }
+    limit = least_open<kManyThreads>(open, rows.pos, open_at);
+    if (limit == INT32_MAX) break;
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------- joining the splits
+//
+// Block (32 packed rows and KV head, channel tile): each thread one float4 of
+// the fragment order over all splits, weighted by 2^(max - maximum).
+constexpr int kJoinThreads = 256;
+template <int HD, int kGroups>
+__global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
+  const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
+  const uint32_t unit = blockIdx.x / (uint32_t)a.cut.kv_heads;
+  Found f;
+  CutRequest req;
+  if (!find_work<true, kJoinThreads>(a, unit / kGroups, &f, &req)) return;
+  const int splits = cut_splits(a.cut, req, f.chunk), chunk = split_tiles(req, splits);
+  const int tile = req.tiles - 1 - f.index, seen = key_tiles_of(tile_keys(a.cut, req, tile));
+  if (seen <= chunk) return;
+  const int used = (seen + chunk - 1) / chunk, group = (int)(unit % kGroups);
+  const int64_t first = (f.parts_before + (int64_t)f.index * splits) * a.cut.kv_heads + kvh;
+  if (first + (int64_t)(used - 1) * a.cut.kv_heads >= a.cut.slots) return;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, quad = 4 * blockIdx.y + (threadIdx.x >> 6);
+  const int m = a.cut.tile_rows * tile + 32 * group + c;
+  if (m >= req.packed) return;
+  auto part = [&](int s) {
+    return a.part + ((first + (int64_t)s * a.cut.kv_heads) * kGroups + group) * PartSlot<HD>::kFloats;
+  };
+  float most = -INFINITY;
+  for (int s = 0; s < used; ++s) most = fmaxf(most, part(s)[32 * HD + c]);
+  const float base = most == -INFINITY ? 0.0f : most;
+  float v[4] = {}, sum = 0.0f;
+  for (int s = 0; s < used; ++s) {
+    const float* p = part(s);
+    const float w = exp2_fast(p[32 * HD + c] - base);
+    const float4 x = reinterpret_cast<const float4*>(p)[quad * 64 + lane];
+    sum += w * p[32 * HD + 32 + c];
+    v[0] += w * x.x, v[1] += w * x.y, v[2] += w * x.z, v[3] += w * x.w;
+  }
+  const RowWriter to(a, req, kvh, m, sum);
+  if (a.gate) to.write<true>(8 * quad + 4 * h, v[0], v[1], v[2], v[3]);
+  else to.write<false>(8 * quad + 4 * h, v[0], v[1], v[2], v[3]);
 }
 
 }  // namespace cq35

@@ -61,4 +61,94 @@ CQ35_BOTH int32_t slot_of(int32_t page, int64_t pages, int64_t position, int shi
   return (int32_t)(((int64_t)page << shift) + (position & ((1 << shift) - 1)));
 }
 
+// ------------------------------------------------- how attention is cut
+//
+// A request's packed rows (row * group + query head of its KV head) are dealt
+// in tiles of `tile_rows`; the keys a tile sees are dealt in tiles of kKeyTile
+// and those in splits of equal length. How long a split is follows from all
+// requests' (row tile, key tile) pairs over the number of items wanted, so
+// that few rows over many keys fill the chip and many rows are not split.
+constexpr int kKeyTile = 32;
+
+struct CutRule {
+  int32_t rows;         // of q; rows * group is below 2^31
+  int32_t most_keys;    // that a table row holds
+  int32_t group, kv_heads, tile_rows;
+  int32_t above, upto;  // requests with more than `above` and at most `upto` packed rows are this launch's
+  int32_t target_shift; // log2 of the items wanted, over all KV heads
+  int32_t min_tiles;    // key tiles of a split at least
+  int32_t max_splits;
+  int64_t slots;        // partial results that the workspace holds
+};
+
+struct CutRequest {
+  int32_t begin, end;  // rows inside q
+  int64_t lead;        // position of row t: lead + t
+  int32_t length;
+  int32_t packed, tiles;
+  int32_t key_tiles;   // that its last row sees
+};
+
+CQ35_BOTH int32_t visible_keys(int64_t position, int32_t length) {
+  return position < 0 ? 0 : position + 1 < length ? (int32_t)(position + 1) : length;
+}
+CQ35_BOTH int32_t key_tiles_of(int32_t keys) { return (int32_t)(((uint32_t)keys + kKeyTile - 1) / kKeyTile); }
+
+CQ35_BOTH CutRequest cut_request(const CutRule& c, int32_t start, int32_t stop, int32_t length) {
+  CutRequest q;
+  q.begin = start < 0 ? 0 : start;
+  q.end = stop < c.rows ? stop : c.rows;
+  q.length = length < 0 ? 0 : length < c.most_keys ? length : c.most_keys;
+  q.lead = (int64_t)q.length - stop;
+  q.packed = q.end > q.begin ? (q.end - q.begin) * c.group : 0;
+  if (q.packed <= c.above || q.packed > c.upto) q.packed = 0;
+  q.tiles = (int32_t)(((uint32_t)q.packed + c.tile_rows - 1) / (uint32_t)c.tile_rows);
+  q.key_tiles = q.packed ? key_tiles_of(visible_keys(q.lead + q.end - 1, q.length)) : 0;
+  return q;
+}
+
+// Key tiles of a split, from the sum over the requests of tiles * key_tiles.
+CQ35_BOTH int32_t cut_chunk(const CutRule& c, int64_t pairs) {
+  const int64_t even = (pairs * c.kv_heads + ((int64_t)1 << c.target_shift) - 1) >> c.target_shift;
+  return even > INT32_MAX / 2 ? INT32_MAX / 2 : even > c.min_tiles ? (int32_t)even : c.min_tiles;
+}
+
+// Splits of a request's row tiles, and the key tiles of each.
+CQ35_BOTH int32_t cut_splits(const CutRule& c, const CutRequest& q, int32_t chunk) {
+  if (q.key_tiles <= chunk) return 1;
+  const int32_t n = (int32_t)(((uint32_t)q.key_tiles + chunk - 1) / (uint32_t)chunk);
+  return n < c.max_splits ? n : c.max_splits;
+}
+CQ35_BOTH int32_t split_tiles(const CutRequest& q, int32_t splits) {
+  return q.key_tiles ? (int32_t)(((uint32_t)q.key_tiles + splits - 1) / (uint32_t)splits) : 1;
+}
+
+// Position of packed row m of a request.
+CQ35_BOTH int64_t packed_position(const CutRule& c, const CutRequest& q, int32_t m) {
+  return q.lead + q.begin + (int32_t)((uint32_t)m / (uint32_t)c.group);
+}
+// Keys that row tile i of a request sees (its last row's).
+CQ35_BOTH int32_t tile_keys(const CutRule& c, const CutRequest& q, int32_t i) {
+  const int64_t past = (int64_t)(i + 1) * c.tile_rows;
+  return visible_keys(packed_position(c, q, (int32_t)(past < q.packed ? past : q.packed) - 1), q.length);
+}
+
+// Bounds that hold for any lengths: row tiles per KV head of a launch over
+// `rows` rows of `requests` requests, items over all KV heads (a split row
+// tile has at most 1 + key_tiles / chunk of them, and the sum of key_tiles /
+// chunk is at most target / kv_heads), partial results (at most twice that
+// sum, as only tiles of two splits or more have any).
+CQ35_BOTH int64_t most_tiles(int64_t rows, int64_t requests, int group, int tile_rows) {
+  return rows * group / tile_rows + (rows < requests ? rows : requests);
+}
+CQ35_BOTH int64_t most_items(int64_t tiles, int kv_heads, int target_shift, int max_splits) {
+  const int64_t a = tiles + ((int64_t)1 << target_shift) / kv_heads, b = tiles * max_splits;
+  return (a < b ? a : b) * kv_heads;
+}
+CQ35_BOTH int64_t most_slots(int64_t tiles, int kv_heads, int target_shift, int max_splits) {
+  if (max_splits == 1) return 0;
+  const int64_t a = (int64_t)2 << target_shift, b = tiles * max_splits * kv_heads;
+  return a < b ? a : b;
+}
+
 }  // namespace cq35

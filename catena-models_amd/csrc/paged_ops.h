@@ -116,6 +116,7 @@ int check_cache(const cq35_paged_cache* c) {
       c->head_stride % 8)
     return fail(CQ35_EINVAL, "paged cache: strides %lld, %lld, %lld are not multiples of 8 elements",
                 (long long)c->page_stride, (long long)c->row_stride, (long long)c->head_stride);
+  if (c->row_stride > 1 << 26) return fail(CQ35_EUNSUPPORTED, "paged cache: rows %lld elements apart", (long long)c->row_stride);
   if (!distinct({{c->pages, c->page_stride}, {c->page_size, c->row_stride}, {c->kv_heads, c->head_stride}}, c->head_dim))
     return fail(CQ35_EINVAL, "paged cache: pages, rows or heads overlap");
   return CQ35_OK;
@@ -210,17 +211,103 @@ extern "C" int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_head
   return launch_operator("paged prepare", kernel, grid, kPrepThreads, 0, s, a);
 }
 
+namespace {
+
+// How a call of paged attention is cut into launches. Requests of up to
+// kFewPacked packed rows (rows times query heads of a KV head) go to
+// k_paged_few, longer ones to k_paged_many; max_rows and max_keys spare a
+// launch where they say that one of them has nothing to do, and then the other
+// takes every request.
+constexpr int kFewPacked = 64;
+constexpr int kFewTarget = 10, kManyTarget = 9;  // log2 of the items wanted
+constexpr int kFewMinTiles = 8, kManyMinTiles = 16;
+constexpr int kMostSplits = 1024;
+
+struct AttendPlan {
+  bool few = false, many = false;
+  CutRule few_cut{}, many_cut{};
+  int64_t few_tiles = 0, many_tiles = 0;  // row tiles per KV head at most
+  int64_t few_floats = 0, many_floats = 0;
+};
+
+AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
+                          int64_t max_keys) {
+  AttendPlan p;
+  const int group = q_heads / kv_heads;
+  const int64_t most_rows = max_rows > 0 ? std::min(max_rows, rows) : rows;
+  p.many = most_rows * group > kFewPacked;
+  p.few = !p.many || (requests > 1 && most_rows * requests != rows);
+  auto cut = [&](CutRule* c, int tile_rows, int target, int min_tiles, int64_t* tiles, int64_t* floats) {
+    c->rows = (int32_t)rows, c->group = group, c->kv_heads = kv_heads, c->tile_rows = tile_rows;
+    c->above = 0, c->upto = INT32_MAX;
+    c->target_shift = target, c->min_tiles = min_tiles;
+    const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
+    c->max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, key_tiles / min_tiles));
+    *tiles = most_tiles(rows, requests, group, tile_rows);
+    c->slots = most_slots(*tiles, kv_heads, target, c->max_splits);
+    *floats = c->slots * (tile_rows / 32) * (32 * (int64_t)head_dim + 64);
+  };
+  if (p.few) cut(&p.few_cut, kFewRows, kFewTarget, kFewMinTiles, &p.few_tiles, &p.few_floats);
+  if (p.many) cut(&p.many_cut, kManyRows, kManyTarget, kManyMinTiles, &p.many_tiles, &p.many_floats);
+  if (p.few && p.many) p.few_cut.upto = p.many_cut.above = kFewPacked;
+  return p;
+}
+
+int check_attention_sizes(const char* what, int64_t rows, int64_t requests, int32_t q_heads, int32_t kv_heads,
+                          int32_t head_dim, int64_t max_rows, int64_t max_keys) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(CQ35_EUNSUPPORTED, "%s: head_dim %d is not 64, 128 or 256", what, head_dim);
+  if (kv_heads < 1 || kv_heads > 1024 || q_heads < 1 || q_heads > 4096 || q_heads % kv_heads)
+    return fail(CQ35_EINVAL, "%s: %d query heads over %d key/value heads", what, q_heads, kv_heads);
+  if (rows < 0 || requests < 0 || requests > INT32_MAX || max_rows < 0 || max_keys < 0 ||
+      rows > INT32_MAX / (q_heads / kv_heads))
+    return fail(CQ35_ERANGE, "%s: %lld rows of %lld requests, at most %lld rows and %lld keys each", what, (long long)rows,
+                (long long)requests, (long long)max_rows, (long long)max_keys);
+  return CQ35_OK;
+}
+
+template <int HD>
+int launch_attention(AttendArgs a, const AttendPlan& p, float* workspace, hipStream_t s) {
+  auto lds = [](const void* kernel, size_t bytes) {
+    return bytes > 65536 ? hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : hipSuccess;
+  };
+  // the first operator's grid, the join's
+  auto grids = [&](const CutRule& c, int64_t tiles, int64_t* items, int64_t* units) {
+    *items = most_items(tiles, c.kv_heads, c.target_shift, c.max_splits);
+    *units = tiles * c.kv_heads * (c.tile_rows / 32);
+    return *items <= INT32_MAX && *units <= INT32_MAX;
+  };
+  int64_t items = 0, units = 0;
+  int rc = CQ35_OK;
+  if (p.many) {
+    a.cut = p.many_cut, a.cut.most_keys = (int32_t)a.most_keys, a.part = workspace;
+    if (!grids(a.cut, p.many_tiles, &items, &units)) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
+    HIP_TRY(lds((const void*)k_paged_many<HD>, many_lds_bytes<HD>()));
+    rc = launch_operator("paged attention", k_paged_many<HD>, dim3((unsigned)items), kManyThreads, many_lds_bytes<HD>(), s, a);
+    if (!rc && a.cut.slots > 0)
+      rc = launch_operator("paged attention", k_paged_join<HD, kManyRows / 32>, dim3((unsigned)units, HD / 32), kJoinThreads, 0, s, a);
+    if (rc) return rc;
+  }
+  if (p.few) {
+    a.cut = p.few_cut, a.cut.most_keys = (int32_t)a.most_keys, a.part = workspace + p.many_floats;
+    if (!grids(a.cut, p.few_tiles, &items, &units)) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
+    HIP_TRY(lds((const void*)k_paged_few<HD>, few_lds_bytes<HD>()));
+    rc = launch_operator("paged attention", k_paged_few<HD>, dim3((unsigned)items), kFewThreads, few_lds_bytes<HD>(), s, a);
+    if (!rc && a.cut.slots > 0)
+      rc = launch_operator("paged attention", k_paged_join<HD, 1>, dim3((unsigned)units, HD / 32), kJoinThreads, 0, s, a);
+  }
+  return rc;
+}
+
+}  // namespace
+
 extern "C" int cq35_paged_attention_workspace(int64_t rows, int64_t requests, int32_t q_heads, int32_t kv_heads,
                                               int32_t head_dim, int64_t max_rows, int64_t max_keys, int64_t* bytes) {
   if (!bytes) return fail(CQ35_EINVAL, "paged attention workspace: null argument");
-  (void)max_rows, (void)max_keys;
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
-    return fail(CQ35_EUNSUPPORTED, "paged attention workspace: head_dim %d is not 64, 128 or 256", head_dim);
-  if (rows < 0 || rows > INT32_MAX || requests < 0 || requests > INT32_MAX || kv_heads < 1 || kv_heads > 1024 ||
-      q_heads < 1 || q_heads > 4096 || q_heads % kv_heads)
-    return fail(CQ35_EINVAL, "paged attention workspace: %lld rows of %lld requests, %d query heads over %d",
-                (long long)rows, (long long)requests, q_heads, kv_heads);
-  *bytes = 0;
+  const int rc = check_attention_sizes("paged attention workspace", rows, requests, q_heads, kv_heads, head_dim, max_rows, max_keys);
+  if (rc) return rc;
+  const AttendPlan p = plan_attention(rows, requests, q_heads, kv_heads, head_dim, max_rows, max_keys);
+  *bytes = (p.few_floats + p.many_floats) * (int64_t)sizeof(float);
   return CQ35_OK;
 }
 
@@ -231,12 +318,7 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
                                     void* workspace, int64_t workspace_bytes, void* stream) {
   int rc = check_cache(cache);
   if (!rc) rc = check_q_heads(cache, q_heads);
-  if (rc) return rc;
-  if (rows < 0 || rows > INT32_MAX || requests < 0 || requests > INT32_MAX || max_rows < 0 || max_keys < 0)
-    return fail(CQ35_ERANGE, "paged attention: %lld rows of %lld requests, at most %lld rows and %lld keys each",
-                (long long)rows, (long long)requests, (long long)max_rows, (long long)max_keys);
-  int64_t need = 0;
-  rc = cq35_paged_attention_workspace(rows, requests, q_heads, cache->kv_heads, cache->head_dim, max_rows, max_keys, &need);
+  if (!rc) rc = check_attention_sizes("paged attention", rows, requests, q_heads, cache->kv_heads, cache->head_dim, max_rows, max_keys);
   if (rc) return rc;
   if (rows == 0 || requests == 0) return CQ35_OK;
   if (!table || !row_start || !lengths) return fail(CQ35_EINVAL, "paged attention: null argument");
@@ -247,6 +329,9 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
   if (!rc && gate) rc = check_heads("paged attention: gate", gate, rows, q_heads, cache->head_dim, false);
   if (!rc) rc = check_heads("paged attention: output", out, rows, q_heads, cache->head_dim, true);
   if (rc) return rc;
+  const int64_t most_keys = width * cache->page_size;
+  const AttendPlan p = plan_attention(rows, requests, q_heads, cache->kv_heads, cache->head_dim, max_rows, max_keys);
+  const int64_t need = (p.few_floats + p.many_floats) * (int64_t)sizeof(float);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(CQ35_EINVAL, "paged attention: %lld bytes of workspace at a 16-byte address needed, %lld given",
                 (long long)need, (long long)(workspace ? workspace_bytes : 0));
@@ -261,9 +346,12 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
   a.out = (uint16_t*)out->data, a.out_row = out->row_stride, a.out_head = out->head_stride;
   a.keys = (const uint16_t*)cache->keys, a.values = (const uint16_t*)cache->values, a.pages = cache->pages;
   a.page_stride = cache->page_stride, a.row_stride = cache->row_stride, a.head_stride = cache->head_stride;
-  a.shift = page_shift(cache->page_size), a.table = table, a.table_stride = table_stride, a.width = width;
-  a.row_start = row_start, a.lengths = lengths, a.requests = (int)requests, a.rows = rows;
-  a.q_heads = q_heads, a.kv_heads = cache->kv_heads, a.group = q_heads / cache->kv_heads, a.scale = scale;
-  auto kernel = cache->head_dim == 256 ? k_paged_simple<256> : cache->head_dim == 128 ? k_paged_simple<128> : k_paged_simple<64>;
-  return launch_operator("paged attention", kernel, dim3((unsigned)rows, (unsigned)q_heads), kSimpleThreads, 0, s, a);
+  a.shift = page_shift(cache->page_size), a.table = table, a.table_stride = table_stride;
+  a.row_start = row_start, a.lengths = lengths, a.requests = (int)requests, a.most_keys = most_keys;
+  a.scale2 = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
+  a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
+  float* part = static_cast<float*>(workspace);
+  if (cache->head_dim == 256) return launch_attention<256>(a, p, part, s);
+  if (cache->head_dim == 128) return launch_attention<128>(a, p, part, s);
+  return launch_attention<64>(a, p, part, s);
 }

@@ -151,6 +151,7 @@ SOURCE = r"""
 #include "paged_index.h"
 #include <cstdio>
 #include <cstdlib>
+#include <vector>
 using namespace cq35;
 int main(int argc, char** argv) {
   // needs: cached length width shift ...; verdicts; requests of rows; slots
@@ -168,6 +169,46 @@ int main(int argc, char** argv) {
     } else if (what == 's') {
       scanf("%lld %lld %lld %lld", &a, &b, &c, &d);
       printf("%d\n", (int)slot_of((int32_t)a, b, c, (int)d));
+    } else if (what == 'c') {  // the cut of a launch: every (packed row, key tile) once, slots apart and within the bound
+      CutRule c{};
+      long long R;
+      scanf("%d %d %d %d %d %d %d %d %d %d", &c.rows, &c.most_keys, &c.group, &c.kv_heads, &c.tile_rows, &c.above, &c.upto,
+            &c.target_shift, &c.min_tiles, &c.max_splits);
+      scanf("%lld", &R);
+      std::vector<int32_t> start(R + 1), length(R);
+      for (auto& x : start) scanf("%d", &x);
+      for (auto& x : length) scanf("%d", &x);
+      const int64_t tiles = most_tiles(c.rows, R, c.group, c.tile_rows);
+      const int64_t items_bound = most_items(tiles, c.kv_heads, c.target_shift, c.max_splits) / c.kv_heads;
+      c.slots = most_slots(tiles, c.kv_heads, c.target_shift, c.max_splits);
+      int64_t pairs = 0, items = 0, parts = 0, tile_count = 0;
+      for (long long r = 0; r < R; ++r) {
+        const CutRequest q = cut_request(c, start[r], start[r + 1], length[r]);
+        pairs += (int64_t)q.tiles * q.key_tiles;
+      }
+      const int32_t chunk = cut_chunk(c, pairs);
+      for (long long r = 0; r < R; ++r) {
+        const CutRequest q = cut_request(c, start[r], start[r + 1], length[r]);
+        const int32_t n = cut_splits(c, q, chunk), each = split_tiles(q, n);
+        tile_count += q.tiles;
+        int64_t covered = 0, want = 0;
+        for (int32_t i = 0; i < q.tiles; ++i) {
+          const int32_t seen = key_tiles_of(tile_keys(c, q, i));
+          want += seen;
+          for (int32_t s = 0; s < n; ++s) {
+            const int32_t t0 = s * each, t1 = t0 + each < seen ? t0 + each : seen;
+            if (t1 > t0) covered += t1 - t0;
+          }
+          if (seen > each && n == 1) return 2;  // parts without a slot
+        }
+        if (covered != want || (int64_t)n * each < q.key_tiles) return 3;
+        items += (int64_t)q.tiles * n;
+        parts += n > 1 ? (int64_t)q.tiles * n : 0;
+      }
+      if (tile_count > tiles) return 4;
+      if (items > items_bound) return 5;
+      if (parts * c.kv_heads > c.slots) return 6;
+      printf("%lld %lld\n", (long long)items, (long long)parts);
     } else {
       scanf("%lld %lld", &a, &b);
       int32_t* s = (int32_t*)malloc(sizeof(int32_t) * a);
@@ -232,3 +273,28 @@ def test_request_of_row(index_program):
             lines.append("r %d %d %s" % (len(starts), t, " ".join(map(str, starts))))
             want.append([int(np.searchsorted(np.cumsum(new), t, side="right"))])
     assert ask(index_program, lines) == want
+
+
+def test_cut_covers_every_tile_once(index_program):
+    """Any lengths: each row tile's key tiles are dealt to its splits once, and
+    items and partial results stay within the bounds that size the launch and
+    the workspace (checked in the program)."""
+    rng = np.random.default_rng(3)
+    lines = []
+    for i in range(400):
+        R = int(rng.choice([1, 2, 5, 40, 300]))
+        group, kvh = int(rng.choice([1, 3, 8, 12])), int(rng.choice([1, 2, 8]))
+        new = rng.integers(0, int(rng.choice([2, 9, 600])), R)
+        length = new + rng.integers(0, int(rng.choice([1, 50, 40000])), R)
+        if i % 7 == 0:
+            length = rng.integers(-5, 100, R)  # rows that see nothing among them
+        rows = int(new.sum()) + int(rng.integers(0, 4)) - (i % 5 == 0)
+        if rows < 1:
+            continue
+        tile_rows = int(rng.choice([32, 256]))
+        above, upto = [(0, 2**31 - 1), (64, 2**31 - 1), (0, 64)][i % 3]
+        lines.append("c %d %d %d %d %d %d %d %d %d %d %d %s %s" % (
+            rows, 1 << 16, group, kvh, tile_rows, above, upto, int(rng.choice([0, 5, 9, 10])), int(rng.choice([1, 4, 16])),
+            int(rng.choice([1, 2, 7, 1024])), R, " ".join(map(str, np.concatenate([[0], np.cumsum(new)]))),
+            " ".join(map(str, length))))
+    assert len(ask(index_program, lines)) == len(lines) > 300
