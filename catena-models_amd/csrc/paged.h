@@ -160,6 +160,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
 constexpr int kPrepThreads = 256;
 constexpr int kPrepMostPairs = 128;
 constexpr int kPrepMostTokens = 8;
+constexpr int kPrepBlocks = 2048;  // eight a CU; more rows share a block's cosines
 
 struct PrepareArgs {
   const uint16_t *q, *k, *v;
@@ -191,6 +192,35 @@ __global__ __launch_bounds__(kPrepThreads) void k_paged_prepare(PrepareArgs a) {
   const int tid = threadIdx.x, c = tid % kLanes, half = a.rope_dim / 2;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int n = (int)min((int64_t)a.tokens, a.rows - t0);
+  const int heads = a.q_heads + 2 * a.kv_heads;
+  // a head of a row: read ahead of the one being worked on
+  struct Unit {
+    int t, h;
+    int32_t slot;
+    u32x4 raw;
+  };
+  auto read = [&](Unit& u) {
+    const int64_t row = t0 + u.t;
+    u.slot = a.slots[row];
+    const int g = u.h - a.q_heads;
+    const uint16_t* src = g < 0 ? a.q + row * a.q_row + u.h * a.q_head
+                          : g < a.kv_heads ? a.k + row * a.k_row + g * a.k_head
+                                           : a.v + row * a.v_row + (g - a.kv_heads) * a.v_head;
+    u.raw = *reinterpret_cast<const u32x4*>(src + 8 * c);
+  };
+  auto advance = [&](Unit& u) {
+    for (u.h += kUnits; u.h >= heads; u.h -= heads) ++u.t;
+  };
+  Unit next = {0, tid / kLanes, -1, {}};
+  for (; next.h >= heads; next.h -= heads) ++next.t;
+  if (next.t < n) read(next);
+  float wq[8], wk[8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 x = reinterpret_cast<const float4*>(a.q_weight + 8 * c)[i], y = reinterpret_cast<const float4*>(a.k_weight + 8 * c)[i];
+    wq[4 * i] = x.x, wq[4 * i + 1] = x.y, wq[4 * i + 2] = x.z, wq[4 * i + 3] = x.w;
+    wk[4 * i] = y.x, wk[4 * i + 1] = y.y, wk[4 * i + 2] = y.z, wk[4 * i + 3] = y.w;
+  }
   for (int i = tid; i < n * half; i += kPrepThreads) {
     const int t = i / half, p = i - t * half;
     const double product = (double)a.positions[a.axis[p] * a.position_stride + t0 + t] * (double)a.inv_freq[p];
@@ -201,54 +231,44 @@ __global__ __launch_bounds__(kPrepThreads) void k_paged_prepare(PrepareArgs a) {
     turn[t][p] = make_float2(co, s);
   }
   __syncthreads();
-  const int heads = a.q_heads + 2 * a.kv_heads;
-  for (int u = tid / kLanes; u < n * heads; u += kUnits) {
-    const int t = u / heads, h = u - t * heads;
-    const int64_t row = t0 + t;
-    const int32_t slot = a.slots[row];
-    if (slot < 0 || (slot >> a.shift) >= a.pages) continue;  // the same for every lane of the head
-    const int64_t cache_row = (int64_t)(slot >> a.shift) * a.page_stride + (int64_t)(slot & ((1 << a.shift) - 1)) * a.row_stride;
-    if (h >= a.q_heads + a.kv_heads) {
-      const int g = h - a.q_heads - a.kv_heads;
-      *reinterpret_cast<u32x4*>(a.values + cache_row + g * a.head_stride + 8 * c) =
-          *reinterpret_cast<const u32x4*>(a.v + row * a.v_row + g * a.v_head + 8 * c);
+  while (next.t < n) {
+    const Unit u = next;
+    advance(next);
+    if (next.t < n) read(next);
+    if (u.slot < 0 || (u.slot >> a.shift) >= a.pages) continue;  // the same for every lane of the head
+    const int64_t cache_row = (int64_t)(u.slot >> a.shift) * a.page_stride + (int64_t)(u.slot & ((1 << a.shift) - 1)) * a.row_stride + 8 * c;
+    const int g = u.h - a.q_heads;
+    if (g >= a.kv_heads) {
+      *reinterpret_cast<u32x4*>(a.values + cache_row + (g - a.kv_heads) * a.head_stride) = u.raw;
       continue;
     }
-    const bool is_q = h < a.q_heads;
-    const int g = is_q ? h : h - a.q_heads;
-    const uint16_t* src = is_q ? a.q + row * a.q_row + g * a.q_head : a.k + row * a.k_row + g * a.k_head;
-    const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 8 * c);
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = lo2f(raw[i]), x[2 * i + 1] = hi2f(raw[i]);
+    for (int i = 0; i < 4; ++i) x[2 * i] = lo2f(u.raw[i]), x[2 * i + 1] = hi2f(u.raw[i]);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
 #pragma unroll
     for (int d = 1; d < kLanes; d <<= 1) sum += __shfl_xor(sum, d, 64);
     const float inverse = 1.0f / sqrtf(sum * (1.0f / HD) + a.eps);
-    const float4* w = reinterpret_cast<const float4*>((is_q ? a.q_weight : a.k_weight) + 8 * c);
-    const float4 w0 = w[0], w1 = w[1];
-    const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * inverse * ww[i];
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * inverse * (g < 0 ? wq[i] : wk[i]);
     // the pairs' other channels lie rope_dim / 16 lanes away
-    const int away = half / 8, in_first = c < away;
-    const int partner = (tid & 63) + (in_first ? away : -away);
-    const int pl = c < 2 * away ? partner : (tid & 63);
+    const int away = half / 8, lane = tid & 63;
+    const bool front = c < away, turned = c < 2 * away;
+    const int from = turned ? (front ? lane + away : lane - away) : lane;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float o = __shfl(x[i], pl, 64);
-      if (c < 2 * away) {
-        const float2 r = turn[t][8 * (in_first ? c : c - away) + i];
-        x[i] = in_first ? x[i] * r.x - o * r.y : x[i] * r.x + o * r.y;
+      const float o = __shfl(x[i], from, 64);
+      if (turned) {
+        const float2 r = turn[u.t][8 * (front ? c : c - away) + i];
+        x[i] = front ? x[i] * r.x - o * r.y : x[i] * r.x + o * r.y;
       }
     }
     u32x4 y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = pack_bf(x[2 * i], x[2 * i + 1]);
-    uint16_t* dst = is_q ? a.out + row * a.out_row + g * a.out_head : a.keys + cache_row + g * a.head_stride;
-    *reinterpret_cast<u32x4*>(dst + 8 * c) = y;
+    *reinterpret_cast<u32x4*>(g < 0 ? a.out + (t0 + u.t) * a.out_row + u.h * a.out_head + 8 * c : a.keys + cache_row + g * a.head_stride) = y;
   }
 }
 

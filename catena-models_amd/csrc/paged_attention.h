@@ -47,7 +47,6 @@ struct AttendArgs {
   int64_t table_stride;
   const int32_t *row_start, *lengths;
   int requests;
-  int64_t most_keys;  // that a table row holds
   // |scale| log2(e): scores in units of a factor 2. The scale's sign goes into
   // the queries' (a scale of 0: queries of 0, scaled by 1), so that masked
   // scores of -inf stay that.
@@ -224,13 +223,13 @@ __device__ __forceinline__ void request_tile(const AttendArgs& a, const TilePlac
       request_lds(to + 1024 * i, base + (i * T::kPer < 16 ? p.half[0] : p.half[1]) + in * a.row_stride, off);
     }
   } else {
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < count; ++n) {
       const int i = i0 + n, row = i * T::kPer + lr;
       const int off = 8 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row)));
+      const bool none = row > last_row || (p.bad >> (row >> 4) & 1);
       const uint16_t* from = base + (i * T::kPer < 16 ? p.half[0] : p.half[1]) + (row & 15) * a.row_stride + off;
-      if (row > last_row || (p.bad >> (row >> 4) & 1)) from = reinterpret_cast<const uint16_t*>(attend_zeros);
-      request_lds(to + 1024 * i, from);
+      request_lds(to + 1024 * i, none ? reinterpret_cast<const uint16_t*>(attend_zeros) : from);
     }
   }
 }
@@ -284,6 +283,9 @@ struct Rows {
     for (int ct = 0; ct < kChannelTiles; ++ct) o[ct] = f32x16_t{};
   }
 
+  // kChains running sums over the channels, added at the end: a wave alone on
+  // its SIMD would otherwise wait for each product before the next.
+  template <int kChains>
   __device__ __forceinline__ void scores(uint32_t keys, f32x16_t& sc) const {
     const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
     const uint32_t at = keys + row * T::kRow + 16 * (h ^ T::key_swizzle(row));
@@ -292,28 +294,38 @@ struct Rows {
     u32x4 k[kAhead];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) k[s] = read(s);
-    sc = f32x16_t{};
+    f32x16_t c[kChains];
+#pragma unroll
+    for (int i = 0; i < kChains; ++i) c[i] = f32x16_t{};
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      sc = mfma32(k[s % kAhead], q[s], sc);
+      c[s % kChains] = mfma32(k[s % kAhead], q[s], c[s % kChains]);
       if (s + kAhead < kSteps) k[s % kAhead] = read(s + kAhead);
       __builtin_amdgcn_sched_barrier(0);
     }
+    sc = c[0];
+#pragma unroll
+    for (int i = 1; i < kChains; ++i) sc += c[i];
   }
 
-  // Scores to weights; `first` is the tile's first key, `mask` where some of
-  // its keys are not seen by some column.
-  __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t& t, bool mask, int first, int bad, u32x4 (&w)[2]) {
+  // Scores of N tiles to weights; `first` is the first tile's first key, `mask`
+  // where some of the keys are not seen by some column (bad: two bits a tile).
+  template <int N>
+  __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t (&t)[N], bool mask, int first, int bad, u32x4 (&w)[N][2]) {
     const int h = (threadIdx.x & 63) >> 5;
     if (mask) {
       const int past = pos - first - 4 * h;  // keys beyond it are not seen
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (8 * (r >> 2) + (r & 3) > past || (bad >> (r >> 3) & 1)) t[r] = -INFINITY;
-    }
-    float most = t[0];
+      for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int r = 1; r < 16; ++r) most = fmaxf(most, t[r]);
+        for (int r = 0; r < 16; ++r)
+          if (kKeyTile * n + 8 * (r >> 2) + (r & 3) > past || (bad >> (2 * n + (r >> 3)) & 1)) t[n][r] = -INFINITY;
+    }
+    float most = t[0][0];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, t[n][r]);
     most = fmaxf(most, other_half(most)) * a.scale2;
     if (__any(most > max + kRescale)) {
       const float grown = fmaxf(max, most), keep = exp2_fast(max - (grown == -INFINITY ? 0.0f : grown));
@@ -325,17 +337,20 @@ struct Rows {
         for (int r = 0; r < 16; ++r) o[ct][r] *= keep;
     }
     const float base = max == -INFINITY ? 0.0f : max;
-    float total = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      t[r] = exp2_fast(__builtin_fmaf(t[r], a.scale2, -base));
-      total += t[r];
+    for (int n = 0; n < N; ++n) {
+      float total = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        t[n][r] = exp2_fast(__builtin_fmaf(t[n][r], a.scale2, -base));
+        total += t[n][r];
+      }
+      sum += total;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[n][s][i] = pack_weights(t[n][8 * s + 2 * i], t[n][8 * s + 2 * i + 1]);
     }
-    sum += total;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[s][i] = pack_weights(t[8 * s + 2 * i], t[8 * s + 2 * i + 1]);
   }
 
   // o += V^T P^T.
@@ -461,7 +476,7 @@ template <int HD>
 constexpr size_t few_lds_bytes() { return 4 * 2 * KvTile<HD>::kBytes; }
 
 template <int HD>
-__global__ __launch_bounds__(kFewThreads, 2) void k_paged_few(AttendArgs a) {
+__global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(AttendArgs a) {
   typedef KvTile<HD> T;
   typedef Rows<HD> R;
   extern __shared__ __align__(1024) uint8_t attend_lds[];
@@ -494,15 +509,15 @@ __global__ __launch_bounds__(kFewThreads, 2) void k_paged_few(AttendArgs a) {
       const bool more = t + 4 < t1;
       if (more) next = place_tile(a, item.request, kv_offset, t + 4, limit);
       arrived_but<T::kLoads>();
-      f32x16_t sc;
-      rows.scores(keys, sc);
+      f32x16_t sc[1];
+      rows.template scores<2>(keys, sc[0]);
       __builtin_amdgcn_sched_barrier(0);
       if (more) request_tile<HD, true>(a, next, limit - kKeyTile * (t + 4), keys, 0, T::kLoads);
-      u32x4 w[2];
-      rows.weights(a, sc, kKeyTile * t + kKeyTile - 1 > least || at.bad, kKeyTile * t, at.bad, w);
+      u32x4 w[1][2];
+      rows.template weights<1>(a, sc, kKeyTile * t + kKeyTile - 1 > least || at.bad, kKeyTile * t, at.bad, w);
       if (more) arrived_but<T::kLoads>();
       else arrived_but<0>();
-      rows.context(values, w);
+      rows.context(values, w[0]);
       __builtin_amdgcn_sched_barrier(0);
       if (more) request_tile<HD, false>(a, next, limit - kKeyTile * (t + 4), values, 0, T::kLoads);
       at = next;
@@ -578,19 +593,23 @@ __global__ __launch_bounds__(kFewThreads, 2) void k_paged_few(AttendArgs a) {
 //
 // One item is 256 packed rows over one split of the keys, 32 rows a wave, two
 // waves a SIMD: one's products run beside the other's softmax. The eight waves
-// share a ring of tiles, each wave requesting an eighth, three tiles ahead;
-// one barrier a tile.
+// share a ring of four stages of 32 keys (of 64 for heads of up to 128
+// channels, whose tiles are short), each wave requesting an eighth, three
+// stages ahead; one barrier a stage.
 constexpr int kManyThreads = 512;
 constexpr int kManyRows = 256;
 constexpr int kManyStages = 4;
+template <int HD>
+constexpr int kStageTiles = HD == 256 ? 1 : 2;
 
 template <int HD>
-constexpr size_t many_lds_bytes() { return kManyStages * 2 * KvTile<HD>::kBytes; }
+constexpr size_t many_lds_bytes() { return kManyStages * kStageTiles<HD> * 2 * KvTile<HD>::kBytes; }
 
 template <int HD>
 __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
   typedef KvTile<HD> T;
   typedef Rows<HD> R;
+  constexpr int N = kStageTiles<HD>;
   extern __shared__ __align__(1024) uint8_t attend_lds[];
   __shared__ int open_at[8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
@@ -604,55 +623,79 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
   rows.load(a, req, kvh, m0);
   const int least = m0 + 32 > req.packed ? -1 : visible_keys(packed_position(a.cut, req, m0), req.length) - 1;
   const uint32_t ring = lds_address(attend_lds);
-  // a wave's share of a tile of keys and of values: an eighth of each, or (64
-  // channels: four requests each) a quarter of one of them
-  constexpr int kOwn = T::kLoads >= 8 ? T::kLoads / 8 : 1, kAll = T::kLoads >= 8 ? 2 * kOwn : 1;
+  // a wave's share of a stage: an eighth of each tile's keys and of its values,
+  // or (64 channels: four requests each) a quarter of either
+  constexpr int kOwn = T::kLoads >= 8 ? T::kLoads / 8 : 1, kAll = N * (T::kLoads >= 8 ? 2 * kOwn : 1);
   bool open = m0 + c < req.packed;
   for (int limit = item.last_key;;) {
     rows.clear();
-    const int t1 = min(item.t1, key_tiles_of(limit + 1));
-    auto request = [&](const TilePlace& p, int t) {
-      const uint32_t to = ring + (uint32_t)((t - item.t0) % kManyStages) * 2 * T::kBytes;
-      const int last = limit - kKeyTile * t;
-      if (T::kLoads >= 8) {
-        request_tile<HD, true>(a, p, last, to, wave * kOwn, kOwn);
-        request_tile<HD, false>(a, p, last, to + T::kBytes, wave * kOwn, kOwn);
-      } else if (wave < 4) {
-        request_tile<HD, true>(a, p, last, to, wave, 1);
-      } else {
-        request_tile<HD, false>(a, p, last, to + T::kBytes, wave - 4, 1);
+    const int t1 = min(item.t1, key_tiles_of(limit + 1)), stages = (t1 - item.t0 + N - 1) / N;
+    struct Place {
+      TilePlace tile[N];
+    };
+    auto place = [&](int i) {  // a tile behind the split's end counts as bad pages
+      Place p;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int t = item.t0 + N * i + n;
+        if (t < t1) p.tile[n] = place_tile(a, item.request, kv_offset, t, limit);
+        else p.tile[n] = {{0, 0}, 3};
+      }
+      return p;
+    };
+    auto request = [&](const Place& p, int i) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const uint32_t to = ring + (uint32_t)(i % kManyStages * N + n) * 2 * T::kBytes;
+        const int last = limit - kKeyTile * (item.t0 + N * i + n);
+        if (T::kLoads >= 8) {
+          request_tile<HD, true>(a, p.tile[n], last, to, wave * kOwn, kOwn);
+          request_tile<HD, false>(a, p.tile[n], last, to + T::kBytes, wave * kOwn, kOwn);
+        } else if (wave < 4) {
+          request_tile<HD, true>(a, p.tile[n], last, to, wave, 1);
+        } else {
+          request_tile<HD, false>(a, p.tile[n], last, to + T::kBytes, wave - 4, 1);
+        }
       }
     };
-    int bad = 0;  // the halves of the ring's tiles, two bits a stage
-    TilePlace next = {};
-    for (int s = 0; s < kManyStages - 1; ++s)
-      if (item.t0 + s < t1) {
-        next = place_tile(a, item.request, kv_offset, item.t0 + s, limit);
-        bad |= next.bad << (2 * s);
-        request(next, item.t0 + s);
+    constexpr int kBits = 2 * N;
+    auto bits = [](const Place& p) {
+      int b = 0;
+      for (int n = 0; n < N; ++n) b |= p.tile[n].bad << (2 * n);
+      return b;
+    };
+    int bad = 0;  // the halves of the ring's tiles
+    Place next = {};
+    for (int i = 0; i < kManyStages - 1; ++i)
+      if (i < stages) {
+        next = place(i);
+        bad |= bits(next) << (kBits * i);
+        request(next, i);
       }
-    if (item.t0 + kManyStages - 1 < t1) next = place_tile(a, item.request, kv_offset, item.t0 + kManyStages - 1, limit);
+    if (kManyStages - 1 < stages) next = place(kManyStages - 1);
 #pragma unroll 1
-    for (int t = item.t0; t < t1; ++t) {
-      if (t + 2 < t1) arrived_but<2 * kAll>();
-      else if (t + 1 < t1) arrived_but<kAll>();
+    for (int i = 0; i < stages; ++i) {
+      if (i + 2 < stages) arrived_but<2 * kAll>();
+      else if (i + 1 < stages) arrived_but<kAll>();
       else arrived_but<0>();
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
-      const int stage = (t - item.t0) % kManyStages;
-      if (t + kManyStages - 1 < t1) {
+      const int stage = i % kManyStages;
+      if (i + kManyStages - 1 < stages) {
         const int ahead = (stage + kManyStages - 1) % kManyStages;
-        bad = (bad & ~(3 << (2 * ahead))) | next.bad << (2 * ahead);
-        request(next, t + kManyStages - 1);
-        if (t + kManyStages < t1) next = place_tile(a, item.request, kv_offset, t + kManyStages, limit);
+        bad = (bad & ~(((1 << kBits) - 1) << (kBits * ahead))) | bits(next) << (kBits * ahead);
+        request(next, i + kManyStages - 1);
+        if (i + kManyStages < stages) next = place(i + kManyStages);
       }
-      const uint32_t keys = ring + (uint32_t)stage * 2 * T::kBytes, values = keys + T::kBytes;
-      const int gone = bad >> (2 * stage) & 3;
-      f32x16_t sc;
-      rows.scores(keys, sc);
-      u32x4 w[2];
-      rows.weights(a, sc, kKeyTile * t + kKeyTile - 1 > least || gone, kKeyTile * t, gone, w);
-      rows.context(values, w);
+      const uint32_t keys = ring + (uint32_t)(stage * N) * 2 * T::kBytes;
+      const int gone = bad >> (kBits * stage) & ((1 << kBits) - 1), first = kKeyTile * (item.t0 + N * i);
+      f32x16_t sc[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) rows.template scores<1>(keys + 2 * n * T::kBytes, sc[n]);
+      u32x4 w[N][2];
+      rows.template weights<N>(a, sc, first + kKeyTile * N - 1 > least || gone, first, gone, w);
+#pragma unroll
+      for (int n = 0; n < N; ++n) rows.context(keys + (2 * n + 1) * T::kBytes, w[n]);
       __builtin_amdgcn_sched_barrier(0);
     }
     bool nan = rows.any_nan();
@@ -692,8 +735,10 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
 // ---------------------------------------------------- joining the splits
 //
 // Block (32 packed rows and KV head, channel tile): each thread one float4 of
-// the fragment order over all splits, weighted by 2^(max - maximum).
+// the fragment order over all splits, weighted by 2^(max - maximum). The
+// weights of up to kJoinKept splits are made once, eight splits at a time.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinKept = 128;
 template <int HD, int kGroups>
 __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
   const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
@@ -704,29 +749,62 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
   const int splits = cut_splits(a.cut, req, f.chunk), chunk = split_tiles(req, splits);
   const int tile = req.tiles - 1 - f.index, seen = key_tiles_of(tile_keys(a.cut, req, tile));
   if (seen <= chunk) return;
-  const int used = (seen + chunk - 1) / chunk, group = (int)(unit % kGroups);
+  const int used = (int)((uint32_t)(seen + chunk - 1) / (uint32_t)chunk), group = (int)(unit % kGroups);
   const int64_t first = (f.parts_before + (int64_t)f.index * splits) * a.cut.kv_heads + kvh;
   if (first + (int64_t)(used - 1) * a.cut.kv_heads >= a.cut.slots) return;
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, quad = 4 * blockIdx.y + (threadIdx.x >> 6);
+  __shared__ float kept[kJoinKept][32], stat[2][8][32];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6, quad = 4 * blockIdx.y + wave;
   const int m = a.cut.tile_rows * tile + 32 * group + c;
-  if (m >= req.packed) return;
-  auto part = [&](int s) {
-    return a.part + ((first + (int64_t)s * a.cut.kv_heads) * kGroups + group) * PartSlot<HD>::kFloats;
-  };
+  const bool row = m < req.packed;
+  const int64_t step = (int64_t)a.cut.kv_heads * kGroups * PartSlot<HD>::kFloats;
+  const float* part = a.part + (first * kGroups + group) * PartSlot<HD>::kFloats;
+  auto max_of = [&](int s) { return part[s * step + 32 * HD + c]; };
+  const int eighth = 2 * wave + h;
   float most = -INFINITY;
-  for (int s = 0; s < used; ++s) most = fmaxf(most, part(s)[32 * HD + c]);
+  if (row)
+#pragma unroll 4
+    for (int s = eighth; s < used; s += 8) most = fmaxf(most, max_of(s));
+  stat[0][eighth][c] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, stat[0][i][c]);
   const float base = most == -INFINITY ? 0.0f : most;
-  float v[4] = {}, sum = 0.0f;
-  for (int s = 0; s < used; ++s) {
-    const float* p = part(s);
-    const float w = exp2_fast(p[32 * HD + c] - base);
-    const float4 x = reinterpret_cast<const float4*>(p)[quad * 64 + lane];
-    sum += w * p[32 * HD + 32 + c];
-    v[0] += w * x.x, v[1] += w * x.y, v[2] += w * x.z, v[3] += w * x.w;
-  }
+  float sum = 0.0f;
+  if (row)
+#pragma unroll 4
+    for (int s = eighth; s < used; s += 8) {
+      const float w = exp2_fast(max_of(s) - base);
+      if (s < kJoinKept) kept[s][c] = w;
+      sum = __builtin_fmaf(w, part[s * step + 32 * HD + 32 + c], sum);
+    }
+  stat[1][eighth][c] = sum;
+  __syncthreads();
+  if (!row) return;
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += stat[1][i][c];
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](auto batch) {
+    constexpr int B = decltype(batch)::value;
+    for (int s0 = 0; s0 < used; s0 += B) {
+      float4 x[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) x[i] = reinterpret_cast<const float4*>(part + min(s0 + i, used - 1) * step)[quad * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int s = s0 + i;
+        if (s >= used) break;
+        const float w = s < kJoinKept ? kept[s][c] : exp2_fast(max_of(s) - base);
+        v.x = __builtin_fmaf(w, x[i].x, v.x), v.y = __builtin_fmaf(w, x[i].y, v.y);
+        v.z = __builtin_fmaf(w, x[i].z, v.z), v.w = __builtin_fmaf(w, x[i].w, v.w);
+      }
+    }
+  };
+  if (used <= 2) add(std::integral_constant<int, 2>{});
+  else add(std::integral_constant<int, 8>{});
   const RowWriter to(a, req, kvh, m, sum);
-  if (a.gate) to.write<true>(8 * quad + 4 * h, v[0], v[1], v[2], v[3]);
-  else to.write<false>(8 * quad + 4 * h, v[0], v[1], v[2], v[3]);
+  if (a.gate) to.write<true>(8 * quad + 4 * h, v.x, v.y, v.z, v.w);
+  else to.write<false>(8 * quad + 4 * h, v.x, v.y, v.z, v.w);
 }
 
 }  // namespace cq35

@@ -74,7 +74,6 @@ struct CutRule {
   int32_t rows;         // of q; rows * group is below 2^31
   int32_t most_keys;    // that a table row holds
   int32_t group, kv_heads, tile_rows;
-  int32_t above, upto;  // requests with more than `above` and at most `upto` packed rows are this launch's
   int32_t target_shift; // log2 of the items wanted, over all KV heads
   int32_t min_tiles;    // key tiles of a split at least
   int32_t max_splits;
@@ -101,7 +100,6 @@ CQ35_BOTH CutRequest cut_request(const CutRule& c, int32_t start, int32_t stop, 
   q.length = length < 0 ? 0 : length < c.most_keys ? length : c.most_keys;
   q.lead = (int64_t)q.length - stop;
   q.packed = q.end > q.begin ? (q.end - q.begin) * c.group : 0;
-  if (q.packed <= c.above || q.packed > c.upto) q.packed = 0;
   q.tiles = (int32_t)(((uint32_t)q.packed + c.tile_rows - 1) / (uint32_t)c.tile_rows);
   q.key_tiles = q.packed ? key_tiles_of(visible_keys(q.lead + q.end - 1, q.length)) : 0;
   return q;

@@ -205,7 +205,7 @@ extern "C" int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_head
   a.rope_dim = rope_dim, a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps, a.inv_freq = inv_freq;
   a.positions = positions, a.position_stride = position_stride, a.slots = slots;
   if (pair_axis) memcpy(a.axis, pair_axis, (size_t)rope_dim / 2);
-  a.tokens = rows <= 1024 ? 1 : kPrepMostTokens;
+  a.tokens = (int)std::min<int64_t>(kPrepMostTokens, std::max<int64_t>(1, rows / kPrepBlocks));
   const dim3 grid((unsigned)((rows + a.tokens - 1) / a.tokens));
   auto kernel = cache->head_dim == 256 ? k_paged_prepare<256> : cache->head_dim == 128 ? k_paged_prepare<128> : k_paged_prepare<64>;
   return launch_operator("paged prepare", kernel, grid, kPrepThreads, 0, s, a);
@@ -213,43 +213,35 @@ extern "C" int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_head
 
 namespace {
 
-// How a call of paged attention is cut into launches. Requests of up to
-// kFewPacked packed rows (rows times query heads of a KV head) go to
-// k_paged_few, longer ones to k_paged_many; max_rows and max_keys spare a
-// launch where they say that one of them has nothing to do, and then the other
-// takes every request.
+// How a call of paged attention is cut: requests of up to kFewPacked packed
+// rows (rows times query heads of a KV head) go to k_paged_few, one longer
+// request takes them all to k_paged_many. max_rows decides without the lengths,
+// max_keys spares the join where no request can be split.
 constexpr int kFewPacked = 64;
-constexpr int kFewTarget = 10, kManyTarget = 9;  // log2 of the items wanted
-constexpr int kFewMinTiles = 8, kManyMinTiles = 16;
+constexpr int kFewTarget = 9, kManyTarget = 9;  // log2 of the items wanted
+constexpr int kFewMinTiles = 4, kManyMinTiles = 16;
 constexpr int kMostSplits = 1024;
 
 struct AttendPlan {
-  bool few = false, many = false;
-  CutRule few_cut{}, many_cut{};
-  int64_t few_tiles = 0, many_tiles = 0;  // row tiles per KV head at most
-  int64_t few_floats = 0, many_floats = 0;
+  bool few;
+  CutRule cut;
+  int64_t tiles;   // row tiles per KV head at most
+  int64_t floats;  // of workspace
 };
 
 AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
                           int64_t max_keys) {
-  AttendPlan p;
+  AttendPlan p{};
   const int group = q_heads / kv_heads;
-  const int64_t most_rows = max_rows > 0 ? std::min(max_rows, rows) : rows;
-  p.many = most_rows * group > kFewPacked;
-  p.few = !p.many || (requests > 1 && most_rows * requests != rows);
-  auto cut = [&](CutRule* c, int tile_rows, int target, int min_tiles, int64_t* tiles, int64_t* floats) {
-    c->rows = (int32_t)rows, c->group = group, c->kv_heads = kv_heads, c->tile_rows = tile_rows;
-    c->above = 0, c->upto = INT32_MAX;
-    c->target_shift = target, c->min_tiles = min_tiles;
-    const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
-    c->max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, key_tiles / min_tiles));
-    *tiles = most_tiles(rows, requests, group, tile_rows);
-    c->slots = most_slots(*tiles, kv_heads, target, c->max_splits);
-    *floats = c->slots * (tile_rows / 32) * (32 * (int64_t)head_dim + 64);
-  };
-  if (p.few) cut(&p.few_cut, kFewRows, kFewTarget, kFewMinTiles, &p.few_tiles, &p.few_floats);
-  if (p.many) cut(&p.many_cut, kManyRows, kManyTarget, kManyMinTiles, &p.many_tiles, &p.many_floats);
-  if (p.few && p.many) p.few_cut.upto = p.many_cut.above = kFewPacked;
+  p.few = (max_rows > 0 ? std::min(max_rows, rows) : rows) * group <= kFewPacked;
+  CutRule& c = p.cut;
+  c.rows = (int32_t)rows, c.group = group, c.kv_heads = kv_heads, c.tile_rows = p.few ? kFewRows : kManyRows;
+  c.target_shift = p.few ? kFewTarget : kManyTarget, c.min_tiles = p.few ? kFewMinTiles : kManyMinTiles;
+  const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
+  c.max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, (key_tiles + c.min_tiles - 1) / c.min_tiles));
+  p.tiles = most_tiles(rows, requests, group, c.tile_rows);
+  c.slots = most_slots(p.tiles, kv_heads, c.target_shift, c.max_splits);
+  p.floats = c.slots * (c.tile_rows / 32) * (32 * (int64_t)head_dim + 64);
   return p;
 }
 
@@ -267,35 +259,17 @@ int check_attention_sizes(const char* what, int64_t rows, int64_t requests, int3
 }
 
 template <int HD>
-int launch_attention(AttendArgs a, const AttendPlan& p, float* workspace, hipStream_t s) {
-  auto lds = [](const void* kernel, size_t bytes) {
-    return bytes > 65536 ? hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : hipSuccess;
-  };
-  // the first operator's grid, the join's
-  auto grids = [&](const CutRule& c, int64_t tiles, int64_t* items, int64_t* units) {
-    *items = most_items(tiles, c.kv_heads, c.target_shift, c.max_splits);
-    *units = tiles * c.kv_heads * (c.tile_rows / 32);
-    return *items <= INT32_MAX && *units <= INT32_MAX;
-  };
-  int64_t items = 0, units = 0;
-  int rc = CQ35_OK;
-  if (p.many) {
-    a.cut = p.many_cut, a.cut.most_keys = (int32_t)a.most_keys, a.part = workspace;
-    if (!grids(a.cut, p.many_tiles, &items, &units)) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
-    HIP_TRY(lds((const void*)k_paged_many<HD>, many_lds_bytes<HD>()));
-    rc = launch_operator("paged attention", k_paged_many<HD>, dim3((unsigned)items), kManyThreads, many_lds_bytes<HD>(), s, a);
-    if (!rc && a.cut.slots > 0)
-      rc = launch_operator("paged attention", k_paged_join<HD, kManyRows / 32>, dim3((unsigned)units, HD / 32), kJoinThreads, 0, s, a);
-    if (rc) return rc;
-  }
-  if (p.few) {
-    a.cut = p.few_cut, a.cut.most_keys = (int32_t)a.most_keys, a.part = workspace + p.many_floats;
-    if (!grids(a.cut, p.few_tiles, &items, &units)) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
-    HIP_TRY(lds((const void*)k_paged_few<HD>, few_lds_bytes<HD>()));
-    rc = launch_operator("paged attention", k_paged_few<HD>, dim3((unsigned)items), kFewThreads, few_lds_bytes<HD>(), s, a);
-    if (!rc && a.cut.slots > 0)
-      rc = launch_operator("paged attention", k_paged_join<HD, 1>, dim3((unsigned)units, HD / 32), kJoinThreads, 0, s, a);
-  }
+int launch_attention(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
+  const int64_t items = most_items(p.tiles, a.cut.kv_heads, a.cut.target_shift, a.cut.max_splits);
+  const int64_t units = p.tiles * a.cut.kv_heads * (a.cut.tile_rows / 32);
+  if (items > INT32_MAX || units > INT32_MAX) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
+  auto kernel = p.few ? k_paged_few<HD> : k_paged_many<HD>;
+  auto join = p.few ? k_paged_join<HD, 1> : k_paged_join<HD, kManyRows / 32>;
+  const size_t lds = p.few ? few_lds_bytes<HD>() : many_lds_bytes<HD>();
+  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  int rc = launch_operator("paged attention", kernel, dim3((unsigned)items), p.few ? kFewThreads : kManyThreads, lds, s, a);
+  if (!rc && a.cut.slots > 0)
+    rc = launch_operator("paged attention", join, dim3((unsigned)units, HD / 32), kJoinThreads, 0, s, a);
   return rc;
 }
 
@@ -307,7 +281,7 @@ extern "C" int cq35_paged_attention_workspace(int64_t rows, int64_t requests, in
   const int rc = check_attention_sizes("paged attention workspace", rows, requests, q_heads, kv_heads, head_dim, max_rows, max_keys);
   if (rc) return rc;
   const AttendPlan p = plan_attention(rows, requests, q_heads, kv_heads, head_dim, max_rows, max_keys);
-  *bytes = (p.few_floats + p.many_floats) * (int64_t)sizeof(float);
+  *bytes = p.floats * (int64_t)sizeof(float);
   return CQ35_OK;
 }
 
@@ -329,9 +303,8 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
   if (!rc && gate) rc = check_heads("paged attention: gate", gate, rows, q_heads, cache->head_dim, false);
   if (!rc) rc = check_heads("paged attention: output", out, rows, q_heads, cache->head_dim, true);
   if (rc) return rc;
-  const int64_t most_keys = width * cache->page_size;
   const AttendPlan p = plan_attention(rows, requests, q_heads, cache->kv_heads, cache->head_dim, max_rows, max_keys);
-  const int64_t need = (p.few_floats + p.many_floats) * (int64_t)sizeof(float);
+  const int64_t need = p.floats * (int64_t)sizeof(float);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(CQ35_EINVAL, "paged attention: %lld bytes of workspace at a 16-byte address needed, %lld given",
                 (long long)need, (long long)(workspace ? workspace_bytes : 0));
@@ -347,11 +320,11 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
   a.keys = (const uint16_t*)cache->keys, a.values = (const uint16_t*)cache->values, a.pages = cache->pages;
   a.page_stride = cache->page_stride, a.row_stride = cache->row_stride, a.head_stride = cache->head_stride;
   a.shift = page_shift(cache->page_size), a.table = table, a.table_stride = table_stride;
-  a.row_start = row_start, a.lengths = lengths, a.requests = (int)requests, a.most_keys = most_keys;
+  a.row_start = row_start, a.lengths = lengths, a.requests = (int)requests;
+  a.cut = p.cut, a.cut.most_keys = (int32_t)(width * cache->page_size), a.part = static_cast<float*>(workspace);
   a.scale2 = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
   a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
-  float* part = static_cast<float*>(workspace);
-  if (cache->head_dim == 256) return launch_attention<256>(a, p, part, s);
-  if (cache->head_dim == 128) return launch_attention<128>(a, p, part, s);
-  return launch_attention<64>(a, p, part, s);
+  if (cache->head_dim == 256) return launch_attention<256>(a, p, s);
+  if (cache->head_dim == 128) return launch_attention<128>(a, p, s);
+  return launch_attention<64>(a, p, s);
 }

@@ -172,8 +172,8 @@ int main(int argc, char** argv) {
     } else if (what == 'c') {  // the cut of a launch: every (packed row, key tile) once, slots apart and within the bound
       CutRule c{};
       long long R;
-      scanf("%d %d %d %d %d %d %d %d %d %d", &c.rows, &c.most_keys, &c.group, &c.kv_heads, &c.tile_rows, &c.above, &c.upto,
-            &c.target_shift, &c.min_tiles, &c.max_splits);
+      scanf("%d %d %d %d %d %d %d %d", &c.rows, &c.most_keys, &c.group, &c.kv_heads, &c.tile_rows, &c.target_shift,
+             &c.min_tiles, &c.max_splits);
       scanf("%lld", &R);
       std::vector<int32_t> start(R + 1), length(R);
       for (auto& x : start) scanf("%d", &x);
@@ -292,9 +292,8 @@ def test_cut_covers_every_tile_once(index_program):
         if rows < 1:
             continue
         tile_rows = int(rng.choice([32, 256]))
-        above, upto = [(0, 2**31 - 1), (64, 2**31 - 1), (0, 64)][i % 3]
-        lines.append("c %d %d %d %d %d %d %d %d %d %d %d %s %s" % (
-            rows, 1 << 16, group, kvh, tile_rows, above, upto, int(rng.choice([0, 5, 9, 10])), int(rng.choice([1, 4, 16])),
+        lines.append("c %d %d %d %d %d %d %d %d %d %s %s" % (
+            rows, 1 << 16, group, kvh, tile_rows, int(rng.choice([0, 5, 9, 10])), int(rng.choice([1, 4, 16])),
             int(rng.choice([1, 2, 7, 1024])), R, " ".join(map(str, np.concatenate([[0], np.cumsum(new)]))),
             " ".join(map(str, length))))
     assert len(ask(index_program, lines)) == len(lines) > 300
