@@ -26,5 +26,6 @@ __all__ += _PAGED
 def __getattr__(name):
     if name in _PAGED:
         from . import paged
-        return getattr(paged, name)
+        globals().update((n, getattr(paged, n)) for n in _PAGED)
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

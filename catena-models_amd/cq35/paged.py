@@ -11,6 +11,7 @@ strides included, head_dim contiguous).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import NamedTuple
 
@@ -31,66 +32,77 @@ class PagePlan(NamedTuple):
 PLAN_STATUS = ("ok", "too few free pages", "too few rows", "lengths outside the tables", "malformed stack of free pages")
 
 
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+
+
 def _tensor(name, t, dtype, dim, device=None):
+    """`t` as it should be, or why not: the checks are cheap (a few tenths of a
+    microsecond) beside the call's launch, the reasons are looked for after."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
+    if t.dtype is dtype and t.dim() == dim and (t.is_cuda if device is None else t.device == device):
+        return t
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
     if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimensions, not {t.dim()}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not {device}")
-    return t
+    raise ValueError(f"{name} is on {t.device}, not {device}")
 
 
 def _flat(name, t, dtype, count, device):
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (count,) and t.device == device and t.is_contiguous():
+        return t.data_ptr()
     _tensor(name, t, dtype, 1, device)
     if t.shape[0] != count:
         raise ValueError(f"{name} must have {count} entries, not {t.shape[0]}")
-    if count > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name} must be contiguous")
-    return t
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _stream(device, stream):
-    s = torch.cuda.current_stream(device) if stream is None else stream
-    if s.device != device:
-        raise ValueError(f"the stream is {s.device}'s, the tensors {device}'s")
-    return s
+    """The raw stream of a call, and what its new tensors are made under."""
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream, _HERE
+    if stream.device != device:
+        raise ValueError(f"the stream is {stream.device}'s, the tensors {device}'s")
+    return stream.cuda_stream, torch.cuda.stream(stream)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _heads(name, t, rows, heads, head_dim, device):
-    _tensor(name, t, torch.bfloat16, 3, device)
-    if tuple(t.shape) != (rows, heads, head_dim):
+    _tensor(name, t, _BF16, 3, device)
+    if t.shape != (rows, heads, head_dim):
         raise ValueError(f"{name} must be {(rows, heads, head_dim)}, not {tuple(t.shape)}")
-    if t.stride(2) != 1:
+    row, head, channel = t.stride()
+    if channel != 1:
         raise ValueError(f"{name}: the channels of a head must be contiguous")
     # the stride of a dimension of length one addresses nothing
-    return _lib.Heads(t.data_ptr(), t.stride(0) if rows > 1 else 0, t.stride(1) if heads > 1 else 0)
+    return _lib.Heads(t.data_ptr(), row if rows > 1 else 0, head if heads > 1 else 0)
 
 
 def _cache(key_cache, value_cache):
-    _tensor("key_cache", key_cache, torch.bfloat16, 4)
-    _tensor("value_cache", value_cache, torch.bfloat16, 4, key_cache.device)
-    if key_cache.shape != value_cache.shape:
-        raise ValueError(f"key_cache {tuple(key_cache.shape)} and value_cache {tuple(value_cache.shape)} differ")
-    if 0 in key_cache.shape:
+    _tensor("key_cache", key_cache, _BF16, 4)
+    _tensor("value_cache", value_cache, _BF16, 4, key_cache.device)
+    shape = key_cache.shape
+    if shape != value_cache.shape:
+        raise ValueError(f"key_cache {tuple(shape)} and value_cache {tuple(value_cache.shape)} differ")
+    if 0 in shape:
         raise ValueError("an empty cache")
-    strides = []
-    for i in range(3):
-        if key_cache.shape[i] > 1 and key_cache.stride(i) != value_cache.stride(i):
-            raise ValueError("key_cache and value_cache have different strides")
-        strides.append(key_cache.stride(i) if key_cache.shape[i] > 1 else 0)
-    if key_cache.stride(3) != 1 or value_cache.stride(3) != 1:
+    ks, vs = key_cache.stride(), value_cache.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the channels of a cached head must be contiguous")
-    pages, page_size, kv_heads, head_dim = key_cache.shape
+    strides = [k if n > 1 else 0 for n, k in zip(shape[:3], ks)]
+    if ks != vs and strides != [v if n > 1 else 0 for n, v in zip(shape[:3], vs)]:
+        raise ValueError("key_cache and value_cache have different strides")
+    pages, page_size, kv_heads, head_dim = shape
     return _lib.PagedCache(key_cache.data_ptr(), value_cache.data_ptr(), pages, page_size, kv_heads, head_dim, *strides)
 
 
 def _table(table, requests, device):
-    _tensor("table", table, torch.int32, 2, device)
+    _tensor("table", table, _I32, 2, device)
     if requests is not None and table.shape[0] != requests:
         raise ValueError(f"table must have {requests} rows, not {table.shape[0]}")
     if table.shape[1] > 1 and table.stride(1) != 1:
@@ -108,30 +120,26 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     earlier plan's tensors to write to. `status` is for the caller to look at
     when it next waits for the GPU: unless status[0] is 0 (PLAN_STATUS), nothing
     was changed and the round has no rows."""
-    device = _tensor("table", table, torch.int32, 2).device
-    requests = table.shape[0]
+    device = _tensor("table", table, _I32, 2).device
+    requests, width = table.shape
     stride = _table(table, None, device)
-    _flat("cached", cached, torch.int32, requests, device)
-    _flat("lengths", lengths, torch.int32, requests, device)
-    _tensor("free_pages", free_pages, torch.int32, 1, device)
-    _flat("free_pages", free_pages, torch.int32, free_pages.shape[0], device)
-    _flat("free_count", free_count, torch.int32, 1, device)
+    cached, lengths = _flat("cached", cached, _I32, requests, device), _flat("lengths", lengths, _I32, requests, device)
+    pages = _tensor("free_pages", free_pages, _I32, 1, device).shape[0]
+    free_pages = _flat("free_pages", free_pages, _I32, pages, device)
+    free_count = _flat("free_count", free_count, _I32, 1, device)
     rows = int(rows)
     if rows < 0:
         raise ValueError(f"rows must not be negative: {rows}")
-    s = _stream(device, stream)
+    raw, under = _stream(device, stream)
+    sizes = (requests + 1, rows, rows, 1, 2)
     if out is None:
-        with torch.cuda.stream(s):
-            sizes = (requests + 1, rows, rows, 1, 2)
-            whole = torch.empty(sum(sizes), dtype=torch.int32, device=device)
-            out = PagePlan(*whole.split(sizes))
+        with under:
+            out = PagePlan(*torch.empty(requests + 2 * rows + 4, dtype=_I32, device=device).split_with_sizes(sizes))
+        at = [t.data_ptr() for t in out]
     else:
-        for name, t, n in zip(PagePlan._fields, out, (requests + 1, rows, rows, 1, 2)):
-            _flat("out." + name, t, torch.int32, n, device)
-    check(_lib.load().cq35_page_plan(
-        table.data_ptr(), stride, requests, table.shape[1], cached.data_ptr(), lengths.data_ptr(),
-        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, rows, out.row_start.data_ptr(),
-        out.positions.data_ptr(), out.slots.data_ptr(), out.free_left.data_ptr(), out.status.data_ptr(), s.cuda_stream))
+        at = [_flat("out." + name, t, _I32, n, device) for name, t, n in zip(PagePlan._fields, out, sizes)]
+    check(_lib.load().cq35_page_plan(table.data_ptr(), stride, requests, width, cached, lengths, free_pages, pages, free_count,
+                                     page_size, rows, *at, raw))
     return out
 
 
@@ -147,38 +155,32 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
     tensor for the queries, q itself allowed."""
     cache = _cache(key_cache, value_cache)
     device = key_cache.device
-    _tensor("q", q, torch.bfloat16, 3, device)
-    rows, q_heads = q.shape[0], q.shape[1]
+    _tensor("q", q, _BF16, 3, device)
+    rows, q_heads = q.shape[:2]
     if q_heads == 0:
         raise ValueError("q has no heads")
     hq = _heads("q", q, rows, q_heads, cache.head_dim, device)
     hk = _heads("k", k, rows, cache.kv_heads, cache.head_dim, device)
     hv = _heads("v", v, rows, cache.kv_heads, cache.head_dim, device)
-    _flat("q_weight", q_weight, torch.float32, cache.head_dim, device)
-    _flat("k_weight", k_weight, torch.float32, cache.head_dim, device)
-    _tensor("inv_freq", inv_freq, torch.float32, 1, device)
-    pairs = inv_freq.shape[0]
-    _flat("inv_freq", inv_freq, torch.float32, pairs, device)
-    if positions.dim() == 1:
-        positions = positions.unsqueeze(0)
-    _tensor("positions", positions, torch.int32, 2, device)
-    axes = positions.shape[0]
-    if positions.shape[1] != rows or (rows > 1 and positions.stride(1) != 1):
+    q_weight, k_weight = (_flat(n, w, _F32, cache.head_dim, device) for n, w in (("q_weight", q_weight), ("k_weight", k_weight)))
+    pairs = _tensor("inv_freq", inv_freq, _F32, 1, device).shape[0]
+    inv_freq = _flat("inv_freq", inv_freq, _F32, pairs, device)
+    dims = _tensor("positions", positions, _I32, min(max(positions.dim(), 1), 2), device).dim()
+    axes, axis_stride = (1, rows) if dims == 1 else (positions.shape[0], positions.stride(0))
+    if positions.shape[-1] != rows or (rows > 1 and positions.stride(-1) != 1):
         raise ValueError(f"positions must be [axes, {rows}] with contiguous rows, not {tuple(positions.shape)}")
-    _flat("slots", slots, torch.int32, rows, device)
+    slots = _flat("slots", slots, _I32, rows, device)
     if pair_axis is not None:
         if len(pair_axis) != pairs or not all(0 <= int(x) < axes for x in pair_axis):
             raise ValueError(f"pair_axis must name one of {axes} axes for each of {pairs} pairs")
         pair_axis = (ctypes.c_uint8 * pairs)(*[int(x) for x in pair_axis])
-    s = _stream(device, stream)
+    raw, under = _stream(device, stream)
     if out is None:
-        with torch.cuda.stream(s):
-            out = torch.empty((rows, q_heads, cache.head_dim), dtype=torch.bfloat16, device=device)
+        with under:
+            out = torch.empty((rows, q_heads, cache.head_dim), dtype=_BF16, device=device)
     ho = _heads("out", out, rows, q_heads, cache.head_dim, device)
-    check(_lib.load().cq35_paged_prepare(
-        ctypes.byref(cache), ctypes.byref(hq), ctypes.byref(hk), ctypes.byref(hv), rows, q_heads, q_weight.data_ptr(),
-        k_weight.data_ptr(), eps, inv_freq.data_ptr(), 2 * pairs, positions.data_ptr(),
-        positions.stride(0) if axes > 1 else rows, axes, pair_axis, slots.data_ptr(), ctypes.byref(ho), s.cuda_stream))
+    check(_lib.load().cq35_paged_prepare(cache, hq, hk, hv, rows, q_heads, q_weight, k_weight, eps, inv_freq, 2 * pairs,
+                                         positions.data_ptr(), axis_stride, axes, pair_axis, slots, ho, raw))
     return out
 
 
@@ -196,33 +198,34 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
     other work at the time, by default allocated for the call."""
     cache = _cache(key_cache, value_cache)
     device = key_cache.device
-    _tensor("q", q, torch.bfloat16, 3, device)
-    rows, q_heads = q.shape[0], q.shape[1]
+    _tensor("q", q, _BF16, 3, device)
+    rows, q_heads = q.shape[:2]
     if q_heads == 0:
         raise ValueError("q has no heads")
     hq = _heads("q", q, rows, q_heads, cache.head_dim, device)
     hg = None if gate is None else _heads("gate", gate, rows, q_heads, cache.head_dim, device)
-    requests = _tensor("lengths", lengths, torch.int32, 1, device).shape[0]
-    _flat("lengths", lengths, torch.int32, requests, device)
-    _flat("row_start", row_start, torch.int32, requests + 1, device)
+    requests = _tensor("lengths", lengths, _I32, 1, device).shape[0]
+    lengths = _flat("lengths", lengths, _I32, requests, device)
+    row_start = _flat("row_start", row_start, _I32, requests + 1, device)
     stride = _table(table, requests, device)
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
     max_rows, max_keys = int(max_rows), int(max_keys)
-    s = _stream(device, stream)
-    need = paged_attention_workspace(rows, requests, q_heads, cache.kv_heads, cache.head_dim, max_rows, max_keys)
+    raw, under = _stream(device, stream)
+    have = at = None
     if workspace is not None:
-        _flat("workspace", workspace, torch.uint8, workspace.shape[0] if workspace.dim() == 1 else -1, device)
-    with torch.cuda.stream(s):
-        if workspace is None and need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        have = workspace.shape[0] if workspace.dim() == 1 else -1
+        at = _flat("workspace", workspace, torch.uint8, have, device)
+    with under:
+        if workspace is None:
+            have = paged_attention_workspace(rows, requests, q_heads, cache.kv_heads, cache.head_dim, max_rows, max_keys)
+            if have:
+                workspace = torch.empty(have, dtype=torch.uint8, device=device)
+                at = workspace.data_ptr()
         if out is None:
-            out = torch.empty((rows, q_heads, cache.head_dim), dtype=torch.bfloat16, device=device)
+            out = torch.empty((rows, q_heads, cache.head_dim), dtype=_BF16, device=device)
     ho = _heads("out", out, rows, q_heads, cache.head_dim, device)
-    check(_lib.load().cq35_paged_attention(
-        ctypes.byref(cache), ctypes.byref(hq), None if hg is None else ctypes.byref(hg), ctypes.byref(ho), rows, q_heads,
-        table.data_ptr(), stride, requests, table.shape[1], row_start.data_ptr(), lengths.data_ptr(), scale, max_rows,
-        max_keys, None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.shape[0],
-        s.cuda_stream))
+    check(_lib.load().cq35_paged_attention(cache, hq, hg, ho, rows, q_heads, table.data_ptr(), stride, requests, table.shape[1],
+                                           row_start, lengths, scale, max_rows, max_keys, at, have, raw))
     return out
 
 

@@ -66,72 +66,98 @@ struct Found {
   int32_t chunk;
 };
 
-// The request that holds item `at` (kTiles: row tile `at`) of the launch. Every
-// block makes the sums over all requests itself: a few KB from L2 instead of a
-// launch in front of this one.
+// Inclusive sums over the lanes of a wave (rows of 16 by shifts, then the rows'
+// ends handed on); every lane active.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int64_t lanes_moved(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kCtrl, kRows, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)x >> 32), kCtrl, kRows, 0xf, false);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t wave_sums(int64_t x) {
+  x += lanes_moved<0x111, 0xf>(x);  // row_shr:1
+  x += lanes_moved<0x112, 0xf>(x);
+  x += lanes_moved<0x114, 0xf>(x);
+  x += lanes_moved<0x118, 0xf>(x);
+  x += lanes_moved<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x += lanes_moved<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The request that holds item `at` (kTiles: row tile `at`) of the launch, in
+// uniform registers. Every block makes the sums over all requests itself, 64
+// of them in the lanes of a wave: up to 64 requests without a barrier (a
+// decode item of 16 keys would otherwise wait for three), and no launch in
+// front of this one.
+constexpr int kAttendMostRequests = 8192;
 template <bool kTiles, int kThreads>
-__device__ bool find_work(const AttendArgs& a, uint32_t at, Found* found, CutRequest* req) {
-  constexpr int W = kThreads / 64;
-  __shared__ int64_t sums[3][W];
-  __shared__ Found hit;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = a.requests;
-  const int per = (R + kThreads - 1) / kThreads;
-  const int first = min(tid * per, R), last = min(first + per, R);
-  auto read = [&](int r) { return cut_request(a.cut, a.row_start[r], a.row_start[r + 1], a.lengths[r]); };
-  CutRequest front = {};
-  if (first < last) front = read(first);
-  auto shape = [&](int r) { return r == first ? front : read(r); };
-  int64_t pairs = 0;
-  for (int r = first; r < last; ++r) {
-    const CutRequest q = shape(r);
-    pairs += (int64_t)q.tiles * q.key_tiles;
-  }
-  for (int d = 1; d < 64; d <<= 1) pairs += __shfl_xor(pairs, d, 64);
-  if (lane == 0) sums[0][wave] = pairs;
-  if (tid == 0) hit.request = -1;
-  __syncthreads();
-  pairs = 0;
-  for (int w = 0; w < W; ++w) pairs += sums[0][w];
-  const int32_t chunk = cut_chunk(a.cut, pairs);
-  int64_t own[2] = {0, 0};  // items (row tiles), partial results
-  for (int r = first; r < last; ++r) {
-    const CutRequest q = shape(r);
-    const int32_t n = cut_splits(a.cut, q, chunk);
-    own[0] += kTiles ? q.tiles : (int64_t)q.tiles * n;
-    own[1] += n > 1 ? (int64_t)q.tiles * n : 0;
-  }
-  int64_t upto[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    int64_t x = own[i];
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
+__device__ __forceinline__ bool find_work(const AttendArgs& a, uint32_t at, Found* found, CutRequest* req) {
+  constexpr int W = kThreads / 64, kSlices = kAttendMostRequests / 64;
+  __shared__ int64_t sums[3][kSlices];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, R = a.requests, slices = (R + 63) / 64;
+  auto shape = [&](int slice) {
+    const int r = 64 * slice + lane;
+    CutRequest q = {};
+    if (r < R) q = cut_request(a.cut, a.row_start[r], a.row_start[r + 1], a.lengths[r]);
+    return q;
+  };
+  auto pairs_of = [](const CutRequest& q) { return (int64_t)q.tiles * q.key_tiles; };
+  auto items_of = [&](const CutRequest& q, int n) { return kTiles ? q.tiles : (int64_t)q.tiles * n; };
+  auto parts_of = [](const CutRequest& q, int n) { return n > 1 ? (int64_t)q.tiles * n : 0; };
+  CutRequest q;
+  int slice = 0, chunk;
+  int64_t before = 0, parts_before = 0;  // of earlier slices
+  if (slices == 1) {
+    q = shape(0);
+    chunk = cut_chunk(a.cut, lane_value(wave_sums(pairs_of(q)), 63));
+  } else {
+    for (int s = wave; s < slices; s += W) {
+      const int64_t x = wave_sums(pairs_of(shape(s)));
+      if (lane == 63) sums[0][s] = x;
     }
-    if (lane == 63) sums[1 + i][wave] = x;
-    upto[i] = x - own[i];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    for (int w = 0; w < wave; ++w) upto[i] += sums[1 + i][w];
-  if (at >= upto[0] && at < upto[0] + own[0]) {
-    for (int r = first; r < last; ++r) {
-      const CutRequest q = shape(r);
-      const int32_t n = cut_splits(a.cut, q, chunk);
-      const int64_t items = kTiles ? q.tiles : (int64_t)q.tiles * n;
-      if (at < upto[0] + items) {
-        hit = {r, (int32_t)(at - upto[0]), upto[1], chunk};
+    __syncthreads();
+    int64_t pairs = 0;
+    for (int s = lane; s < slices; s += 64) pairs += sums[0][s];
+    chunk = cut_chunk(a.cut, lane_value(wave_sums(pairs), 63));
+    for (int s = wave; s < slices; s += W) {
+      q = shape(s);
+      const int n = cut_splits(a.cut, q, chunk);
+      const int64_t x = wave_sums(items_of(q, n)), y = wave_sums(parts_of(q, n));
+      if (lane == 63) sums[1][s] = x, sums[2][s] = y;
+    }
+    __syncthreads();
+    for (;; slice += 64) {  // 64 slices at a time
+      if (slice >= slices) return false;
+      const bool in = slice + lane < slices;
+      const int64_t own = in ? sums[1][slice + lane] : 0, parts = in ? sums[2][slice + lane] : 0;
+      const int64_t upto = wave_sums(own), parts_upto = wave_sums(parts);
+      const uint64_t past = __ballot(at < before + upto);
+      const int hit = past ? __builtin_ctzll(past) : 63;
+      if (past) {
+        before += lane_value(upto - own, hit), parts_before += lane_value(parts_upto - parts, hit);
+        slice += hit;
         break;
       }
-      upto[0] += items;
-      upto[1] += n > 1 ? (int64_t)q.tiles * n : 0;
+      before += lane_value(upto, 63), parts_before += lane_value(parts_upto, 63);
     }
+    q = shape(slice);
   }
-  __syncthreads();
-  *found = hit;
-  if (found->request < 0) return false;
-  *req = read(found->request);
+  const int n = cut_splits(a.cut, q, chunk);
+  const int64_t own = items_of(q, n), parts = parts_of(q, n), upto = wave_sums(own), parts_upto = wave_sums(parts);
+  const uint64_t past = __ballot(at < before + upto);
+  if (!past) return false;
+  const int hit = __builtin_ctzll(past);
+  found->request = 64 * slice + hit;
+  found->index = (int32_t)(at - before - lane_value(upto - own, hit));
+  found->parts_before = parts_before + lane_value(parts_upto - parts, hit);
+  found->chunk = chunk;
+  auto value = [&](int32_t x) { return __builtin_amdgcn_readlane(x, hit); };
+  *req = {value(q.begin), value(q.end), lane_value(q.lead, hit), value(q.length), value(q.packed), value(q.tiles), value(q.key_tiles)};
   return true;
 }
 
@@ -309,9 +335,11 @@ struct Rows {
   }
 
   // Scores of N tiles to weights; `first` is the first tile's first key, `mask`
-  // where some of the keys are not seen by some column (bad: two bits a tile).
+  // where some of the keys are not seen by some column (bad: two bits a tile), `fresh`
+  // in front of the first product.
   template <int N>
-  __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t (&t)[N], bool mask, int first, int bad, u32x4 (&w)[N][2]) {
+  __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t (&t)[N], bool mask, int first, int bad, bool fresh,
+                                          u32x4 (&w)[N][2]) {
     const int h = (threadIdx.x & 63) >> 5;
     if (mask) {
       const int past = pos - first - 4 * h;  // keys beyond it are not seen
@@ -331,10 +359,12 @@ struct Rows {
       const float grown = fmaxf(max, most), keep = exp2_fast(max - (grown == -INFINITY ? 0.0f : grown));
       max = grown;
       sum *= keep;
+      if (!fresh) {
 #pragma unroll
-      for (int ct = 0; ct < kChannelTiles; ++ct)
+        for (int ct = 0; ct < kChannelTiles; ++ct)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[ct][r] *= keep;
+          for (int r = 0; r < 16; ++r) o[ct][r] *= keep;
+      }
     }
     const float base = max == -INFINITY ? 0.0f : max;
 #pragma unroll
@@ -514,7 +544,7 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
       __builtin_amdgcn_sched_barrier(0);
       if (more) request_tile<HD, true>(a, next, limit - kKeyTile * (t + 4), keys, 0, T::kLoads);
       u32x4 w[1][2];
-      rows.template weights<1>(a, sc, kKeyTile * t + kKeyTile - 1 > least || at.bad, kKeyTile * t, at.bad, w);
+      rows.template weights<1>(a, sc, kKeyTile * t + kKeyTile - 1 > least || at.bad, kKeyTile * t, at.bad, t == mine, w);
       if (more) arrived_but<T::kLoads>();
       else arrived_but<0>();
       rows.context(values, w[0]);
@@ -693,7 +723,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
 #pragma unroll
       for (int n = 0; n < N; ++n) rows.template scores<1>(keys + 2 * n * T::kBytes, sc[n]);
       u32x4 w[N][2];
-      rows.template weights<N>(a, sc, first + kKeyTile * N - 1 > least || gone, first, gone, w);
+      rows.template weights<N>(a, sc, first + kKeyTile * N - 1 > least || gone, first, gone, i == 0, w);
 #pragma unroll
       for (int n = 0; n < N; ++n) rows.context(keys + (2 * n + 1) * T::kBytes, w[n]);
       __builtin_amdgcn_sched_barrier(0);

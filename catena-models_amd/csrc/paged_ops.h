@@ -251,7 +251,7 @@ int check_attention_sizes(const char* what, int64_t rows, int64_t requests, int3
     return fail(CQ35_EUNSUPPORTED, "%s: head_dim %d is not 64, 128 or 256", what, head_dim);
   if (kv_heads < 1 || kv_heads > 1024 || q_heads < 1 || q_heads > 4096 || q_heads % kv_heads)
     return fail(CQ35_EINVAL, "%s: %d query heads over %d key/value heads", what, q_heads, kv_heads);
-  if (rows < 0 || requests < 0 || requests > INT32_MAX || max_rows < 0 || max_keys < 0 ||
+  if (rows < 0 || requests < 0 || requests > kAttendMostRequests || max_rows < 0 || max_keys < 0 ||
       rows > INT32_MAX / (q_heads / kv_heads))
     return fail(CQ35_ERANGE, "%s: %lld rows of %lld requests, at most %lld rows and %lld keys each", what, (long long)rows,
                 (long long)requests, (long long)max_rows, (long long)max_keys);

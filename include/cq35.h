@@ -425,7 +425,8 @@ int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const
  * BF16 once. The same call gives the same bits.
  * A row that sees no key (p < 0) gets zeros. Keys in pages whose number is
  * outside the cache are not seen; lengths are cut to what the table holds.
- * Rows outside every request are left alone. out may be q itself, laid out
+ * Rows outside every request are left alone; up to 8192 requests, rows *
+ * q_heads / kv_heads below 2^31. out may be q itself, laid out
  * alike; it overlaps no other operand.
  * max_rows and max_keys are what the caller knows of the most rows and keys
  * of any request, 0 for nothing: they steer how the work is cut and the

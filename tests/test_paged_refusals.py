@@ -42,7 +42,7 @@ BAD_CACHES = [
     (dict(page_size=1 << 17), -4, "power of two"), (dict(pages=0), -2, "pages"), (dict(pages=1 << 27), -2, "pages"),
     (dict(pages=-1), -2, "pages"), (dict(keys=BASE + 8), -1, "16-byte"), (dict(values=BASE + 2), -1, "16-byte"),
     (dict(row_stride=132), -1, "multiples of 8"), (dict(page_stride=-2048), -1, "multiples of 8"),
-    (dict(row_stride=64), -1, "overlap"), (dict(page_stride=1024), -1, "overlap"), (dict(head_stride=32), -1, "overlap"),
+    (dict(row_stride=64), -1, "overlap"), (dict(row_stride=(1 << 26) + 8), -4, "apart"), (dict(page_stride=1024), -1, "overlap"), (dict(head_stride=32), -1, "overlap"),
     (dict(page_stride=0), -1, "overlap"), (dict(page_stride=1 << 62), -1, "overlap"),
 ]
 
@@ -63,7 +63,8 @@ def test_cache_refusals(change, code, text):
 
 @pytest.mark.parametrize("change,code,text", [
     (dict(q_heads=3), -1, "query heads"), (dict(q_heads=0), -1, "query heads"), (dict(rows=-1), -2, "rows"),
-    (dict(rows=1 << 31), -2, "rows"), (dict(requests=-1), -2, "requests"), (dict(max_rows=-1), -2, "rows"),
+    (dict(rows=1 << 31), -2, "rows"), (dict(requests=-1), -2, "requests"), (dict(requests=8193), -2, "requests"), (dict(rows=1 << 30), -2, "rows"),
+    (dict(max_rows=-1), -2, "rows"),
     (dict(max_keys=-1), -2, "keys"), (dict(table=None), -1, "null"), (dict(row_start=None), -1, "null"),
     (dict(lengths=None), -1, "null"), (dict(width=0), -2, "tables"), (dict(width=1 << 28), -2, "tables"),
     (dict(table_stride=-1), -2, "tables"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"),
