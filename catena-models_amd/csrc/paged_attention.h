@@ -114,7 +114,9 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, uint32_t at, Foun
   int64_t before = 0, parts_before = 0;  // of earlier slices
   if (slices == 1) {
     q = shape(0);
-    chunk = cut_chunk(a.cut, lane_value(wave_sums(pairs_of(q)), 63));
+    chunk = cut_chunk(a.cut, lane_value(wave_sums(pairs_of(q)), 63), [&](int32_t x) {
+      return lane_value(wave_sums((int64_t)q.tiles * cut_splits(a.cut, q, x)), 63);
+    });
   } else {
     for (int s = wave; s < slices; s += W) {
       const int64_t x = wave_sums(pairs_of(shape(s)));
@@ -123,7 +125,9 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, uint32_t at, Foun
     __syncthreads();
     int64_t pairs = 0;
     for (int s = lane; s < slices; s += 64) pairs += sums[0][s];
-    chunk = cut_chunk(a.cut, lane_value(wave_sums(pairs), 63));
+    CutRule plain = a.cut;
+    plain.search = 0;
+    chunk = cut_chunk(plain, lane_value(wave_sums(pairs), 63), [](int32_t) { return (int64_t)0; });
     for (int s = wave; s < slices; s += W) {
       q = shape(s);
       const int n = cut_splits(a.cut, q, chunk);
@@ -176,6 +180,14 @@ struct KvTile {
   }
 };
 
+// The lane's number, made anew: what follows from it is not kept in registers
+// around a loop that has none to spare.
+__device__ __forceinline__ int lane_here() {
+  int l = threadIdx.x & 63;
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
@@ -204,58 +216,64 @@ __device__ __forceinline__ void arrived_but() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Where the 32 keys of a tile lie: two runs of 16 rows (pages hold a multiple
-// of 16), each in one page.
-struct TilePlace {
-  int64_t half[2];  // elements
-  int bad;          // bit per half: a page number outside the cache
-};
-
-__device__ __forceinline__ TilePlace place_tile(const AttendArgs& a, int request, int64_t kv_offset, int tile, int last_key) {
-  // uniform: through the scalar cache
-  typedef const __attribute__((address_space(4))) int32_t* Entry;
-  TilePlace p;
-  p.bad = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    // the second run may lie behind the last key, where the table may end
-    int key = kKeyTile * tile + 16 * h;
-    if (key > last_key) key = kKeyTile * tile;
-    const Entry e = (Entry)(uintptr_t)(a.table + request * a.table_stride + (key >> a.shift));
-    int32_t page = __builtin_amdgcn_readfirstlane(*e);
-    if (page < 0 || page >= a.pages) page = 0, p.bad |= 1 << h;
-    p.half[h] = page * a.page_stride + (key & ((1 << a.shift) - 1)) * a.row_stride + kv_offset;
+// Where keys lie: runs of 16 rows, each in one page (pages hold a multiple of
+// 16). A window keeps the places of the runs of 32 tiles, `step` tiles apart, in
+// the lanes of a wave (lane 2 i + h: run h of the window's tile i), as bytes
+// from the cache's base: a table entry read for every tile would be waited for
+// with the tile's LDS reads, which share its counter, and its products cost as
+// many scalar instructions as a tile's softmax has vector ones. Runs of pages
+// outside the cache and of tiles from `end` on are bad and lie nowhere.
+struct Window {
+  uint32_t lo, hi;
+  uint64_t bad;
+  // tiles first, first + step, ...
+  __device__ __forceinline__ void fill(const AttendArgs& a, int request, int64_t kv_offset, int first, int step, int end,
+                                       int last_key) {
+    const int lane = lane_here(), tile = first + (lane >> 1) * step;
+    // the second run of the last tile may lie behind the last key, where the
+    // table may end; its rows are not read
+    const int key = min(kKeyTile * min(tile, end - 1) + 16 * (lane & 1), last_key);
+    const int32_t page = a.table[request * a.table_stride + (key >> a.shift)];
+    const bool none = tile >= end || page < 0 || page >= a.pages;
+    const int row = (key & ~15) & ((1 << a.shift) - 1);
+    const int64_t at = none ? 0 : 2 * (page * a.page_stride + row * a.row_stride + kv_offset);
+    lo = (uint32_t)at, hi = (uint32_t)((uint64_t)at >> 32);
+    bad = __ballot(none);
   }
-  return p;
-}
+  __device__ __forceinline__ int64_t at(int run) const {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, run) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, run));
+  }
+};
 
 // Zeros in place of rows that must not be read.
 __device__ __align__(16) uint32_t attend_zeros[4];
 
-// Requests i0 .. i0 + count - 1 of a tile of keys (or of values), zeros for
-// rows behind `last_row` of the tile and those of bad pages.
+// `count` requests of the rows from `row` (of the tile) of a run at byte `at`,
+// into the tile at LDS `to`; zeros for rows behind `last_row` of the tile, and
+// for a bad run.
 template <int HD, bool kKeys>
-__device__ __forceinline__ void request_tile(const AttendArgs& a, const TilePlace& p, int last_row, uint32_t to, int i0,
+__device__ __forceinline__ void request_rows(const AttendArgs& a, int64_t at, bool bad, int row0, int last_row, uint32_t to,
                                              int count) {
   typedef KvTile<HD> T;
-  const int lane = threadIdx.x & 63, lr = lane / T::kPieces, piece = lane % T::kPieces;
-  const uint16_t* base = kKeys ? a.keys : a.values;
-  if (last_row >= 31 && !p.bad) {
+  const int lane = lane_here(), lr = lane / T::kPieces, piece = lane % T::kPieces;
+  const uint8_t* base = reinterpret_cast<const uint8_t*>(kKeys ? a.keys : a.values) + at;
+  const int rs = 2 * (int)a.row_stride;
+  to += row0 * T::kRow;
+  if (!bad && last_row >= row0 + count * T::kPer - 1) {
+    base += (int64_t)(row0 & 15) * rs;
 #pragma unroll
     for (int n = 0; n < count; ++n) {
-      const int i = i0 + n, row = i * T::kPer + lr;
-      const int in = (i * T::kPer) & 15;  // the request's first row in its run of 16
-      const uint32_t off = lr * (uint32_t)a.row_stride * 2 + 16 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row)));
-      request_lds(to + 1024 * i, base + (i * T::kPer < 16 ? p.half[0] : p.half[1]) + in * a.row_stride, off);
+      const int row = row0 + n * T::kPer + lr;
+      request_lds(to + 1024 * n, base, lr * rs + 16 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row))));
+      base += (int64_t)T::kPer * rs;
     }
   } else {
 #pragma unroll 1
     for (int n = 0; n < count; ++n) {
-      const int i = i0 + n, row = i * T::kPer + lr;
-      const int off = 8 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row)));
-      const bool none = row > last_row || (p.bad >> (row >> 4) & 1);
-      const uint16_t* from = base + (i * T::kPer < 16 ? p.half[0] : p.half[1]) + (row & 15) * a.row_stride + off;
-      request_lds(to + 1024 * i, none ? reinterpret_cast<const uint16_t*>(attend_zeros) : from);
+      const int row = row0 + n * T::kPer + lr;
+      const int off = 16 * (piece ^ (kKeys ? T::key_swizzle(row) : T::value_swizzle(row)));
+      const uint8_t* from = base + (int64_t)(row & 15) * rs + off;
+      request_lds(to + 1024 * n, bad || row > last_row ? reinterpret_cast<const uint8_t*>(attend_zeros) : from);
     }
   }
 }
@@ -286,11 +304,12 @@ __device__ __forceinline__ uint2 read_transposed(uint32_t at) {
 template <int HD>
 struct Rows {
   typedef KvTile<HD> T;
-  static constexpr int kSteps = HD / 16, kChannelTiles = HD / 32, kAhead = 4;
+  static constexpr int kSteps = HD / 16, kChannelTiles = HD / 32, kAhead = 4, kMixAhead = HD == 256 ? 2 : 4;
   u32x4 q[kSteps];
   f32x16_t o[kChannelTiles];
   float max, sum;  // sum: this half's keys
   int pos;         // last key that the column sees, -1: none
+  uint32_t places; // of the lane's operands in a tile of values (high half) and of keys
 
   // the columns are packed rows m0 ..
   __device__ __forceinline__ void load(const AttendArgs& a, const CutRequest& r, int kvh, int m0) {
@@ -303,6 +322,12 @@ struct Rows {
     for (int s = 0; s < kSteps; ++s) q[s] = (*reinterpret_cast<const u32x4*>(from + 16 * s) & a.q_and) ^ a.q_xor;
     pos = m < r.packed ? visible_keys(r.lead + row, r.length) - 1 : -1;
   }
+  __device__ __forceinline__ void place() {
+    const int lane = threadIdx.x & 63, j = lane & 15, h = lane >> 5, upper = lane >> 4 & 1;
+    const int vrow = 4 * h + (j >> 2), krow = lane & 31;
+    places = (uint32_t)(vrow * T::kRow + 16 * ((2 * upper + (j >> 1 & 1)) ^ T::value_swizzle(vrow)) + 8 * (j & 1)) << 16 |
+             (uint32_t)(krow * T::kRow + 16 * (h ^ T::key_swizzle(krow)));
+  }
   __device__ __forceinline__ void clear() {
     max = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -313,7 +338,7 @@ struct Rows {
   // its SIMD would otherwise wait for each product before the next.
   template <int kChains>
   __device__ __forceinline__ void scores(uint32_t keys, f32x16_t& sc) const {
-    const int lane = threadIdx.x & 63, row = lane & 31, h = lane >> 5;
+    const int lane = lane_here(), row = lane & 31, h = lane >> 5;
     const uint32_t at = keys + row * T::kRow + 16 * (h ^ T::key_swizzle(row));
     auto read = [&](int s) { return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(at ^ (32 * s)); };
     // four operands on their way: more would not fit the registers beside q and o
@@ -340,7 +365,7 @@ struct Rows {
   template <int N>
   __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t (&t)[N], bool mask, int first, int bad, bool fresh,
                                           u32x4 (&w)[N][2]) {
-    const int h = (threadIdx.x & 63) >> 5;
+    const int h = lane_here() >> 5;
     if (mask) {
       const int past = pos - first - 4 * h;  // keys beyond it are not seen
 #pragma unroll
@@ -403,6 +428,41 @@ struct Rows {
       if (n + kAhead < 2 * kChannelTiles) v[n % kAhead] = read(n + kAhead);
       __builtin_amdgcn_sched_barrier(0);
     }
+  }
+
+  // o += V^T P^T and the next tile's scores in one run, product by product: the
+  // scores' sum alone would have each product wait for the one before.
+  __device__ __forceinline__ void mix(uint32_t values, const u32x4 (&w)[2], uint32_t keys, f32x16_t& sc) {
+    uint32_t both = places;
+    asm volatile("" : "+v"(both));  // taken apart here, not kept apart around the loop
+    const uint32_t vat = values + (both >> 16), kat = keys + (both & 0xffff);
+    auto read_value = [&](int n) {
+      const uint2 x0 = read_transposed((vat ^ (32 * (n & ~1))) + (16 * (n & 1)) * T::kRow);
+      const uint2 x1 = read_transposed((vat ^ (32 * (n & ~1))) + (16 * (n & 1) + 8) * T::kRow);
+      return u32x4{x0.x, x0.y, x1.x, x1.y};
+    };
+    // steps s and s + kSteps / 2 in turn: half a row apart, their addresses differ
+    // by a constant that the swizzle does not touch (256 channels)
+    auto step = [](int n) { return HD == 256 ? (n >> 1) + (n & 1) * (kSteps / 2) : n; };
+    auto read_key = [&](int n) {
+      const uint32_t at = HD == 256 ? (kat ^ (32 * (n >> 1))) + 256 * (n & 1) : kat ^ (32 * n);
+      return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
+    };
+    constexpr int A = kMixAhead;
+    u32x4 v[A], k[A];
+#pragma unroll
+    for (int n = 0; n < A; ++n) v[n] = read_value(n), k[n] = read_key(n);
+    f32x16_t next = {};
+#pragma unroll
+    for (int n = 0; n < kSteps; ++n) {
+      o[n >> 1] = mfma32(v[n % A], w[n & 1], o[n >> 1]);
+      if (n + A < kSteps) v[n % A] = read_value(n + A);
+      __builtin_amdgcn_sched_barrier(0);
+      next = mfma32(k[n % A], q[step(n)], next);
+      if (n + A < kSteps) k[n % A] = read_key(n + A);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    sc = next;
   }
 
   // Whether a result of a column that sees anything is NaN (or infinite).
@@ -528,29 +588,44 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
   for (int limit = item.last_key;;) {
     rows.clear();
     const int t1 = min(item.t1, key_tiles_of(limit + 1)), mine = item.t0 + wave;
-    TilePlace at = {}, next = {};
+    Window runs;
+    int window = mine;  // the window's first tile
+    if (mine < t1) runs.fill(a, item.request, kv_offset, mine, 4, t1, limit);
+    // tile t's keys or values
+    auto request = [&](auto kind, int t) {
+      constexpr bool kKeys = decltype(kind)::value;
+#pragma unroll
+      for (int run = 0; run < 2; ++run) {
+        const int at = (t - window) / 2 + run;
+        request_rows<HD, kKeys>(a, runs.at(at), runs.bad >> at & 1, 16 * run, limit - kKeyTile * t, kKeys ? keys : values, T::kLoads / 2);
+      }
+    };
     if (mine < t1) {
-      at = place_tile(a, item.request, kv_offset, mine, limit);
-      request_tile<HD, true>(a, at, limit - kKeyTile * mine, keys, 0, T::kLoads);
-      request_tile<HD, false>(a, at, limit - kKeyTile * mine, values, 0, T::kLoads);
+      request(std::true_type{}, mine);
+      request(std::false_type{}, mine);
     }
 #pragma unroll 1
     for (int t = mine; t < t1; t += 4) {
       const bool more = t + 4 < t1;
-      if (more) next = place_tile(a, item.request, kv_offset, t + 4, limit);
+      const int gone = (int)(runs.bad >> ((t - window) / 2)) & 3;
       arrived_but<T::kLoads>();
       f32x16_t sc[1];
       rows.template scores<2>(keys, sc[0]);
       __builtin_amdgcn_sched_barrier(0);
-      if (more) request_tile<HD, true>(a, next, limit - kKeyTile * (t + 4), keys, 0, T::kLoads);
+      if (more) {
+        if (t + 4 == window + 128) {
+          window = t + 4;
+          runs.fill(a, item.request, kv_offset, window, 4, t1, limit);
+        }
+        request(std::true_type{}, t + 4);
+      }
       u32x4 w[1][2];
-      rows.template weights<1>(a, sc, kKeyTile * t + kKeyTile - 1 > least || at.bad, kKeyTile * t, at.bad, t == mine, w);
+      rows.template weights<1>(a, sc, kKeyTile * t + kKeyTile - 1 > least || gone, kKeyTile * t, gone, t == mine, w);
       if (more) arrived_but<T::kLoads>();
       else arrived_but<0>();
       rows.context(values, w[0]);
       __builtin_amdgcn_sched_barrier(0);
-      if (more) request_tile<HD, false>(a, next, limit - kKeyTile * (t + 4), values, 0, T::kLoads);
-      at = next;
+      if (more) request(std::false_type{}, t + 4);
     }
     // join the waves
     const float total = rows.sum + other_half(rows.sum);
@@ -652,82 +727,79 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
   R rows;
   rows.load(a, req, kvh, m0);
   const int least = m0 + 32 > req.packed ? -1 : visible_keys(packed_position(a.cut, req, m0), req.length) - 1;
-  const uint32_t ring = lds_address(attend_lds);
-  // a wave's share of a stage: an eighth of each tile's keys and of its values,
-  // or (64 channels: four requests each) a quarter of either
-  constexpr int kOwn = T::kLoads >= 8 ? T::kLoads / 8 : 1, kAll = N * (T::kLoads >= 8 ? 2 * kOwn : 1);
+  const bool idle = m0 >= req.packed;  // no rows: the wave only requests tiles
+  const bool late = wave >= 4;
+  const uint32_t key_ring = lds_address(attend_lds), value_ring = key_ring + kManyStages * N * T::kBytes;
+  // The first four waves request a stage's keys, the others its values; a
+  // wave's share is of one run of 16 rows (half a run for 256 channels).
+  constexpr int kOwn = N * T::kLoads / 4;
+  const int share = (wave & 3) * kOwn, own_tile = share / T::kLoads, own_row = share % T::kLoads * T::kPer;
+  const int own_run = 2 * own_tile + (own_row >> 4);
   bool open = m0 + c < req.packed;
   for (int limit = item.last_key;;) {
     rows.clear();
     const int t1 = min(item.t1, key_tiles_of(limit + 1)), stages = (t1 - item.t0 + N - 1) / N;
-    struct Place {
-      TilePlace tile[N];
-    };
-    auto place = [&](int i) {  // a tile behind the split's end counts as bad pages
-      Place p;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const int t = item.t0 + N * i + n;
-        if (t < t1) p.tile[n] = place_tile(a, item.request, kv_offset, t, limit);
-        else p.tile[n] = {{0, 0}, 3};
+    Window runs;
+    uint64_t bad_before = 0;  // of the window before
+    auto request = [&](int i) {
+      const int run = 2 * N * i & 63;
+      if (run == 0) {
+        bad_before = i > 0 ? runs.bad : 0;
+        runs.fill(a, item.request, kv_offset, item.t0 + N * i, 1, t1, limit);
       }
-      return p;
+      const bool bad = runs.bad >> (run + own_run) & 1;
+      const int last = limit - kKeyTile * (item.t0 + N * i + own_tile);
+      const uint32_t slot = (uint32_t)(i % kManyStages * N + own_tile) * T::kBytes;
+      if (late) request_rows<HD, false>(a, runs.at(run + own_run), bad, own_row, last, value_ring + slot, kOwn);
+      else request_rows<HD, true>(a, runs.at(run + own_run), bad, own_row, last, key_ring + slot, kOwn);
     };
-    auto request = [&](const Place& p, int i) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const uint32_t to = ring + (uint32_t)(i % kManyStages * N + n) * 2 * T::kBytes;
-        const int last = limit - kKeyTile * (item.t0 + N * i + n);
-        if (T::kLoads >= 8) {
-          request_tile<HD, true>(a, p.tile[n], last, to, wave * kOwn, kOwn);
-          request_tile<HD, false>(a, p.tile[n], last, to + T::kBytes, wave * kOwn, kOwn);
-        } else if (wave < 4) {
-          request_tile<HD, true>(a, p.tile[n], last, to, wave, 1);
-        } else {
-          request_tile<HD, false>(a, p.tile[n], last, to + T::kBytes, wave - 4, 1);
-        }
-      }
+    // the bad runs of stage i; the window may be a later one's by then
+    const int ahead = late ? 2 : 3;
+    auto bad_runs = [&](int i) {
+      const int newest = min(i + ahead, stages - 1);  // requested by now
+      const uint64_t b = (2 * N * newest) / 64 == (2 * N * i) / 64 ? runs.bad : bad_before;
+      return (int)(b >> (2 * N * i & 63)) & ((1 << 2 * N) - 1);
     };
-    constexpr int kBits = 2 * N;
-    auto bits = [](const Place& p) {
-      int b = 0;
-      for (int n = 0; n < N; ++n) b |= p.tile[n].bad << (2 * n);
-      return b;
-    };
-    int bad = 0;  // the halves of the ring's tiles
-    Place next = {};
-    for (int i = 0; i < kManyStages - 1; ++i)
-      if (i < stages) {
-        next = place(i);
-        bad |= bits(next) << (kBits * i);
-        request(next, i);
-      }
-    if (kManyStages - 1 < stages) next = place(kManyStages - 1);
 #pragma unroll 1
-    for (int i = 0; i < stages; ++i) {
-      if (i + 2 < stages) arrived_but<2 * kAll>();
-      else if (i + 1 < stages) arrived_but<kAll>();
+    for (int i = 0; i < ahead; ++i)
+      if (i < stages) request(i);
+    // Barrier i: the keys of stage i + 1 and the values of stage i are in LDS
+    // for every wave, the keys of stage i - 1 and the values of stage i - 2 done
+    // with.
+    auto enter = [&](int i) {
+      if (i + ahead - 1 < stages) arrived_but<kOwn>();
       else arrived_but<0>();
-      __syncthreads();
+      __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
-      const int stage = i % kManyStages;
-      if (i + kManyStages - 1 < stages) {
-        const int ahead = (stage + kManyStages - 1) % kManyStages;
-        bad = (bad & ~(((1 << kBits) - 1) << (kBits * ahead))) | bits(next) << (kBits * ahead);
-        request(next, i + kManyStages - 1);
-        if (i + kManyStages < stages) next = place(i + kManyStages);
-      }
-      const uint32_t keys = ring + (uint32_t)(stage * N) * 2 * T::kBytes;
-      const int gone = bad >> (kBits * stage) & ((1 << kBits) - 1), first = kKeyTile * (item.t0 + N * i);
+      if (i + ahead < stages) request(i + ahead);
+    };
+    auto keys_at = [&](int i) { return key_ring + (uint32_t)(i % kManyStages * N) * T::kBytes; };
+    auto values_at = [&](int i) { return value_ring + (uint32_t)(i % kManyStages * N) * T::kBytes; };
+    rows.place();
+    if (stages <= 0) {  // no key is seen
+    } else if (idle) {
+#pragma unroll 1
+      for (int i = 0; i <= stages; ++i) enter(i);
+    } else {
       f32x16_t sc[N];
+      enter(0);
 #pragma unroll
-      for (int n = 0; n < N; ++n) rows.template scores<1>(keys + 2 * n * T::kBytes, sc[n]);
-      u32x4 w[N][2];
-      rows.template weights<N>(a, sc, first + kKeyTile * N - 1 > least || gone, first, gone, i == 0, w);
+      for (int n = 0; n < N; ++n) rows.template scores<1>(keys_at(0) + n * T::kBytes, sc[n]);
+#pragma unroll 1
+      for (int i = 0; i < stages; ++i) {
+        if (!late && i > 0) enter(i);
+        const int gone = bad_runs(i), first = kKeyTile * (item.t0 + N * i);
+        u32x4 w[N][2];
+        rows.template weights<N>(a, sc, first + kKeyTile * N - 1 > least || gone, first, gone, i == 0, w);
+        __builtin_amdgcn_sched_barrier(0);
+        if (late) enter(i + 1);
+        // behind the last stage the scores are of what the ring held: not used
 #pragma unroll
-      for (int n = 0; n < N; ++n) rows.context(keys + (2 * n + 1) * T::kBytes, w[n]);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < N; ++n) rows.mix(values_at(i) + n * T::kBytes, w[n], keys_at(i + 1) + n * T::kBytes, sc[n]);
+      }
+      if (!late) enter(stages);
     }
+    __syncthreads();
     bool nan = rows.any_nan();
     nan |= __shfl_xor((int)nan, 32, 64) != 0;
     const float sum = rows.sum + other_half(rows.sum);

@@ -77,6 +77,7 @@ struct CutRule {
   int32_t target_shift; // log2 of the items wanted, over all KV heads
   int32_t min_tiles;    // key tiles of a split at least
   int32_t max_splits;
+  int32_t search;       // up to 64 requests: look for the chunk of the fewest rounds
   int64_t slots;        // partial results that the workspace holds
 };
 
@@ -105,12 +106,6 @@ CQ35_BOTH CutRequest cut_request(const CutRule& c, int32_t start, int32_t stop, 
   return q;
 }
 
-// Key tiles of a split, from the sum over the requests of tiles * key_tiles.
-CQ35_BOTH int32_t cut_chunk(const CutRule& c, int64_t pairs) {
-  const int64_t even = (pairs * c.kv_heads + ((int64_t)1 << c.target_shift) - 1) >> c.target_shift;
-  return even > INT32_MAX / 2 ? INT32_MAX / 2 : even > c.min_tiles ? (int32_t)even : c.min_tiles;
-}
-
 // Splits of a request's row tiles, and the key tiles of each.
 CQ35_BOTH int32_t cut_splits(const CutRule& c, const CutRequest& q, int32_t chunk) {
   if (q.key_tiles <= chunk) return 1;
@@ -119,6 +114,28 @@ CQ35_BOTH int32_t cut_splits(const CutRule& c, const CutRequest& q, int32_t chun
 }
 CQ35_BOTH int32_t split_tiles(const CutRequest& q, int32_t splits) {
   return q.key_tiles ? (int32_t)(((uint32_t)q.key_tiles + splits - 1) / (uint32_t)splits) : 1;
+}
+
+// Key tiles of a split, from the sum over the requests of tiles * key_tiles:
+// that sum dealt evenly to the items wanted, or up to twice that (`search`)
+// where the requests' ends then make fewer rounds of items: one CU holds one,
+// and an item costs some tiles' time besides its own (kItemTiles, measured).
+// items_at(chunk): the items per KV head that splits of `chunk` make.
+constexpr int kItemTiles = 6;
+template <typename F>
+CQ35_BOTH int32_t cut_chunk(const CutRule& c, int64_t pairs, F items_at) {
+  const int64_t even = (pairs * c.kv_heads + ((int64_t)1 << c.target_shift) - 1) >> c.target_shift;
+  const int32_t base = even > INT32_MAX / 4 ? INT32_MAX / 4 : even > c.min_tiles ? (int32_t)even : c.min_tiles;
+  if (!c.search) return base;
+  int32_t best = base;
+  int64_t least = INT64_MAX;
+  for (int k = 0; k < 5; ++k) {
+    const int32_t chunk = base + (base >> 2) * k;
+    const int64_t rounds = (items_at(chunk) * c.kv_heads + ((int64_t)1 << c.target_shift) - 1) >> c.target_shift;
+    const int64_t cost = rounds * (chunk + kItemTiles);
+    if (cost < least) least = cost, best = chunk;
+  }
+  return best;
 }
 
 // Position of packed row m of a request.

@@ -218,8 +218,8 @@ namespace {
 // request takes them all to k_paged_many. max_rows decides without the lengths,
 // max_keys spares the join where no request can be split.
 constexpr int kFewPacked = 64;
-constexpr int kFewTarget = 9, kManyTarget = 9;  // log2 of the items wanted
-constexpr int kFewMinTiles = 4, kManyMinTiles = 16;
+constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
+constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
 constexpr int kMostSplits = 1024;
 
 struct AttendPlan {
@@ -237,6 +237,7 @@ AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_he
   CutRule& c = p.cut;
   c.rows = (int32_t)rows, c.group = group, c.kv_heads = kv_heads, c.tile_rows = p.few ? kFewRows : kManyRows;
   c.target_shift = p.few ? kFewTarget : kManyTarget, c.min_tiles = p.few ? kFewMinTiles : kManyMinTiles;
+  c.search = !p.few;
   const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
   c.max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, (key_tiles + c.min_tiles - 1) / c.min_tiles));
   p.tiles = most_tiles(rows, requests, group, c.tile_rows);

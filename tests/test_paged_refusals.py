@@ -173,8 +173,8 @@ int main(int argc, char** argv) {
     } else if (what == 'c') {  // the cut of a launch: every (packed row, key tile) once, slots apart and within the bound
       CutRule c{};
       long long R;
-      scanf("%d %d %d %d %d %d %d %d", &c.rows, &c.most_keys, &c.group, &c.kv_heads, &c.tile_rows, &c.target_shift,
-             &c.min_tiles, &c.max_splits);
+      scanf("%d %d %d %d %d %d %d %d %d", &c.rows, &c.most_keys, &c.group, &c.kv_heads, &c.tile_rows, &c.target_shift,
+             &c.min_tiles, &c.max_splits, &c.search);
       scanf("%lld", &R);
       std::vector<int32_t> start(R + 1), length(R);
       for (auto& x : start) scanf("%d", &x);
@@ -187,7 +187,14 @@ int main(int argc, char** argv) {
         const CutRequest q = cut_request(c, start[r], start[r + 1], length[r]);
         pairs += (int64_t)q.tiles * q.key_tiles;
       }
-      const int32_t chunk = cut_chunk(c, pairs);
+      const int32_t chunk = cut_chunk(c, pairs, [&](int32_t x) {
+        int64_t n = 0;
+        for (long long r = 0; r < R; ++r) {
+          const CutRequest q = cut_request(c, start[r], start[r + 1], length[r]);
+          n += (int64_t)q.tiles * cut_splits(c, q, x);
+        }
+        return n;
+      });
       for (long long r = 0; r < R; ++r) {
         const CutRequest q = cut_request(c, start[r], start[r + 1], length[r]);
         const int32_t n = cut_splits(c, q, chunk), each = split_tiles(q, n);
@@ -293,8 +300,8 @@ def test_cut_covers_every_tile_once(index_program):
         if rows < 1:
             continue
         tile_rows = int(rng.choice([32, 256]))
-        lines.append("c %d %d %d %d %d %d %d %d %d %s %s" % (
+        lines.append("c %d %d %d %d %d %d %d %d %d %d %s %s" % (
             rows, 1 << 16, group, kvh, tile_rows, int(rng.choice([0, 5, 9, 10])), int(rng.choice([1, 4, 16])),
-            int(rng.choice([1, 2, 7, 1024])), R, " ".join(map(str, np.concatenate([[0], np.cumsum(new)]))),
+            int(rng.choice([1, 2, 7, 1024])), int(R <= 64 and i % 2), R, " ".join(map(str, np.concatenate([[0], np.cumsum(new)]))),
             " ".join(map(str, length))))
     assert len(ask(index_program, lines)) == len(lines) > 300
