@@ -800,7 +800,9 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
       if (!late) enter(stages);
     }
     __syncthreads();
-    bool nan = rows.any_nan();
+    // keys that every row sees are no reason to do a row again
+    const bool whole = kKeyTile * item.t1 <= visible_keys(packed_position(a.cut, req, kManyRows * item.row_tile), req.length);
+    bool nan = !whole && rows.any_nan();
     nan |= __shfl_xor((int)nan, 32, 64) != 0;
     const float sum = rows.sum + other_half(rows.sum);
     if (open && ((!nan && limit == item.last_key) || rows.pos == limit)) {
@@ -836,12 +838,14 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
 
 // ---------------------------------------------------- joining the splits
 //
-// Block (32 packed rows and KV head, channel tile): each thread one float4 of
-// the fragment order over all splits, weighted by 2^(max - maximum). The
-// weights of up to kJoinKept splits are made once, eight splits at a time.
+// Block (32 packed rows and KV head, kTiles channel tiles): each thread a
+// float4 of the fragment order per channel tile over all splits, weighted by
+// 2^(max - maximum). The splits' maxima and sums are read once, eight splits at
+// a time, each eighth of them joined as it comes; the first parts and the gate
+// are on their way meanwhile.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinKept = 128;
-template <int HD, int kGroups>
+constexpr int kJoinKept = 128;  // splits whose maxima stay in LDS
+template <int HD, int kGroups, int kTiles>
 __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
   const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
   const uint32_t unit = blockIdx.x / (uint32_t)a.cut.kv_heads;
@@ -855,58 +859,60 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
   const int64_t first = (f.parts_before + (int64_t)f.index * splits) * a.cut.kv_heads + kvh;
   if (first + (int64_t)(used - 1) * a.cut.kv_heads >= a.cut.slots) return;
   __shared__ float kept[kJoinKept][32], stat[2][8][32];
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6, quad = 4 * blockIdx.y + wave;
-  const int m = a.cut.tile_rows * tile + 32 * group + c;
-  const bool row = m < req.packed;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
+  const int m0 = a.cut.tile_rows * tile + 32 * group, m = min(m0 + c, req.packed - 1);
+  if (m0 >= req.packed) return;
+  const bool row = m0 + c < req.packed;  // other columns' parts were not written
   const int64_t step = (int64_t)a.cut.kv_heads * kGroups * PartSlot<HD>::kFloats;
   const float* part = a.part + (first * kGroups + group) * PartSlot<HD>::kFloats;
-  auto max_of = [&](int s) { return part[s * step + 32 * HD + c]; };
-  const int eighth = 2 * wave + h;
-  float most = -INFINITY;
+  const int quad0 = 4 * kTiles * blockIdx.y + wave;  // this thread's quads: quad0 + 4 j
+  const RowWriter to(a, req, kvh, m, 1.0f);
+  constexpr int kBatch = 8;
+  float4 x[kBatch];
+  auto read = [&](int s0, int j) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      x[i] = s0 + i < used && row ? reinterpret_cast<const float4*>(part + (s0 + i) * step)[(quad0 + 4 * j) * 64 + lane]
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  read(0, 0);
+  float most = -INFINITY, sum = 0.0f;
   if (row)
 #pragma unroll 4
-    for (int s = eighth; s < used; s += 8) most = fmaxf(most, max_of(s));
-  stat[0][eighth][c] = most;
+    for (int s = 2 * wave + h; s < used; s += 8) {
+      const float x = part[s * step + 32 * HD + c], l = part[s * step + 32 * HD + 32 + c];
+      if (s < kJoinKept) kept[s][c] = x;
+      const float grown = fmaxf(most, x), base = grown == -INFINITY ? 0.0f : grown;
+      sum = __builtin_fmaf(l, exp2_fast(x - base), sum * exp2_fast(most - base));
+      most = grown;
+    }
+  stat[0][2 * wave + h][c] = most, stat[1][2 * wave + h][c] = sum;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) most = fmaxf(most, stat[0][i][c]);
   const float base = most == -INFINITY ? 0.0f : most;
-  float sum = 0.0f;
-  if (row)
-#pragma unroll 4
-    for (int s = eighth; s < used; s += 8) {
-      const float w = exp2_fast(max_of(s) - base);
-      if (s < kJoinKept) kept[s][c] = w;
-      sum = __builtin_fmaf(w, part[s * step + 32 * HD + 32 + c], sum);
-    }
-  stat[1][eighth][c] = sum;
-  __syncthreads();
-  if (!row) return;
   sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum += stat[1][i][c];
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](auto batch) {
-    constexpr int B = decltype(batch)::value;
-    for (int s0 = 0; s0 < used; s0 += B) {
-      float4 x[B];
+  for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(stat[1][i][c], exp2_fast(stat[0][i][c] - base), sum);
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int i = 0; i < B; ++i) x[i] = reinterpret_cast<const float4*>(part + min(s0 + i, used - 1) * step)[quad * 64 + lane];
+  for (int j = 0; j < kTiles; ++j) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < used; s0 += kBatch) {
+      if (s0 > 0 || j > 0) read(s0, j);
 #pragma unroll
-      for (int i = 0; i < B; ++i) {
+      for (int i = 0; i < kBatch; ++i) {
         const int s = s0 + i;
         if (s >= used) break;
-        const float w = s < kJoinKept ? kept[s][c] : exp2_fast(max_of(s) - base);
+        const float w = exp2_fast((s < kJoinKept ? kept[s][c] : part[s * step + 32 * HD + c]) - base) * inverse;
         v.x = __builtin_fmaf(w, x[i].x, v.x), v.y = __builtin_fmaf(w, x[i].y, v.y);
         v.z = __builtin_fmaf(w, x[i].z, v.z), v.w = __builtin_fmaf(w, x[i].w, v.w);
       }
     }
-  };
-  if (used <= 2) add(std::integral_constant<int, 2>{});
-  else add(std::integral_constant<int, 8>{});
-  const RowWriter to(a, req, kvh, m, sum);
-  if (a.gate) to.write<true>(8 * quad + 4 * h, v.x, v.y, v.z, v.w);
-  else to.write<false>(8 * quad + 4 * h, v.x, v.y, v.z, v.w);
+    if (!row) continue;
+    if (a.gate) to.template write<true>(8 * (quad0 + 4 * j) + 4 * h, v.x, v.y, v.z, v.w);
+    else to.template write<false>(8 * (quad0 + 4 * j) + 4 * h, v.x, v.y, v.z, v.w);
+  }
 }
 
 }  // namespace cq35

@@ -221,6 +221,7 @@ constexpr int kFewPacked = 64;
 constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
 constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
 constexpr int kMostSplits = 1024;
+constexpr int kWideJoin = 512;  // units of 32 packed rows and KV head
 
 struct AttendPlan {
   bool few;
@@ -265,12 +266,15 @@ int launch_attention(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
   const int64_t units = p.tiles * a.cut.kv_heads * (a.cut.tile_rows / 32);
   if (items > INT32_MAX || units > INT32_MAX) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
   auto kernel = p.few ? k_paged_few<HD> : k_paged_many<HD>;
-  auto join = p.few ? k_paged_join<HD, 1> : k_paged_join<HD, kManyRows / 32>;
+  // a block a channel tile where there are few rows, all of them where there are many
+  const bool wide = units >= kWideJoin;
+  auto join = p.few ? (wide ? k_paged_join<HD, 1, HD / 32> : k_paged_join<HD, 1, 1>)
+                    : (wide ? k_paged_join<HD, kManyRows / 32, HD / 32> : k_paged_join<HD, kManyRows / 32, 1>);
   const size_t lds = p.few ? few_lds_bytes<HD>() : many_lds_bytes<HD>();
   if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   int rc = launch_operator("paged attention", kernel, dim3((unsigned)items), p.few ? kFewThreads : kManyThreads, lds, s, a);
   if (!rc && a.cut.slots > 0)
-    rc = launch_operator("paged attention", join, dim3((unsigned)units, HD / 32), kJoinThreads, 0, s, a);
+    rc = launch_operator("paged attention", join, dim3((unsigned)units, wide ? 1 : HD / 32), kJoinThreads, 0, s, a);
   return rc;
 }
 

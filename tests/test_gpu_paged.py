@@ -365,6 +365,36 @@ def test_attention_rows_that_see_nothing():
         assert hidden and bool((got[hidden] == 0).all())
 
 
+@pytest.mark.parametrize("new,length,QH,KVH,HD,page", [
+    (40, 3000, 4, 1, 256, 16), (33, 2500, 2, 2, 128, 32), (70, 2300, 1, 1, 64, 64), (1, 9000, 8, 2, 256, 16), (2, 5000, 3, 1, 64, 16),
+])
+def test_attention_long_splits(new, length, QH, KVH, HD, page):
+    """Splits of more tiles than a wave keeps places of, with pages outside the
+    cache in several of those stretches."""
+    say("long splits", new, length, HD)
+    s = attention_case(length, [new, 1], [length, 40], QH, KVH, HD, page)
+    check_attention(s, run_attention(s, max_rows=new, max_keys=1))
+    check_attention(s, run_attention(s, max_rows=new, max_keys=length))
+    for j in (0, 1030, 1100, 2100, length - 1):
+        s["table"][0, j // page] = -3
+    check_attention(s, run_attention(s, max_rows=new, max_keys=1))
+    check_attention(s, run_attention(s))
+
+
+@pytest.mark.parametrize("R,most_new,most,HD,QH,KVH", [(64, 3, 200, 64, 2, 1), (65, 1, 300, 128, 4, 2), (70, 40, 90, 64, 4, 1),
+                                                       (300, 2, 100, 64, 2, 2), (1500, 2, 40, 64, 1, 1), (8192, 1, 20, 64, 1, 1)])
+def test_attention_many_requests(R, most_new, most, HD, QH, KVH):
+    say("many requests", R, most_new, most)
+    rng = np.random.default_rng(R)
+    new = rng.integers(0, most_new + 1, R).tolist()
+    lengths = [int(n + rng.integers(0, most)) for n in new]
+    if most_new == 1:
+        lengths[3] = 5000  # one that is split
+    s = attention_case(R, new, lengths, QH, KVH, HD, 16)
+    check_attention(s, run_attention(s))
+    check_attention(s, run_attention(s, max_rows=most_new, max_keys=max(lengths)))
+
+
 def test_attention_leaves_other_rows():
     """Rows behind the last request, in front of the first, and requests whose rows pass the tensor's end."""
     s = attention_case(11, [3, 30], [40, 90], 4, 2, 128, 16, width_extra=80)
@@ -413,6 +443,29 @@ def test_attention_non_finite_values_that_are_not_seen(HD, new, length, QH):
     got = run_attention(s)
     check_attention(dict(s, **clean), got, rows=slice(0, new - 2))
     assert bool(torch.isnan(got[new - 1]).all())
+
+
+@pytest.mark.parametrize("HD,QH,KVH,new,length", [(256, 8, 1, 60, 400), (64, 2, 2, 300, 500), (128, 4, 2, 3, 100)])
+def test_attention_non_finite_values_that_are_seen(HD, QH, KVH, new, length):
+    """Each channel's infinity or NaN reaches the rows that see it, as the
+    formula has it, and no other channel or row."""
+    say("non-finite seen", HD, new, length)
+    s = attention_case(18, [new], [length], QH, KVH, HD, 16)
+    page = s["table"][0]
+    start = length - new
+    odd = {5: (1, float("nan")), 40: (7, float("inf")), start + new // 2: (9, float("-inf")), start + new // 2 + 1: (11, float("nan"))}
+    clean = s["v"].clone()
+    for j, (c, x) in odd.items():
+        s["v"][int(page[j // 16]), j % 16, :, c] = x
+        clean[int(page[j // 16]), j % 16, :, c] = 0
+    got = run_attention(s).cpu().double()
+    want, tol = ref.attention(s["q"], s["k"].cpu(), clean.cpu(), s["table"], s["row_start"], s["lengths"], s["scale"])
+    for t in range(new):
+        for j, (c, x) in odd.items():
+            if j <= start + t:
+                assert bool((torch.isnan(got[t, :, c]) if x != x else got[t, :, c] == x).all()), (t, j, c)
+                got[t, :, c] = want[t, :, c]
+    assert bool(((got - want).abs() <= tol).all())
 
 
 def test_attention_extreme_scores():
