@@ -63,7 +63,7 @@ def _flat(name, t, dtype, count, device):
 def _stream(device, stream):
     """The raw stream of a call, and what its new tensors are made under."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, _HERE
+        return torch._C._cuda_getCurrentRawStream(device.index), _HERE  # a Stream object would take a tenth of the call
     if stream.device != device:
         raise ValueError(f"the stream is {stream.device}'s, the tensors {device}'s")
     return stream.cuda_stream, torch.cuda.stream(stream)
@@ -171,9 +171,9 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
         raise ValueError(f"positions must be [axes, {rows}] with contiguous rows, not {tuple(positions.shape)}")
     slots = _flat("slots", slots, _I32, rows, device)
     if pair_axis is not None:
-        if len(pair_axis) != pairs or not all(0 <= int(x) < axes for x in pair_axis):
+        if len(pair_axis) != pairs or not 0 <= min(pair_axis) <= max(pair_axis) < axes:
             raise ValueError(f"pair_axis must name one of {axes} axes for each of {pairs} pairs")
-        pair_axis = (ctypes.c_uint8 * pairs)(*[int(x) for x in pair_axis])
+        pair_axis = bytes(pair_axis)
     raw, under = _stream(device, stream)
     if out is None:
         with under:

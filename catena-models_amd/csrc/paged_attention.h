@@ -360,8 +360,8 @@ struct Rows {
   }
 
   // Scores of N tiles to weights; `first` is the first tile's first key, `mask`
-  // where some of the keys are not seen by some column (bad: two bits a tile), `fresh`
-  // in front of the first product.
+  // where some of the keys are not seen by some column (bad: two bits a tile),
+  // `fresh` in front of the first product.
   template <int N>
   __device__ __forceinline__ void weights(const AttendArgs& a, f32x16_t (&t)[N], bool mask, int first, int bad, bool fresh,
                                           u32x4 (&w)[N][2]) {
@@ -770,6 +770,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
       if (i + ahead - 1 < stages) arrived_but<kOwn>();
       else arrived_but<0>();
       __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");  // no LDS read of the stages in front of it
       __builtin_amdgcn_sched_barrier(0);
       if (i + ahead < stages) request(i + ahead);
     };

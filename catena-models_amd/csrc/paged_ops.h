@@ -170,7 +170,7 @@ extern "C" int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_head
   int rc = check_cache(cache);
   if (!rc) rc = check_q_heads(cache, q_heads);
   if (rc) return rc;
-  if (rows < 0 || rows > INT32_MAX) return fail(CQ35_ERANGE, "paged prepare: %lld rows", (long long)rows);
+  if (rows < 0 || rows > 1 << 26) return fail(CQ35_ERANGE, "paged prepare: %lld rows, not up to 2^26", (long long)rows);
   if (rope_dim < 16 || rope_dim > cache->head_dim || rope_dim % 16)
     return fail(CQ35_EINVAL, "paged prepare: rotary width %d of heads of %d is not a multiple of 16", rope_dim,
                 cache->head_dim);
@@ -221,13 +221,14 @@ constexpr int kFewPacked = 64;
 constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
 constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
 constexpr int kMostSplits = 1024;
+constexpr int64_t kMostBlocks = 1 << 22;  // times 512 threads: a launch takes below 2^32
 constexpr int kWideJoin = 512;  // units of 32 packed rows and KV head
 
 struct AttendPlan {
   bool few;
   CutRule cut;
-  int64_t tiles;   // row tiles per KV head at most
-  int64_t floats;  // of workspace
+  int64_t items, units;  // at most: blocks of the attention, 32-row groups of the join
+  int64_t floats;        // of workspace
 };
 
 AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
@@ -241,8 +242,10 @@ AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_he
   c.search = !p.few;
   const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
   c.max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, (key_tiles + c.min_tiles - 1) / c.min_tiles));
-  p.tiles = most_tiles(rows, requests, group, c.tile_rows);
-  c.slots = most_slots(p.tiles, kv_heads, c.target_shift, c.max_splits);
+  const int64_t tiles = most_tiles(rows, requests, group, c.tile_rows);
+  p.items = most_items(tiles, kv_heads, c.target_shift, c.max_splits);
+  p.units = tiles * kv_heads * (c.tile_rows / 32);
+  c.slots = most_slots(tiles, kv_heads, c.target_shift, c.max_splits);
   p.floats = c.slots * (c.tile_rows / 32) * (32 * (int64_t)head_dim + 64);
   return p;
 }
@@ -257,24 +260,24 @@ int check_attention_sizes(const char* what, int64_t rows, int64_t requests, int3
       rows > INT32_MAX / (q_heads / kv_heads))
     return fail(CQ35_ERANGE, "%s: %lld rows of %lld requests, at most %lld rows and %lld keys each", what, (long long)rows,
                 (long long)requests, (long long)max_rows, (long long)max_keys);
+  const AttendPlan p = plan_attention(rows, requests, q_heads, kv_heads, head_dim, max_rows, max_keys);
+  if (p.items > kMostBlocks || p.units > kMostBlocks)
+    return fail(CQ35_ERANGE, "%s: too many rows for one call: %lld", what, (long long)rows);
   return CQ35_OK;
 }
 
 template <int HD>
 int launch_attention(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
-  const int64_t items = most_items(p.tiles, a.cut.kv_heads, a.cut.target_shift, a.cut.max_splits);
-  const int64_t units = p.tiles * a.cut.kv_heads * (a.cut.tile_rows / 32);
-  if (items > INT32_MAX || units > INT32_MAX) return fail(CQ35_ERANGE, "paged attention: too many rows for one call");
   auto kernel = p.few ? k_paged_few<HD> : k_paged_many<HD>;
   // a block a channel tile where there are few rows, all of them where there are many
-  const bool wide = units >= kWideJoin;
+  const bool wide = p.units >= kWideJoin;
   auto join = p.few ? (wide ? k_paged_join<HD, 1, HD / 32> : k_paged_join<HD, 1, 1>)
                     : (wide ? k_paged_join<HD, kManyRows / 32, HD / 32> : k_paged_join<HD, kManyRows / 32, 1>);
   const size_t lds = p.few ? few_lds_bytes<HD>() : many_lds_bytes<HD>();
   if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  int rc = launch_operator("paged attention", kernel, dim3((unsigned)items), p.few ? kFewThreads : kManyThreads, lds, s, a);
+  int rc = launch_operator("paged attention", kernel, dim3((unsigned)p.items), p.few ? kFewThreads : kManyThreads, lds, s, a);
   if (!rc && a.cut.slots > 0)
-    rc = launch_operator("paged attention", join, dim3((unsigned)units, wide ? 1 : HD / 32), kJoinThreads, 0, s, a);
+    rc = launch_operator("paged attention", join, dim3((unsigned)p.units, wide ? 1 : HD / 32), kJoinThreads, 0, s, a);
   return rc;
 }
 
@@ -301,9 +304,9 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
   if (rc) return rc;
   if (rows == 0 || requests == 0) return CQ35_OK;
   if (!table || !row_start || !lengths) return fail(CQ35_EINVAL, "paged attention: null argument");
-  if (width < 1 || width > INT32_MAX / cache->page_size || table_stride < 0)
+  if (width < 1 || width > (1 << 30) / cache->page_size || table_stride < 0)
     return fail(CQ35_ERANGE, "paged attention: tables of %lld pages", (long long)width);
-  if (!std::isfinite(scale)) return fail(CQ35_EINVAL, "paged attention: scale %g", (double)scale);
+  if (!std::isfinite(scale * 1.44269504f)) return fail(CQ35_EINVAL, "paged attention: scale %g", (double)scale);
   rc = check_heads("paged attention: queries", q, rows, q_heads, cache->head_dim, false);
   if (!rc && gate) rc = check_heads("paged attention: gate", gate, rows, q_heads, cache->head_dim, false);
   if (!rc) rc = check_heads("paged attention: output", out, rows, q_heads, cache->head_dim, true);

@@ -404,7 +404,7 @@ int cq35_page_plan(int32_t* table, int64_t table_stride, int64_t requests, int64
  * 64 bits, each result rounded to BF16 once. q_out may be q itself, laid out
  * alike. A row whose slot is negative or past the cache is left alone: neither
  * its query nor the cache is written. Slots of one call differ; of two equal
- * ones either row may end up in the cache, piece by piece. */
+ * ones either row may end up in the cache, piece by piece. Up to 2^26 rows. */
 int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const cq35_heads* k,
                        const cq35_heads* v, int64_t rows, int32_t q_heads, const float* q_weight,
                        const float* k_weight, float eps, const float* inv_freq, int32_t rope_dim,
@@ -423,14 +423,14 @@ int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const
  * the second product as BF16 (relative error 2^-9 each, as the values they
  * meet), the sums and the running maximum stay F32, the result is rounded to
  * BF16 once. The same call gives the same bits.
- * A row that sees no key (p < 0) gets zeros. Keys in pages whose number is
- * outside the cache are not seen; lengths are cut to what the table holds.
- * Rows outside every request are left alone; up to 8192 requests, rows *
- * q_heads / kv_heads below 2^31. out may be q itself, laid out
- * alike; it overlaps no other operand.
- * max_rows and max_keys are what the caller knows of the most rows and keys
- * of any request, 0 for nothing: they steer how the work is cut and the
- * launches spared, results hold whatever they say.
+ * A row that sees no key (p < 0), or none with a score above -inf, gets zeros.
+ * Keys in pages whose number is outside the cache are not seen; lengths are
+ * cut to what the table holds (at most 2^30 keys). Rows outside every request
+ * are left alone. Up to 8192 requests; rows * q_heads below about 2^27. out may be
+ * q itself, laid out alike; it overlaps no other operand.
+ * max_rows and max_keys are what the caller knows of the most rows and keys of
+ * any request, 0 for nothing: they steer how the work is cut and the launches
+ * spared, results hold whatever they say.
  * workspace: cq35_paged_attention_workspace bytes (of the same arguments) at
  * a 16-byte address, used during the call's work only and by no other work at
  * that time; NULL where 0 bytes are needed. */

@@ -67,6 +67,7 @@ def test_cache_refusals(change, code, text):
     (dict(max_rows=-1), -2, "rows"),
     (dict(max_keys=-1), -2, "keys"), (dict(table=None), -1, "null"), (dict(row_start=None), -1, "null"),
     (dict(lengths=None), -1, "null"), (dict(width=0), -2, "tables"), (dict(width=1 << 28), -2, "tables"),
+    (dict(width=(1 << 26) + 1), -2, "tables"), (dict(scale=3e38), -1, "scale"), (dict(rows=1 << 29, q_heads=2), -2, "rows"),
     (dict(table_stride=-1), -2, "tables"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"),
     (dict(q=heads(BASE + 4)), -1, "16-byte"), (dict(q=heads(None)), -1, "null"), (dict(q=heads(row=130)), -1, "multiples of 8"),
     (dict(q=heads(head=-64)), -1, "multiples of 8"), (dict(out=heads(row=128)), -1, "overlap"),
@@ -85,7 +86,7 @@ def prepare(c=None, q=None, k=None, v=None, rows=3, q_heads=4, qw=BASE, kw=BASE,
 
 
 @pytest.mark.parametrize("change,code,text", [
-    (dict(rows=-1), -2, "rows"), (dict(q_heads=5), -1, "query heads"), (dict(rope=8), -1, "rotary"), (dict(rope=24), -1, "rotary"),
+    (dict(rows=-1), -2, "rows"), (dict(rows=(1 << 26) + 1), -2, "rows"), (dict(q_heads=5), -1, "query heads"), (dict(rope=8), -1, "rotary"), (dict(rope=24), -1, "rotary"),
     (dict(rope=80), -1, "rotary"), (dict(axes=0), -1, "axes"), (dict(axes=5), -1, "axes"), (dict(axes=3), -1, "each pair"),
     (dict(pair_axis=(ctypes.c_uint8 * 8)(0, 0, 0, 1)), -1, "pair 3"), (dict(eps=-1.0), -1, "eps"), (dict(eps=float("nan")), -1, "eps"),
     (dict(qw=None), -1, "null"), (dict(kw=None), -1, "null"), (dict(freq=None), -1, "null"), (dict(pos=None), -1, "null"),
