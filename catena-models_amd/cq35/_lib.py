@@ -100,6 +100,8 @@ def load():
         "cq35_step_static": ([P, P, I64, U64, I64, P, ctypes.POINTER(U64), P], ctypes.c_int),
         "cq35_session_set_attention_split": ([P, I64], ctypes.c_int),
         "cq35_session_attention_split": ([P, ctypes.POINTER(I64)], ctypes.c_int),
+        "cq35_session_set_online_attention": ([P, ctypes.c_int], ctypes.c_int),
+        "cq35_session_online_attention": ([P, ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
         "cq35_page_plan": ([P, I64, I64, I64, P, P, P, I64, P, I32, I64, P, P, P, P, P, P], ctypes.c_int),
         "cq35_paged_prepare": ([PG, PH, PH, PH, I64, I32, P, P, ctypes.c_float, P, I32, P, I64, I32, P, P, PH, P],
                                ctypes.c_int),
@@ -137,5 +139,6 @@ EXPORTED = [
     "cq35_gguf_config", "cq35_gguf_validate", "cq35_model_load_gguf", "cq35_gguf_tensor_name",
     "cq35_step_batch", "cq35_step_static", "cq35_session_set_attention_split",
     "cq35_session_attention_split", "cq35_session_phase_trace",
+    "cq35_session_set_online_attention", "cq35_session_online_attention",
     "cq35_page_plan", "cq35_paged_prepare", "cq35_paged_attention_workspace", "cq35_paged_attention",
 ]

@@ -334,6 +334,18 @@ class Session:
         check(_lib.load().cq35_session_matrix_prefill(self._h, ctypes.byref(v)))
         return v.value
 
+    def set_online_attention(self, enabled: bool) -> None:
+        """Run the MATRIX_ATTENTION component of multi-token calls as one pass
+        over the keys (the paged attention operator over the session's cache;
+        scores and sums in F32) instead of the reference's rounding points."""
+        check(_lib.load().cq35_session_set_online_attention(self._h, 1 if enabled else 0))
+
+    @property
+    def online_attention(self) -> bool:
+        v = ctypes.c_int()
+        check(_lib.load().cq35_session_online_attention(self._h, ctypes.byref(v)))
+        return bool(v.value)
+
     def set_matrix_decode(self, enabled: bool) -> None:
         """Let cq35_step_batch run the weight-shared step's products on MFMA
         (tolerance-level) when every session of the batch has this set; a

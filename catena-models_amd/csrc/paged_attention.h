@@ -29,6 +29,7 @@
 // and those of pages outside the cache are never read: zeros take their place.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "mfma.h"
@@ -913,6 +914,88 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
     if (!row) continue;
     if (a.gate) to.template write<true>(8 * (quad0 + 4 * j) + 4 * h, v.x, v.y, v.z, v.w);
     else to.template write<false>(8 * (quad0 + 4 * j) + 4 * h, v.x, v.y, v.z, v.w);
+  }
+}
+
+// ------------------------------------------------------------- host side
+
+// How a call of paged attention is cut: requests of up to kFewPacked packed
+// rows (rows times query heads of a KV head) go to k_paged_few, one longer
+// request takes them all to k_paged_many. max_rows decides without the lengths,
+// max_keys spares the join where no request can be split.
+constexpr int kFewPacked = 64;
+constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
+constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
+constexpr int kMostSplits = 1024;
+constexpr int64_t kMostBlocks = 1 << 22;  // times 512 threads: a launch takes below 2^32
+constexpr int kWideJoin = 512;  // units of 32 packed rows and KV head
+
+struct AttendPlan {
+  bool few;
+  CutRule cut;
+  int64_t items, units;  // at most: blocks of the attention, 32-row groups of the join
+  int64_t floats;        // of workspace
+};
+
+inline AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
+                          int64_t max_keys) {
+  AttendPlan p{};
+  const int group = q_heads / kv_heads;
+  p.few = (max_rows > 0 ? std::min(max_rows, rows) : rows) * group <= kFewPacked;
+  CutRule& c = p.cut;
+  c.rows = (int32_t)rows, c.group = group, c.kv_heads = kv_heads, c.tile_rows = p.few ? kFewRows : kManyRows;
+  c.target_shift = p.few ? kFewTarget : kManyTarget, c.min_tiles = p.few ? kFewMinTiles : kManyMinTiles;
+  c.search = !p.few;
+  const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
+  c.max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, (key_tiles + c.min_tiles - 1) / c.min_tiles));
+  const int64_t tiles = most_tiles(rows, requests, group, c.tile_rows);
+  p.items = most_items(tiles, kv_heads, c.target_shift, c.max_splits);
+  p.units = tiles * kv_heads * (c.tile_rows / 32);
+  c.slots = most_slots(tiles, kv_heads, c.target_shift, c.max_splits);
+  p.floats = c.slots * (c.tile_rows / 32) * (32 * (int64_t)head_dim + 64);
+  return p;
+}
+
+struct AttendKernels {
+  void (*attend)(AttendArgs);
+  void (*join)(AttendArgs);
+  dim3 grid, join_grid;
+  int threads;
+  size_t lds;
+};
+
+template <int HD>
+AttendKernels attend_kernels(const AttendPlan& p) {
+  // a block a channel tile where there are few rows, all of them where there are many
+  const bool wide = p.units >= kWideJoin;
+  AttendKernels k;
+  k.attend = p.few ? k_paged_few<HD> : k_paged_many<HD>;
+  k.join = p.few ? (wide ? k_paged_join<HD, 1, HD / 32> : k_paged_join<HD, 1, 1>)
+                 : (wide ? k_paged_join<HD, kManyRows / 32, HD / 32> : k_paged_join<HD, kManyRows / 32, 1>);
+  k.grid = dim3((unsigned)p.items), k.join_grid = dim3((unsigned)p.units, wide ? 1 : HD / 32);
+  k.threads = p.few ? kFewThreads : kManyThreads;
+  k.lds = p.few ? few_lds_bytes<HD>() : many_lds_bytes<HD>();
+  return k;
+}
+
+inline void attend_scale(AttendArgs* a, float scale) {
+  a->scale2 = scale == 0.0f ? 1.0f : (scale < 0.0f ? -scale : scale) * 1.44269504f;
+  a->q_and = scale == 0.0f ? 0u : ~0u, a->q_xor = scale < 0.0f ? 0x80008000u : 0u;
+}
+
+// One request over a contiguous cache: its rows, length and a table of pages
+// that follow each other, for attention over the session's own cache.
+constexpr int kSpanShift = 16, kSpanTable = 64;  // rows of a page (log2), pages
+struct PromptSpan {
+  int32_t row_start[2], length, pad;
+  int32_t table[kSpanTable];
+};
+__global__ void k_prompt_span(const uint64_t* __restrict__ params, int t, int rows_n, PromptSpan* __restrict__ span) {
+  const int i = threadIdx.x;
+  if (i < kSpanTable) span->table[i] = i;
+  if (i == 0) {
+    span->row_start[0] = 0, span->row_start[1] = rows_n;
+    span->length = (int32_t)(step_position(params, t) + rows_n);
   }
 }
 

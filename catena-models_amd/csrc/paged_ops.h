@@ -213,43 +213,6 @@ extern "C" int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_head
 
 namespace {
 
-// How a call of paged attention is cut: requests of up to kFewPacked packed
-// rows (rows times query heads of a KV head) go to k_paged_few, one longer
-// request takes them all to k_paged_many. max_rows decides without the lengths,
-// max_keys spares the join where no request can be split.
-constexpr int kFewPacked = 64;
-constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
-constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
-constexpr int kMostSplits = 1024;
-constexpr int64_t kMostBlocks = 1 << 22;  // times 512 threads: a launch takes below 2^32
-constexpr int kWideJoin = 512;  // units of 32 packed rows and KV head
-
-struct AttendPlan {
-  bool few;
-  CutRule cut;
-  int64_t items, units;  // at most: blocks of the attention, 32-row groups of the join
-  int64_t floats;        // of workspace
-};
-
-AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
-                          int64_t max_keys) {
-  AttendPlan p{};
-  const int group = q_heads / kv_heads;
-  p.few = (max_rows > 0 ? std::min(max_rows, rows) : rows) * group <= kFewPacked;
-  CutRule& c = p.cut;
-  c.rows = (int32_t)rows, c.group = group, c.kv_heads = kv_heads, c.tile_rows = p.few ? kFewRows : kManyRows;
-  c.target_shift = p.few ? kFewTarget : kManyTarget, c.min_tiles = p.few ? kFewMinTiles : kManyMinTiles;
-  c.search = !p.few;
-  const int64_t key_tiles = max_keys > 0 ? (std::min<int64_t>(max_keys, INT32_MAX) + kKeyTile - 1) / kKeyTile : INT32_MAX;
-  c.max_splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, (key_tiles + c.min_tiles - 1) / c.min_tiles));
-  const int64_t tiles = most_tiles(rows, requests, group, c.tile_rows);
-  p.items = most_items(tiles, kv_heads, c.target_shift, c.max_splits);
-  p.units = tiles * kv_heads * (c.tile_rows / 32);
-  c.slots = most_slots(tiles, kv_heads, c.target_shift, c.max_splits);
-  p.floats = c.slots * (c.tile_rows / 32) * (32 * (int64_t)head_dim + 64);
-  return p;
-}
-
 int check_attention_sizes(const char* what, int64_t rows, int64_t requests, int32_t q_heads, int32_t kv_heads,
                           int32_t head_dim, int64_t max_rows, int64_t max_keys) {
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
@@ -268,16 +231,10 @@ int check_attention_sizes(const char* what, int64_t rows, int64_t requests, int3
 
 template <int HD>
 int launch_attention(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
-  auto kernel = p.few ? k_paged_few<HD> : k_paged_many<HD>;
-  // a block a channel tile where there are few rows, all of them where there are many
-  const bool wide = p.units >= kWideJoin;
-  auto join = p.few ? (wide ? k_paged_join<HD, 1, HD / 32> : k_paged_join<HD, 1, 1>)
-                    : (wide ? k_paged_join<HD, kManyRows / 32, HD / 32> : k_paged_join<HD, kManyRows / 32, 1>);
-  const size_t lds = p.few ? few_lds_bytes<HD>() : many_lds_bytes<HD>();
-  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  int rc = launch_operator("paged attention", kernel, dim3((unsigned)p.items), p.few ? kFewThreads : kManyThreads, lds, s, a);
-  if (!rc && a.cut.slots > 0)
-    rc = launch_operator("paged attention", join, dim3((unsigned)p.units, wide ? 1 : HD / 32), kJoinThreads, 0, s, a);
+  const AttendKernels k = attend_kernels<HD>(p);
+  if (k.lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)k.attend, hipFuncAttributeMaxDynamicSharedMemorySize, (int)k.lds));
+  int rc = launch_operator("paged attention", k.attend, k.grid, k.threads, k.lds, s, a);
+  if (!rc && a.cut.slots > 0) rc = launch_operator("paged attention", k.join, k.join_grid, kJoinThreads, 0, s, a);
   return rc;
 }
 
@@ -330,8 +287,7 @@ extern "C" int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_he
   a.shift = page_shift(cache->page_size), a.table = table, a.table_stride = table_stride;
   a.row_start = row_start, a.lengths = lengths, a.requests = (int)requests;
   a.cut = p.cut, a.cut.most_keys = (int32_t)(width * cache->page_size), a.part = static_cast<float*>(workspace);
-  a.scale2 = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
-  a.q_and = scale == 0.0f ? 0u : ~0u, a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
+  attend_scale(&a, scale);
   if (cache->head_dim == 256) return launch_attention<256>(a, p, s);
   if (cache->head_dim == 128) return launch_attention<128>(a, p, s);
   return launch_attention<64>(a, p, s);

@@ -26,6 +26,7 @@
 #include "prefill.h"
 #include "bgemm.h"
 #include "mfma.h"
+#include "paged_attention.h"
 #include "gguf.h"
 #include "workspace.h"
 #include "batch.h"
@@ -813,6 +814,7 @@ struct cq35_session {
   uint32_t seq = 0;
   int prefill_rows = 0;    // token rows per chunk of multi-token calls (0: the rule of prefill_buffers)
   int matrix = 0;          // CQ35_MATRIX_* components of multi-token calls on MFMA
+  int online_attention = 0;  // the attention component as one pass (k_paged_many)
   int matrix_decode = 0;   // weight-shared batched decode products on MFMA
   int64_t split_keys = CQ35_SPLIT_KEYS_DEFAULT;  // decode attention splits above this many keys
   // kernel timing
@@ -1533,10 +1535,19 @@ struct Prefill {
   int *eoff = nullptr, *order = nullptr;    // experts: buckets
   int* tiles = nullptr;                     // matrix-core experts: tiles that hold work
   int* ids = nullptr;
+  PromptSpan* span = nullptr;  // one-pass attention: the chunk as a request
+  float* joint = nullptr;      // its splits' partial results
   uint32_t* ranges = nullptr;  // k_bgemm: magnitude ranges of a launch's weight and token tiles
   int attn_tokens = 0;         // tokens per staged-attention launch (scratch rows)
   int rows = 0;                // tokens per chunk
 };
+
+// Whether multi-token calls of this session attend in one pass.
+bool online_attention(const cq35_session* s) {
+  const int64_t hd = s->model->d.HD;
+  return s->online_attention && (s->matrix & CQ35_MATRIX_ATTENTION) && (hd == 64 || hd == 128 || hd == 256) &&
+         s->capacity <= (int64_t)kSpanTable << kSpanShift;
+}
 
 // Carve the buffers for chunks of `rows` tokens out of `base` (256-byte
 // aligned pieces). Returns the bytes needed; pointers are only assigned when
@@ -1575,6 +1586,13 @@ size_t prefill_layout(const cq35_session* s, int64_t rows, unsigned char* base, 
     take(&pf->tiles, 1 + moe_tiles(m, d.K, d.E));
     take(&pf->part, m * d.K * d.H);
     take(&pf->spart, m * d.H);
+  }
+  if (online_attention(s)) {
+    // no chunk of fewer rows needs more than the most of either kernel
+    const int group = (int)(d.Q / d.KVH);
+    auto floats = [&](int64_t n) { return plan_attention(n, 1, (int)d.Q, (int)d.KVH, (int)d.HD, n, s->capacity).floats; };
+    take(&pf->span, 1);
+    take(&pf->joint, std::max(floats(m), floats(std::min<int64_t>(m, std::max(1, kFewPacked / group)))));
   }
   // staged attention scratch rows, at most 64 MiB
   const int64_t per_token = d.Q * (int64_t)s->attn_stride;
@@ -1646,6 +1664,7 @@ void enqueue_prefill(cq35_session* s, int64_t n, const Prefill& pf) {
     const unsigned tiles = (unsigned)((rows_n + 4 * kBTokens - 1) / (4 * kBTokens));
     L(KC_EMBED, k_bembed, dim3(rows_n), dim3(kBlock), 0, params, first, (const uint16_t*)Wt(0), H,
       pf.h, c0 + rows_n == n ? s->d_best : (unsigned long long*)nullptr);
+    if (pf.span) L(KC_EMBED, k_prompt_span, dim3(1), dim3(64), 0, params, first, rows_n, pf.span);
     // matrix-core projections when selected (K a multiple of the MFMA step)
     const bool mp = (s->matrix & CQ35_MATRIX_PROJECTIONS) != 0;
     // matrix-core projections: LDS-staged tiles for widths of whole 128-column
@@ -1730,7 +1749,28 @@ void enqueue_prefill(cq35_session* s, int64_t n, const Prefill& pf) {
             first, rows_n, (int)d.KVS, (int)d.Q, (int)(d.Q / d.KVH), scale, ctx);
         };
         const bool ma = (s->matrix & CQ35_MATRIX_ATTENTION) != 0;
-        if (ma && d.HD == 256) mattention(k_mattention<256>);
+        auto online = [&](auto hd) {
+          constexpr int HD = decltype(hd)::value;
+          const AttendPlan p = plan_attention(rows_n, 1, (int)d.Q, (int)d.KVH, HD, rows_n,
+                                              (int64_t)s->h_params[0] + first + rows_n);
+          AttendArgs at{};
+          at.q = qr, at.q_row = d.QS, at.q_head = HD;
+          at.gate = qg + HD, at.gate_row = 2 * d.QS, at.gate_head = 2 * HD;
+          at.out = ctx, at.out_row = d.QS, at.out_head = HD;
+          at.keys = s->cache + key_base, at.values = s->cache + value_base;
+          at.pages = (cap + (1 << kSpanShift) - 1) >> kSpanShift, at.page_stride = d.KVS << kSpanShift;
+          at.row_stride = d.KVS, at.head_stride = HD, at.shift = kSpanShift;
+          at.table = pf.span->table, at.row_start = pf.span->row_start, at.lengths = &pf.span->length, at.requests = 1;
+          attend_scale(&at, scale);
+          at.cut = p.cut, at.cut.most_keys = (int32_t)cap, at.part = pf.joint;
+          const AttendKernels k = attend_kernels<HD>(p);
+          L(KC_ATTENTION, k.attend, k.grid, dim3(k.threads), k.lds, at);
+          if (at.cut.slots > 0) L(KC_ATTENTION, k.join, k.join_grid, dim3(kJoinThreads), 0, at);
+        };
+        if (pf.span && d.HD == 256) online(std::integral_constant<int, 256>{});
+        else if (pf.span && d.HD == 128) online(std::integral_constant<int, 128>{});
+        else if (pf.span) online(std::integral_constant<int, 64>{});
+        else if (ma && d.HD == 256) mattention(k_mattention<256>);
         else if (ma && d.HD == 128) mattention(k_mattention<128>);
         else if (ma && d.HD == 64) mattention(k_mattention<64>);
         else {  // the exact staged kernels
@@ -2077,6 +2117,35 @@ extern "C" int cq35_session_set_matrix_prefill(cq35_session* s, int components) 
 extern "C" int cq35_session_matrix_prefill(const cq35_session* s, int* components) {
   if (!s || !components) return fail(CQ35_EINVAL, "null argument");
   *components = s->matrix;
+  return CQ35_OK;
+}
+
+extern "C" int cq35_session_set_online_attention(cq35_session* s, int enabled) {
+  if (!s) return fail(CQ35_EINVAL, "null argument");
+  if (enabled != 0 && enabled != 1) return fail(CQ35_EINVAL, "one-pass attention option must be 0 or 1, not %d", enabled);
+  const int64_t hd = s->model->d.HD;
+  if (enabled && hd != 64 && hd != 128 && hd != 256)
+    return fail(CQ35_EUNSUPPORTED, "one-pass attention: head_dim %lld is not 64, 128 or 256", (long long)hd);
+  if (enabled) {
+    HIP_TRY(hipSetDevice(s->model->device));
+    auto optin = [](const void* few, size_t few_lds, const void* many, size_t many_lds) {
+      hipError_t e = hipSuccess;
+      if (few_lds > 65536) e = hipFuncSetAttribute(few, hipFuncAttributeMaxDynamicSharedMemorySize, (int)few_lds);
+      if (e == hipSuccess && many_lds > 65536)
+        e = hipFuncSetAttribute(many, hipFuncAttributeMaxDynamicSharedMemorySize, (int)many_lds);
+      return e;
+    };
+    HIP_TRY(hd == 256   ? optin((const void*)k_paged_few<256>, few_lds_bytes<256>(), (const void*)k_paged_many<256>, many_lds_bytes<256>())
+            : hd == 128 ? optin((const void*)k_paged_few<128>, few_lds_bytes<128>(), (const void*)k_paged_many<128>, many_lds_bytes<128>())
+                        : optin((const void*)k_paged_few<64>, few_lds_bytes<64>(), (const void*)k_paged_many<64>, many_lds_bytes<64>()));
+  }
+  s->online_attention = enabled;
+  return CQ35_OK;
+}
+
+extern "C" int cq35_session_online_attention(const cq35_session* s, int* enabled) {
+  if (!s || !enabled) return fail(CQ35_EINVAL, "null argument");
+  *enabled = s->online_attention;
   return CQ35_OK;
 }
 
@@ -2865,6 +2934,7 @@ extern "C" int cq35_session_copy(const cq35_session* src, cq35_session** out) {
   }
   s->graph_enabled = src->graph_enabled;
   s->matrix = src->matrix;  // session options travel with the state
+  s->online_attention = src->online_attention;
   s->matrix_decode = src->matrix_decode;
   if (src->split_keys != s->split_keys) {
     const int r = cq35_session_set_attention_split(s, src->split_keys);

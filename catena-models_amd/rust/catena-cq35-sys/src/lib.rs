@@ -69,6 +69,28 @@ pub struct cq35_session {
     _p: [u8; 0],
 }
 
+/// Pages of keys and values in device memory (cq35_paged_cache).
+#[repr(C)]
+pub struct cq35_paged_cache {
+    pub keys: *mut c_void,
+    pub values: *mut c_void,
+    pub pages: i64,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+    pub page_stride: i64,
+    pub row_stride: i64,
+    pub head_stride: i64,
+}
+
+/// Rows of heads in device memory (cq35_heads).
+#[repr(C)]
+pub struct cq35_heads {
+    pub data: *mut c_void,
+    pub row_stride: i64,
+    pub head_stride: i64,
+}
+
 extern "C" {
     pub fn cq35_last_error() -> *const c_char;
     pub fn cq35_abi_version() -> c_int;
@@ -99,7 +121,24 @@ extern "C" {
     pub fn cq35_session_set_persistent(session: *mut cq35_session, enabled: c_int) -> c_int;
     pub fn cq35_session_set_attention_split(session: *mut cq35_session, keys: i64) -> c_int;
     pub fn cq35_session_set_matrix_prefill(session: *mut cq35_session, components: c_int) -> c_int;
+    pub fn cq35_session_set_online_attention(session: *mut cq35_session, enabled: c_int) -> c_int;
     pub fn cq35_session_set_matrix_decode(session: *mut cq35_session, enabled: c_int) -> c_int;
+    pub fn cq35_page_plan(table: *mut i32, table_stride: i64, requests: i64, width: i64, cached: *const i32,
+                          lengths: *const i32, free_pages: *mut i32, pages: i64, free_count: *const i32, page_size: i32,
+                          rows: i64, row_start: *mut i32, positions: *mut i32, slots: *mut i32, free_left: *mut i32,
+                          status: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn cq35_paged_prepare(cache: *const cq35_paged_cache, q: *const cq35_heads, k: *const cq35_heads,
+                              v: *const cq35_heads, rows: i64, q_heads: i32, q_weight: *const f32, k_weight: *const f32,
+                              eps: f32, inv_freq: *const f32, rope_dim: i32, positions: *const i32, position_stride: i64,
+                              axes: i32, pair_axis: *const u8, slots: *const i32, q_out: *const cq35_heads,
+                              stream: *mut c_void) -> c_int;
+    pub fn cq35_paged_attention_workspace(rows: i64, requests: i64, q_heads: i32, kv_heads: i32, head_dim: i32,
+                                          max_rows: i64, max_keys: i64, bytes: *mut i64) -> c_int;
+    pub fn cq35_paged_attention(cache: *const cq35_paged_cache, q: *const cq35_heads, gate: *const cq35_heads,
+                                out: *const cq35_heads, rows: i64, q_heads: i32, table: *const i32, table_stride: i64,
+                                requests: i64, width: i64, row_start: *const i32, lengths: *const i32, scale: f32,
+                                max_rows: i64, max_keys: i64, workspace: *mut c_void, workspace_bytes: i64,
+                                stream: *mut c_void) -> c_int;
 }
 
 /// `Ok(())` for CQ35_OK, else the code with the library's message for this thread.
@@ -198,6 +237,12 @@ impl<'m> Session<'m> {
     /// InferenceOptions::wmma_prefill (src/catena.rs:12-26): CQ35_MATRIX_* bits.
     pub fn set_matrix_prefill(&mut self, components: c_int) -> anyhow::Result<()> {
         check(unsafe { cq35_session_set_matrix_prefill(self.raw, components) })
+    }
+
+    /// The attention component of `set_matrix_prefill` as one pass over the
+    /// keys (tolerance-level; no reference counterpart).
+    pub fn set_online_attention(&mut self, enabled: bool) -> anyhow::Result<()> {
+        check(unsafe { cq35_session_set_online_attention(self.raw, enabled as c_int) })
     }
 
     /// Matrix-core products in `step_batch` when every session of the batch

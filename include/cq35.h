@@ -269,6 +269,18 @@ int cq35_session_attention_split(const cq35_session* session, int64_t* keys);
 int cq35_session_set_matrix_prefill(cq35_session* session, int components);
 int cq35_session_matrix_prefill(const cq35_session* session, int* components);
 
+/* One-pass attention of multi-token calls (no reference counterpart): 1 runs
+ * the attention component (CQ35_MATRIX_ATTENTION, which has to be selected for
+ * it to matter) as cq35_paged_attention over the session's cache: a running
+ * maximum and sum instead of two passes over the keys, scores and probabilities
+ * kept in F32 where the reference's matrix-core path rounds them to BF16 (the
+ * unnormalised weights enter the second product as BF16), keys split over the
+ * device where a chunk has few rows (so a call's chunks change its rounding).
+ * Tolerance-level, as the component is; 0 (the default) keeps the reference's rounding points. head_dim 64, 128 or 256.
+ * Prompt buffers hold up to 135 MB more. Copied by cq35_session_copy. */
+int cq35_session_set_online_attention(cq35_session* session, int enabled);
+int cq35_session_online_attention(const cq35_session* session, int* enabled);
+
 /* Matrix-core batched decode (no reference counterpart): 1 lets the
  * weight-shared step of cq35_step_batch run its products on MFMA (hardware
  * accumulation order, tolerance-level) for a batch in which EVERY session has
