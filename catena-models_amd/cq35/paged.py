@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -86,28 +87,31 @@ def _heads(name, t, rows, heads, head_dim, device):
 def _cache(key_cache, value_cache):
     _tensor("key_cache", key_cache, _BF16, 4)
     _tensor("value_cache", value_cache, _BF16, 4, key_cache.device)
-    shape = key_cache.shape
-    if shape != value_cache.shape:
-        raise ValueError(f"key_cache {tuple(shape)} and value_cache {tuple(value_cache.shape)} differ")
-    if 0 in shape:
+    if key_cache.shape != value_cache.shape:
+        raise ValueError(f"key_cache {tuple(key_cache.shape)} and value_cache {tuple(value_cache.shape)} differ")
+    pages, page_size, kv_heads, head_dim = key_cache.shape
+    if not (pages and page_size and kv_heads and head_dim):
         raise ValueError("an empty cache")
-    ks, vs = key_cache.stride(), value_cache.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    # the stride of a dimension of length one addresses nothing
+    page, row, head, channel = strides = key_cache.stride()
+    other = value_cache.stride()
+    if channel != 1 or other[3] != 1:
         raise ValueError("the channels of a cached head must be contiguous")
-    strides = [k if n > 1 else 0 for n, k in zip(shape[:3], ks)]
-    if ks != vs and strides != [v if n > 1 else 0 for n, v in zip(shape[:3], vs)]:
+    if strides != other and any(n > 1 and x != y for n, x, y in zip(key_cache.shape, strides, other)):
         raise ValueError("key_cache and value_cache have different strides")
-    pages, page_size, kv_heads, head_dim = shape
-    return _lib.PagedCache(key_cache.data_ptr(), value_cache.data_ptr(), pages, page_size, kv_heads, head_dim, *strides)
+    return _lib.PagedCache(key_cache.data_ptr(), value_cache.data_ptr(), pages, page_size, kv_heads, head_dim,
+                           page if pages > 1 else 0, row if page_size > 1 else 0, head if kv_heads > 1 else 0)
 
 
 def _table(table, requests, device):
     _tensor("table", table, _I32, 2, device)
-    if requests is not None and table.shape[0] != requests:
-        raise ValueError(f"table must have {requests} rows, not {table.shape[0]}")
-    if table.shape[1] > 1 and table.stride(1) != 1:
+    count, width = table.shape
+    if requests is not None and count != requests:
+        raise ValueError(f"table must have {requests} rows, not {count}")
+    row, entry = table.stride()
+    if entry != 1 and width > 1:
         raise ValueError("the entries of a table row must be contiguous")
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    return row if count > 1 else width
 
 
 def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows, out=None, stream=None) -> PagePlan:
@@ -134,7 +138,7 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     sizes = (requests + 1, rows, rows, 1, 2)
     if out is None:
         with under:
-            out = PagePlan(*torch.empty(requests + 2 * rows + 4, dtype=_I32, device=device).split_with_sizes(sizes))
+            out = PagePlan(*table.new_empty(requests + 2 * rows + 4).split_with_sizes(sizes))
         at = [t.data_ptr() for t in out]
     else:
         at = [_flat("out." + name, t, _I32, n, device) for name, t, n in zip(PagePlan._fields, out, sizes)]
@@ -177,7 +181,7 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
     raw, under = _stream(device, stream)
     if out is None:
         with under:
-            out = torch.empty((rows, q_heads, cache.head_dim), dtype=_BF16, device=device)
+            out = q.new_empty((rows, q_heads, cache.head_dim))
     ho = _heads("out", out, rows, q_heads, cache.head_dim, device)
     check(_lib.load().cq35_paged_prepare(cache, hq, hk, hv, rows, q_heads, q_weight, k_weight, eps, inv_freq, 2 * pairs,
                                          positions.data_ptr(), axis_stride, axes, pair_axis, slots, ho, raw))
@@ -219,16 +223,17 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
         if workspace is None:
             have = paged_attention_workspace(rows, requests, q_heads, cache.kv_heads, cache.head_dim, max_rows, max_keys)
             if have:
-                workspace = torch.empty(have, dtype=torch.uint8, device=device)
+                workspace = q.new_empty((have + 1) // 2)
                 at = workspace.data_ptr()
         if out is None:
-            out = torch.empty((rows, q_heads, cache.head_dim), dtype=_BF16, device=device)
+            out = q.new_empty((rows, q_heads, cache.head_dim))
     ho = _heads("out", out, rows, q_heads, cache.head_dim, device)
     check(_lib.load().cq35_paged_attention(cache, hq, hg, ho, rows, q_heads, table.data_ptr(), stride, requests, table.shape[1],
                                            row_start, lengths, scale, max_rows, max_keys, at, have, raw))
     return out
 
 
+@functools.lru_cache(maxsize=1024)  # of sizes alone
 def paged_attention_workspace(rows, requests, q_heads, kv_heads, head_dim, max_rows=0, max_keys=0) -> int:
     """Bytes of workspace that paged_attention needs for these sizes."""
     b = ctypes.c_int64()
