@@ -26,7 +26,9 @@ namespace cq35 {
 // one launch does it, each block repeating the sums over the requests (a few
 // KB from L2) instead of waiting for a block that makes them.
 //
-// Latency-bound.
+// Latency-bound: 3.7 us for 8 requests, 7.3 us for 500 with 27 thousand rows,
+// 6.1 us for 64 prompts with 99 thousand (an empty launch takes about 2; the
+// sums' loads, their two reductions and the rows' search are the rest).
 constexpr int kPlanThreads = 256;
 constexpr int kPlanMostRequests = 8192;
 
@@ -156,7 +158,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
 //
 // A head is head_dim / 8 lanes of 16 bytes; a block takes `tokens` rows, makes
 // their cosines and sines once in LDS (one pair per thread) and deals the
-// rows' heads to its waves. HBM-bound.
+// rows' heads to its waves, each reading its next head while it works on one.
+// HBM-bound: 8192 rows of 16 + 2 + 2 heads of 256 take 40 us, 4.2 TB/s (a large
+// copy: 4.9); 2048 blocks of four rows against 1024 of eight: 40 and 55 us.
+// Few rows are latency-bound, 7 us for 16 to 777.
 constexpr int kPrepThreads = 256;
 constexpr int kPrepMostPairs = 128;
 constexpr int kPrepMostTokens = 8;

@@ -15,8 +15,8 @@
 // rows of a key operand and the 8 rows of a value operand spread over the
 // banks.
 //
-// The weights' rounding to BF16 (relative error 2^-9 on average half that) is
-// of the size of the values' own and an eighth of the work of F32 products;
+// The weights' rounding to BF16 (at most 2^-8 of each, as the values' own) takes
+// a sixteenth of the time that products of F32 weights would;
 // the sum of the weights takes them unrounded, in F32. A row's maximum moves
 // only when it grows by more than 8 (in units of a factor 2; the first tile
 // aside): weights stay below 2^8, exact to scale in BF16 and F32, and the
@@ -538,10 +538,10 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int kvh, Item* it
   return !item->parts || item->slot < a.cut.slots;
 }
 
-// Where an item's rows came out NaN it is done again up to the least position
-// among them, for the rows of that position, until none is left: a row whose
-// own pass is NaN is so from what it sees. The first pass, up to the item's
-// last key, writes every row that is not NaN.
+// Where rows of an item came out NaN it is done again up to the least position
+// among them, for the rows of that position, until none is left: a row whose own
+// pass is NaN is so from what it sees. The first pass, up to the item's last key,
+// writes every row that is not NaN.
 
 // The least position among the columns of the block for which `open` holds, or
 // INT32_MAX.
@@ -559,7 +559,15 @@ __device__ __forceinline__ int least_open(bool open, int pos, int* shared) {
 //
 // One item is 32 packed rows over one split of the keys; its key tiles go
 // round the four waves, each with tiles of its own in LDS and no barrier until
-// the end, where the waves' results are joined through LDS.
+// the end, where the waves' results are joined through LDS. A wave's next keys
+// are requested when its scores are made, its next values behind the context:
+// 64 KB and more are on their way per CU.
+//
+// Bound by the keys and values: 8 tokens over 14 to 32 thousand keys of 2 heads
+// of 256, 457 MB, 90 us or 5.1 TB/s (a large copy: 4.9), and 12 us for the join.
+// 512 items: one of 256 gives 125 us in all, one of 1024 (half a split each) 129.
+// A single token over 520 keys is bound by its chain of loads (request, table,
+// keys), 10.5 us: splits of four tiles, one a wave, against two: 20.3 and 21.3.
 constexpr int kFewThreads = 256;
 constexpr int kFewRows = 32;
 
@@ -698,10 +706,25 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
 // -------------------------------------------- many rows: rows over waves
 //
 // One item is 256 packed rows over one split of the keys, 32 rows a wave, two
-// waves a SIMD: one's products run beside the other's softmax. The eight waves
-// share a ring of four stages of 32 keys (of 64 for heads of up to 128
-// channels, whose tiles are short), each wave requesting an eighth, three
-// stages ahead; one barrier a stage.
+// waves a SIMD. The waves share rings of four stages of 32 keys (of 64 for heads
+// of up to 128 channels, whose tiles are short), half of them requesting the
+// keys, half the values, two to three stages ahead; one barrier a stage.
+//
+// A stage is its softmax on the vector unit and a run of products (its values',
+// the next stage's scores) on the matrix cores. The first half of the waves
+// enters a stage in front of its softmax, the second, on the same SIMDs, in
+// front of the products of the stage before, so that one's softmax meets the
+// other's products. No register of a lane is left at 256 channels (q 64, o 128,
+// scores 16, weights 8, operands under way 16): what can be made anew in the
+// loop is, since a spilled register's reload waits for all requests.
+//
+// Bound by power: 2048 tokens of 16 heads over 32768 keys of 2 heads of 256 take
+// 0.99 ms, 1.08 PFLOP/s (a large product: 1.2), the matrix cores busy half of the
+// cycles of a clock that falls from 2.3 to 1.8 - 2.0 GHz. In step, scores in a
+// run of their own: 1.08 ms; a phase apart with that run: 1.15 ms; values'
+// products and scores in one run without places in the lanes (table and strides
+// worked on every stage): 1.26 ms. Short prompts are bound by an item's start
+// and end (about 12 us with the partial results' write) and the softmax.
 constexpr int kManyThreads = 512;
 constexpr int kManyRows = 256;
 constexpr int kManyStages = 4;
@@ -919,11 +942,19 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
 
 // ------------------------------------------------------------- host side
 
-// How a call of paged attention is cut: requests of up to kFewPacked packed
-// rows (rows times query heads of a KV head) go to k_paged_few, one longer
-// request takes them all to k_paged_many. max_rows decides without the lengths,
-// max_keys spares the join where no request can be split.
-constexpr int kFewPacked = 64;
+// How a call of paged attention is cut. k_paged_few reads the keys again for
+// every 32 packed rows (rows times query heads of a KV head), k_paged_many for
+// every 256 but with an item's start and end, about 12 us. Requests of up to 32
+// packed rows, and calls whose 32-row tiles of a KV head times keys times
+// channels stay below kFewWork, go to the first. Measured in us, few and many,
+// at tiles x keys: 256 channels 512 x 600 42, 52; 128 x 4000 57, 61; 1024 x 600
+// 82, 68; 256 x 4000 90, 77; 64 x 16000 85, 76. 128 channels 256 x 4000 40, 43;
+// 512 x 4000 61, 59; 256 x 16000 116, 92. 64 channels 2048 x 600 31, 38; 512 x
+// 4000 46, 43; 256 x 16000 84, 67. max_rows and max_keys tell without the
+// lengths, a call without max_keys counts as one of kKeysAssumed; max_keys also
+// spares the join where no request can be split.
+constexpr int64_t kFewWork = 1 << 27;
+constexpr int64_t kKeysAssumed = 4096;
 constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
 constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
 constexpr int kMostSplits = 1024;
@@ -937,11 +968,11 @@ struct AttendPlan {
   int64_t floats;        // of workspace
 };
 
-inline AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
-                          int64_t max_keys) {
+inline AttendPlan cut_attention(bool few, int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim,
+                                int64_t max_keys) {
   AttendPlan p{};
   const int group = q_heads / kv_heads;
-  p.few = (max_rows > 0 ? std::min(max_rows, rows) : rows) * group <= kFewPacked;
+  p.few = few;
   CutRule& c = p.cut;
   c.rows = (int32_t)rows, c.group = group, c.kv_heads = kv_heads, c.tile_rows = p.few ? kFewRows : kManyRows;
   c.target_shift = p.few ? kFewTarget : kManyTarget, c.min_tiles = p.few ? kFewMinTiles : kManyMinTiles;
@@ -954,6 +985,21 @@ inline AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, in
   c.slots = most_slots(tiles, kv_heads, c.target_shift, c.max_splits);
   p.floats = c.slots * (c.tile_rows / 32) * (32 * (int64_t)head_dim + 64);
   return p;
+}
+
+inline AttendPlan plan_attention(int64_t rows, int64_t requests, int q_heads, int kv_heads, int head_dim, int64_t max_rows,
+                                 int64_t max_keys) {
+  const int64_t group = q_heads / kv_heads, longest = (max_rows > 0 ? std::min(max_rows, rows) : rows) * group;
+  const int64_t tiles = rows * group / kFewRows * kv_heads, keys = max_keys > 0 ? max_keys : kKeysAssumed;
+  return cut_attention(longest <= kFewRows || tiles <= kFewWork / head_dim / keys, rows, requests, q_heads, kv_heads, head_dim,
+                       max_keys);
+}
+
+// The most floats of workspace that one request of up to `rows` rows and
+// `max_keys` keys asks for.
+inline int64_t most_attend_floats(int64_t rows, int q_heads, int kv_heads, int head_dim, int64_t max_keys) {
+  return std::max(cut_attention(true, rows, 1, q_heads, kv_heads, head_dim, max_keys).floats,
+                  cut_attention(false, rows, 1, q_heads, kv_heads, head_dim, max_keys).floats);
 }
 
 struct AttendKernels {

@@ -1588,11 +1588,8 @@ size_t prefill_layout(const cq35_session* s, int64_t rows, unsigned char* base, 
     take(&pf->spart, m * d.H);
   }
   if (online_attention(s)) {
-    // no chunk of fewer rows needs more than the most of either kernel
-    const int group = (int)(d.Q / d.KVH);
-    auto floats = [&](int64_t n) { return plan_attention(n, 1, (int)d.Q, (int)d.KVH, (int)d.HD, n, s->capacity).floats; };
     take(&pf->span, 1);
-    take(&pf->joint, std::max(floats(m), floats(std::min<int64_t>(m, std::max(1, kFewPacked / group)))));
+    take(&pf->joint, most_attend_floats(m, (int)d.Q, (int)d.KVH, (int)d.HD, s->capacity));
   }
   // staged attention scratch rows, at most 64 MiB
   const int64_t per_token = d.Q * (int64_t)s->attn_stride;

@@ -432,7 +432,7 @@ int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const
  *   out = sum_j softmax_j(scale q . k_j) v_j, times sigmoid(gate) where gate
  * is not NULL; query head h reads key/value head h * kv_heads / q_heads.
  * Products on the matrix cores with F32 sums; the weights e^(s - max) enter
- * the second product as BF16 (relative error 2^-9 each, as the values they
+ * the second product as BF16 (off by at most 2^-8 each, as the values they
  * meet), the sums and the running maximum stay F32, the result is rounded to
  * BF16 once. The same call gives the same bits.
  * A row that sees no key (p < 0), or none with a score above -inf, gets zeros.

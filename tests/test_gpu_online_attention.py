@@ -108,9 +108,11 @@ def test_option_travels_and_is_checked():
     assert _lib.load().cq35_session_set_online_attention(None, 1) == -1
 
 
-def test_long_context_chunk():
-    """A chunk far into a context that is split over the device, with the other
-    components: against the two-pass kernel."""
+@pytest.mark.parametrize("held", [8900, 1500])
+def test_long_context_chunk(held):
+    """A chunk far into a context that is split over the device, and a long one
+    (of the kernel for long chunks), with the other components: against the
+    two-pass kernel."""
     cfg = dict(cc.preset("mini"))
     m = cq35.Model.synthetic(cfg, seed=9)
     ids = prompts(cfg, [9000])[0]
@@ -119,8 +121,8 @@ def test_long_context_chunk():
         s = m.session(9100)
         s.set_matrix_prefill(ATT | Session.MATRIX_PROJECTIONS)
         s.set_online_attention(on)
-        s.step_raw(ids[:8900])
-        out.append(f32(s.step_raw(ids[8900:])[0]))
+        s.step_raw(ids[:held])
+        out.append(f32(s.step_raw(ids[held:])[0]))
     r = rel_rms(out[1], out[0])
     say("long chunk: relative logit RMS %.4f" % r)
     assert r <= 0.05

@@ -304,7 +304,21 @@ def attention_case(seed, new, lengths, QH, KVH, HD, page, layout="rows", gate=Fa
                 gate=torch.randn(T, QH, HD, generator=g).to(BF) if gate else None, scale=HD ** -0.5)
 
 
+# The bounds choose the kernel besides the cut: an unknown or a small max_keys
+# leaves these sizes with the one for short work, a large one gives chunks of
+# more than 32 rows of a KV head to the one for long chunks.
+KEYS = [0]
+
+
+@pytest.fixture(params=[0, 1 << 22], ids=["short", "long"])
+def steered(request):
+    KEYS[0] = request.param
+    yield
+    KEYS[0] = 0
+
+
 def run_attention(s, **kw):
+    kw.setdefault("max_keys", KEYS[0])
     return ops().paged_attention(s["q"].cuda(), s["k"], s["v"], s["table"].cuda(), s["row_start"].cuda(), s["lengths"].cuda(),
                                  gate=None if s["gate"] is None else s["gate"].cuda(), scale=s["scale"], **kw)
 
@@ -342,7 +356,7 @@ SHAPES = [
 
 
 @pytest.mark.parametrize("new,lengths,QH,KVH,HD,page,layout,gate", SHAPES)
-def test_attention(new, lengths, QH, KVH, HD, page, layout, gate):
+def test_attention(new, lengths, QH, KVH, HD, page, layout, gate, steered):
     say("attention", new, lengths, QH, KVH, HD, page, layout, gate)
     s = attention_case(sum(lengths) + HD, new, lengths, QH, KVH, HD, page, layout, gate)
     plain = run_attention(s)
@@ -353,7 +367,7 @@ def test_attention(new, lengths, QH, KVH, HD, page, layout, gate):
     check_attention(s, run_attention(s, max_rows=1, max_keys=1))
 
 
-def test_attention_rows_that_see_nothing():
+def test_attention_rows_that_see_nothing(steered):
     """More new tokens than the request holds, no tokens at all, requests
     without rows: zeros where no key is seen."""
     for HD, new, lengths in ((64, [5, 3, 0, 4], [3, 0, 7, -2]), (256, [40, 1], [30, 0])):
@@ -368,7 +382,7 @@ def test_attention_rows_that_see_nothing():
 @pytest.mark.parametrize("new,length,QH,KVH,HD,page", [
     (40, 3000, 4, 1, 256, 16), (33, 2500, 2, 2, 128, 32), (70, 2300, 1, 1, 64, 64), (1, 9000, 8, 2, 256, 16), (2, 5000, 3, 1, 64, 16),
 ])
-def test_attention_long_splits(new, length, QH, KVH, HD, page):
+def test_attention_long_splits(new, length, QH, KVH, HD, page, steered):
     """Splits of more tiles than a wave keeps places of, with pages outside the
     cache in several of those stretches."""
     say("long splits", new, length, HD)
@@ -383,7 +397,7 @@ def test_attention_long_splits(new, length, QH, KVH, HD, page):
 
 @pytest.mark.parametrize("R,most_new,most,HD,QH,KVH", [(64, 3, 200, 64, 2, 1), (65, 1, 300, 128, 4, 2), (70, 40, 90, 64, 4, 1),
                                                        (300, 2, 100, 64, 2, 2), (1500, 2, 40, 64, 1, 1), (8192, 1, 20, 64, 1, 1)])
-def test_attention_many_requests(R, most_new, most, HD, QH, KVH):
+def test_attention_many_requests(R, most_new, most, HD, QH, KVH, steered):
     say("many requests", R, most_new, most)
     rng = np.random.default_rng(R)
     new = rng.integers(0, most_new + 1, R).tolist()
@@ -395,7 +409,7 @@ def test_attention_many_requests(R, most_new, most, HD, QH, KVH):
     check_attention(s, run_attention(s, max_rows=most_new, max_keys=max(lengths)))
 
 
-def test_attention_leaves_other_rows():
+def test_attention_leaves_other_rows(steered):
     """Rows behind the last request, in front of the first, and requests whose rows pass the tensor's end."""
     s = attention_case(11, [3, 30], [40, 90], 4, 2, 128, 16, width_extra=80)
     s["q"] = torch.cat([s["q"][:2], s["q"], s["q"][:4]])
@@ -412,7 +426,7 @@ def test_attention_leaves_other_rows():
     check_attention(dict(s, q=s["q"][5:39], row_start=i32([0, 34]), lengths=i32([34]), table=s["table"][1:2]), got[5:39])
 
 
-def test_attention_bad_pages():
+def test_attention_bad_pages(steered):
     """Keys of pages outside the cache are not seen; lengths past the table are cut to it."""
     for HD, new in ((64, [1, 6]), (256, [1, 50])):
         say("bad pages", HD, new)
@@ -429,7 +443,7 @@ def test_attention_bad_pages():
 
 
 @pytest.mark.parametrize("HD,new,length,QH", [(64, 3, 40, 4), (256, 9, 70, 16), (128, 80, 130, 8), (256, 40, 40, 4)])
-def test_attention_non_finite_values_that_are_not_seen(HD, new, length, QH):
+def test_attention_non_finite_values_that_are_not_seen(HD, new, length, QH, steered):
     """NaN and infinities past the length (stale pages) and in later tokens of
     the chunk never reach a row that does not see them."""
     say("non-finite", HD, new, length)
@@ -446,7 +460,7 @@ def test_attention_non_finite_values_that_are_not_seen(HD, new, length, QH):
 
 
 @pytest.mark.parametrize("HD,QH,KVH,new,length", [(256, 8, 1, 60, 400), (64, 2, 2, 300, 500), (128, 4, 2, 3, 100)])
-def test_attention_non_finite_values_that_are_seen(HD, QH, KVH, new, length):
+def test_attention_non_finite_values_that_are_seen(HD, QH, KVH, new, length, steered):
     """Each channel's infinity or NaN reaches the rows that see it, as the
     formula has it, and no other channel or row."""
     say("non-finite seen", HD, new, length)
@@ -468,7 +482,7 @@ def test_attention_non_finite_values_that_are_seen(HD, QH, KVH, new, length):
     assert bool(((got - want).abs() <= tol).all())
 
 
-def test_attention_extreme_scores():
+def test_attention_extreme_scores(steered):
     """Scores far past the exponential's range, one key that outweighs all
     others, equal scores: finite, and the weights those of the maximum."""
     for QH, new in ((4, 1), (4, 40)):
@@ -487,26 +501,26 @@ def test_attention_extreme_scores():
         check_attention(s, run_attention(s))
 
 
-def test_attention_negative_and_zero_scale():
+def test_attention_negative_and_zero_scale(steered):
     s = attention_case(23, [20], [90], 4, 2, 64, 16)
     for scale in (0.0, -0.125, 0.5):
         s["scale"] = scale
         check_attention(s, run_attention(s))
 
 
-def test_attention_strided_and_in_place():
+def test_attention_strided_and_in_place(steered):
     T, QH, HD = 45, 8, 128
     s = attention_case(29, [T], [300], QH, 2, HD, 16, gate=True)
     both = torch.stack([s["q"], s["gate"]], 2).cuda()  # [T, QH, 2, HD]
     dev = [s[n].cuda() for n in ("table", "row_start", "lengths")]
     want = run_attention(s)
-    got = ops().paged_attention(both[:, :, 0], s["k"], s["v"], *dev, gate=both[:, :, 1], out=both[:, :, 0])
+    got = ops().paged_attention(both[:, :, 0], s["k"], s["v"], *dev, gate=both[:, :, 1], out=both[:, :, 0], max_keys=KEYS[0])
     assert torch.equal(got, want) and torch.equal(both[:, :, 1].cpu(), s["gate"])
     by_head = s["q"].cuda().transpose(0, 1).contiguous().transpose(0, 1)
-    assert torch.equal(ops().paged_attention(by_head, s["k"], s["v"], *dev, gate=both[:, :, 1]), want)
+    assert torch.equal(ops().paged_attention(by_head, s["k"], s["v"], *dev, gate=both[:, :, 1], max_keys=KEYS[0]), want)
     one = s["q"][:1].cuda().expand(T, -1, -1)  # one query row for every token
     s["q"] = s["q"][:1].expand(T, -1, -1)
-    check_attention(s, ops().paged_attention(one, s["k"], s["v"], *dev, gate=both[:, :, 1]))
+    check_attention(s, ops().paged_attention(one, s["k"], s["v"], *dev, gate=both[:, :, 1], max_keys=KEYS[0]))
 
 
 def test_attention_long_offsets():
@@ -519,13 +533,14 @@ def test_attention_long_offsets():
     g = torch.Generator().manual_seed(1)
     k = torch.zeros(pages, page, KVH, HD, dtype=BF, device="cuda")
     v = torch.zeros_like(k)
-    for new, length in ((1, 700), (50, 700)):
+    for new, length, most in ((1, 700, 0), (50, 700, 0), (50, 700, 1 << 22)):
         n = ref.ceil(length, page)
         at = [pages - 1 - 3 * i for i in range(n - 1)] + [1]
         kk, vv = torch.randn(n, page, KVH, HD, generator=g).to(BF), torch.randn(n, page, KVH, HD, generator=g).to(BF)
         k[at], v[at] = kk.cuda(), vv.cuda()
         q = (2 * torch.randn(new, 16, HD, generator=g)).to(BF)
-        got = ops().paged_attention(q.cuda(), k, v, i32([at]).cuda(), i32([0, new]).cuda(), i32([length]).cuda())
+        got = ops().paged_attention(q.cuda(), k, v, i32([at]).cuda(), i32([0, new]).cuda(), i32([length]).cuda(),
+                                    max_keys=most)
         small = dict(q=q, k=kk, v=vv, table=i32([list(range(n))]), row_start=i32([0, new]), lengths=i32([length]),
                      scale=HD ** -0.5, gate=None)
         check_attention(small, got)
@@ -541,7 +556,7 @@ def test_attention_long_offsets():
 # ------------------------------------------------------- streams and graphs
 
 
-def test_other_stream():
+def test_other_stream(steered):
     s = attention_case(37, [9, 1], [200, 900], 8, 2, 128, 16)
     want = run_attention(s)
     torch.cuda.synchronize()
@@ -555,13 +570,13 @@ def test_other_stream():
     assert torch.equal(got, want)
 
 
-def test_two_streams_at_once():
+def test_two_streams_at_once(steered):
     """Calls on two streams, each with a workspace of its own."""
     cases = [attention_case(41 + i, [7 + 40 * i], [3000], 8, 2, 128, 16) for i in range(2)]
     dev = [[c[n].cuda() for n in ("q", "table", "row_start", "lengths")] for c in cases]
     def call(i):
         q, *rest = dev[i]
-        return ops().paged_attention(q, cases[i]["k"], cases[i]["v"], *rest)
+        return ops().paged_attention(q, cases[i]["k"], cases[i]["v"], *rest, max_keys=KEYS[0])
     want = [call(i) for i in range(2)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -592,11 +607,11 @@ def run_round(st, qg, kv, cached, lengths, rows):
     p = ops().page_plan(st["table"], cached, lengths, st["stack"], st["free"], page_size=st["page"], rows=rows)
     q = ops().paged_prepare(qg[:, :, 0], kv[:, :KVH], kv[:, KVH:], st["qw_dev"], st["kw_dev"], st["freq_dev"], p.positions,
                             p.slots, st["k"], st["v"])
-    out = ops().paged_attention(q, st["k"], st["v"], st["table"], p.row_start, lengths, gate=qg[:, :, 1])
+    out = ops().paged_attention(q, st["k"], st["v"], st["table"], p.row_start, lengths, gate=qg[:, :, 1], max_keys=KEYS[0])
     return out, p, q
 
 
-def test_rounds_together():
+def test_rounds_together(steered):
     """Rounds of prompts, single tokens, drafts that are taken back and finished
     requests: each round's attention against one over the tokens kept by hand."""
     say("rounds together")
@@ -670,7 +685,7 @@ def test_round_without_pages_does_nothing():
     assert torch.equal(before.view(torch.int16), st["k"].view(torch.int16))
 
 
-def test_captured_round():
+def test_captured_round(steered):
     """A round captured into a graph and replayed with new lengths and rows, the
     program's own work between the replays: the same as eager calls."""
     say("captured round")
@@ -717,18 +732,18 @@ def test_captured_round():
         held = to
 
 
-def test_two_threads():
+def test_two_threads(steered):
     """Calls from two threads, each on a stream of its own."""
     import threading
     s = attention_case(43, [30, 1], [400, 2000], 8, 2, 128, 16)
     dev = [s[n].cuda() for n in ("q", "table", "row_start", "lengths")]
-    want = ops().paged_attention(dev[0], s["k"], s["v"], *dev[1:])
+    want = ops().paged_attention(dev[0], s["k"], s["v"], *dev[1:], max_keys=KEYS[0])
     torch.cuda.synchronize()
     bad = []
     def work():
         stream = torch.cuda.Stream()
         for _ in range(20):
-            got = ops().paged_attention(dev[0], s["k"], s["v"], *dev[1:], stream=stream)
+            got = ops().paged_attention(dev[0], s["k"], s["v"], *dev[1:], stream=stream, max_keys=KEYS[0])
             stream.synchronize()
             if not torch.equal(got, want):
                 bad.append(1)
