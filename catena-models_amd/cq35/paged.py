@@ -5,7 +5,8 @@ tokens over the pages (`paged_attention`).
 
 Tensors lie on one GPU, which need not be the current one; work goes to that
 device's current torch stream, or to `stream` (a torch.cuda.Stream). Nothing
-waits for the GPU, and every call may be captured into a graph. A cache is a
+waits for the GPU, and every call may be captured into a graph. Results carry no
+gradients. A cache is a
 pair of BF16 tensors [pages, page_size, kv_heads, head_dim] (views with other
 strides included, head_dim contiguous).
 """
@@ -36,26 +37,32 @@ PLAN_STATUS = ("ok", "too few free pages", "too few rows", "lengths outside the 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
 
-def _tensor(name, t, dtype, dim, device=None):
-    """`t` as it should be, or why not: the checks are cheap (a few tenths of a
-    microsecond) beside the call's launch, the reasons are looked for after."""
+def _why(name, t, dtype, dim, device):
+    """Why a tensor was refused: looked for after the cheap checks of a call,
+    which take a few tenths of a microsecond each, beside a launch of about 3."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.dtype is dtype and t.dim() == dim and (t.is_cuda if device is None else t.device == device):
-        return t
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
     if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimensions, not {t.dim()}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
-    raise ValueError(f"{name} is on {t.device}, not {device}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+
+
+def _tensor(name, t, dtype, dim, device=None):
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.dim() == dim and
+            (t.is_cuda if device is None else t.device == device)):
+        _why(name, t, dtype, dim, device)
+    return t
 
 
 def _flat(name, t, dtype, count, device):
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (count,) and t.device == device and t.is_contiguous():
         return t.data_ptr()
-    _tensor(name, t, dtype, 1, device)
+    _why(name, t, dtype, 1, device)
     if t.shape[0] != count:
         raise ValueError(f"{name} must have {count} entries, not {t.shape[0]}")
     raise ValueError(f"{name} must be contiguous")
@@ -73,23 +80,38 @@ def _stream(device, stream):
 _HERE = contextlib.nullcontext()
 
 
-def _heads(name, t, rows, heads, head_dim, device):
-    _tensor(name, t, _BF16, 3, device)
-    if t.shape != (rows, heads, head_dim):
-        raise ValueError(f"{name} must be {(rows, heads, head_dim)}, not {tuple(t.shape)}")
+def _heads(name, t, shape, device):
+    if not (isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.shape == shape and t.device == device):
+        _why(name, t, _BF16, 3, device)
+        raise ValueError(f"{name} must be {shape}, not {tuple(t.shape)}")
     row, head, channel = t.stride()
     if channel != 1:
         raise ValueError(f"{name}: the channels of a head must be contiguous")
     # the stride of a dimension of length one addresses nothing
-    return _lib.Heads(t.data_ptr(), row if rows > 1 else 0, head if heads > 1 else 0)
+    return _lib.Heads(t.data_ptr(), row if shape[0] > 1 else 0, head if shape[1] > 1 else 0)
+
+
+def _new_like(q, shape):
+    """A contiguous tensor like q and its description."""
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    return out, _lib.Heads(out.data_ptr(), shape[1] * shape[2], shape[2])
+
+
+def _query_shape(q, cache, device):
+    """q's shape as it has to be, its rows and its heads."""
+    rows, q_heads, _ = _tensor("q", q, _BF16, 3, device).shape
+    if q_heads == 0:
+        raise ValueError("q has no heads")
+    return (rows, q_heads, cache.head_dim), rows, q_heads
 
 
 def _cache(key_cache, value_cache):
-    _tensor("key_cache", key_cache, _BF16, 4)
-    _tensor("value_cache", value_cache, _BF16, 4, key_cache.device)
-    if key_cache.shape != value_cache.shape:
-        raise ValueError(f"key_cache {tuple(key_cache.shape)} and value_cache {tuple(value_cache.shape)} differ")
-    pages, page_size, kv_heads, head_dim = key_cache.shape
+    shape, device = _tensor("key_cache", key_cache, _BF16, 4).shape, key_cache.device
+    if not (isinstance(value_cache, torch.Tensor) and value_cache.dtype is _BF16 and value_cache.shape == shape and
+            value_cache.device == device):
+        _why("value_cache", value_cache, _BF16, 4, device)
+        raise ValueError(f"key_cache {tuple(shape)} and value_cache {tuple(value_cache.shape)} differ")
+    pages, page_size, kv_heads, head_dim = shape
     if not (pages and page_size and kv_heads and head_dim):
         raise ValueError("an empty cache")
     # the stride of a dimension of length one addresses nothing
@@ -97,15 +119,14 @@ def _cache(key_cache, value_cache):
     other = value_cache.stride()
     if channel != 1 or other[3] != 1:
         raise ValueError("the channels of a cached head must be contiguous")
-    if strides != other and any(n > 1 and x != y for n, x, y in zip(key_cache.shape, strides, other)):
+    if strides != other and any(n > 1 and x != y for n, x, y in zip(shape, strides, other)):
         raise ValueError("key_cache and value_cache have different strides")
-    return _lib.PagedCache(key_cache.data_ptr(), value_cache.data_ptr(), pages, page_size, kv_heads, head_dim,
+    return device, _lib.PagedCache(key_cache.data_ptr(), value_cache.data_ptr(), pages, page_size, kv_heads, head_dim,
                            page if pages > 1 else 0, row if page_size > 1 else 0, head if kv_heads > 1 else 0)
 
 
 def _table(table, requests, device):
-    _tensor("table", table, _I32, 2, device)
-    count, width = table.shape
+    count, width = _tensor("table", table, _I32, 2, device).shape
     if requests is not None and count != requests:
         raise ValueError(f"table must have {requests} rows, not {count}")
     row, entry = table.stride()
@@ -128,7 +149,7 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     requests, width = table.shape
     stride = _table(table, None, device)
     cached, lengths = _flat("cached", cached, _I32, requests, device), _flat("lengths", lengths, _I32, requests, device)
-    pages = _tensor("free_pages", free_pages, _I32, 1, device).shape[0]
+    pages = free_pages.numel() if isinstance(free_pages, torch.Tensor) else 0
     free_pages = _flat("free_pages", free_pages, _I32, pages, device)
     free_count = _flat("free_count", free_count, _I32, 1, device)
     rows = int(rows)
@@ -157,20 +178,17 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
     weights F32 [head_dim]; inv_freq F32 [rope_dim / 2]; positions int32 [rows],
     or [axes, rows] with pair_axis[i] the axis of rotated pair i. `out`: the
     tensor for the queries, q itself allowed."""
-    cache = _cache(key_cache, value_cache)
-    device = key_cache.device
-    _tensor("q", q, _BF16, 3, device)
-    rows, q_heads = q.shape[:2]
-    if q_heads == 0:
-        raise ValueError("q has no heads")
-    hq = _heads("q", q, rows, q_heads, cache.head_dim, device)
-    hk = _heads("k", k, rows, cache.kv_heads, cache.head_dim, device)
-    hv = _heads("v", v, rows, cache.kv_heads, cache.head_dim, device)
-    q_weight, k_weight = (_flat(n, w, _F32, cache.head_dim, device) for n, w in (("q_weight", q_weight), ("k_weight", k_weight)))
-    pairs = _tensor("inv_freq", inv_freq, _F32, 1, device).shape[0]
+    device, cache = _cache(key_cache, value_cache)
+    shape, rows, q_heads = _query_shape(q, cache, device)
+    kv_shape = (rows, cache.kv_heads, cache.head_dim)
+    hq, hk, hv = _heads("q", q, shape, device), _heads("k", k, kv_shape, device), _heads("v", v, kv_shape, device)
+    q_weight = _flat("q_weight", q_weight, _F32, shape[2], device)
+    k_weight = _flat("k_weight", k_weight, _F32, shape[2], device)
+    pairs = inv_freq.numel() if isinstance(inv_freq, torch.Tensor) else 0
     inv_freq = _flat("inv_freq", inv_freq, _F32, pairs, device)
-    dims = _tensor("positions", positions, _I32, min(max(positions.dim(), 1), 2), device).dim()
-    axes, axis_stride = (1, rows) if dims == 1 else (positions.shape[0], positions.stride(0))
+    flat = isinstance(positions, torch.Tensor) and positions.dim() == 1
+    _tensor("positions", positions, _I32, 1 if flat else 2, device)
+    axes, axis_stride = (1, rows) if flat else (positions.shape[0], positions.stride(0))
     if positions.shape[-1] != rows or (rows > 1 and positions.stride(-1) != 1):
         raise ValueError(f"positions must be [axes, {rows}] with contiguous rows, not {tuple(positions.shape)}")
     slots = _flat("slots", slots, _I32, rows, device)
@@ -181,8 +199,9 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
     raw, under = _stream(device, stream)
     if out is None:
         with under:
-            out = q.new_empty((rows, q_heads, cache.head_dim))
-    ho = _heads("out", out, rows, q_heads, cache.head_dim, device)
+            out, ho = _new_like(q, shape)
+    else:
+        ho = _heads("out", out, shape, device)
     check(_lib.load().cq35_paged_prepare(cache, hq, hk, hv, rows, q_heads, q_weight, k_weight, eps, inv_freq, 2 * pairs,
                                          positions.data_ptr(), axis_stride, axes, pair_axis, slots, ho, raw))
     return out
@@ -200,15 +219,11 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
     (rows outside every request are left as they were), q itself allowed.
     `workspace`: a uint8 tensor of paged_attention_workspace bytes used by no
     other work at the time, by default allocated for the call."""
-    cache = _cache(key_cache, value_cache)
-    device = key_cache.device
-    _tensor("q", q, _BF16, 3, device)
-    rows, q_heads = q.shape[:2]
-    if q_heads == 0:
-        raise ValueError("q has no heads")
-    hq = _heads("q", q, rows, q_heads, cache.head_dim, device)
-    hg = None if gate is None else _heads("gate", gate, rows, q_heads, cache.head_dim, device)
-    requests = _tensor("lengths", lengths, _I32, 1, device).shape[0]
+    device, cache = _cache(key_cache, value_cache)
+    shape, rows, q_heads = _query_shape(q, cache, device)
+    hq = _heads("q", q, shape, device)
+    hg = None if gate is None else _heads("gate", gate, shape, device)
+    requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
     lengths = _flat("lengths", lengths, _I32, requests, device)
     row_start = _flat("row_start", row_start, _I32, requests + 1, device)
     stride = _table(table, requests, device)
@@ -217,7 +232,7 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
     raw, under = _stream(device, stream)
     have = at = None
     if workspace is not None:
-        have = workspace.shape[0] if workspace.dim() == 1 else -1
+        have = workspace.numel() if isinstance(workspace, torch.Tensor) else 0
         at = _flat("workspace", workspace, torch.uint8, have, device)
     with under:
         if workspace is None:
@@ -226,8 +241,9 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
                 workspace = q.new_empty((have + 1) // 2)
                 at = workspace.data_ptr()
         if out is None:
-            out = q.new_empty((rows, q_heads, cache.head_dim))
-    ho = _heads("out", out, rows, q_heads, cache.head_dim, device)
+            out, ho = _new_like(q, shape)
+        else:
+            ho = _heads("out", out, shape, device)
     check(_lib.load().cq35_paged_attention(cache, hq, hg, ho, rows, q_heads, table.data_ptr(), stride, requests, table.shape[1],
                                            row_start, lengths, scale, max_rows, max_keys, at, have, raw))
     return out

@@ -782,3 +782,20 @@ def test_refusals_on_the_device():
     with pytest.raises(ops().CQ35Error, match="power of two"):
         c = torch.zeros(2, 24, 2, 64, dtype=BF, device="cuda")
         call(k=c, v=c)
+    for name in ("q", "k", "table", "row_start", "lengths"):
+        with pytest.raises(TypeError, match="tensor"):
+            call(**{name: [0]})
+    with pytest.raises(TypeError, match="workspace must be a tensor"):
+        call(more=dict(workspace=1 << 20))
+    with pytest.raises(ValueError, match=r"q must be \(2, 4, 64\)"):
+        call(q=torch.zeros(2, 4, 128, dtype=BF, device="cuda"))
+    p = prepare_case(1, 3, 4, 2, 64, 32, 1)
+    k, v = cache_tensors(4, 16, 2, 64)
+    q, kv = p["qg"][:, :, :64].cuda(), p["kv"].cuda()
+    args = dict(q_weight=p["qw"].cuda(), k_weight=p["kw"].cuda(), inv_freq=p["freq"].cuda(), positions=i32([0, 1, 2]).cuda(),
+                slots=i32([0, 1, 2]).cuda())
+    for name in args:
+        with pytest.raises(TypeError, match=name + " must be a tensor"):
+            ops().paged_prepare(q, kv[:, :2], kv[:, 2:], key_cache=k, value_cache=v, **dict(args, **{name: [0]}))
+        with pytest.raises(ValueError, match=name):
+            ops().paged_prepare(q, kv[:, :2], kv[:, 2:], key_cache=k, value_cache=v, **dict(args, **{name: args[name].cpu()}))
