@@ -125,14 +125,15 @@ def _cache(key_cache, value_cache):
                            page if pages > 1 else 0, row if page_size > 1 else 0, head if kv_heads > 1 else 0)
 
 
-def _table(table, requests, device):
+def _table(table, requests, device=None):
+    """Rows, width and row stride of a block table."""
     count, width = _tensor("table", table, _I32, 2, device).shape
     if requests is not None and count != requests:
         raise ValueError(f"table must have {requests} rows, not {count}")
     row, entry = table.stride()
     if entry != 1 and width > 1:
         raise ValueError("the entries of a table row must be contiguous")
-    return row if count > 1 else width
+    return count, width, row if count > 1 else width
 
 
 def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows, out=None, stream=None) -> PagePlan:
@@ -145,9 +146,8 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     earlier plan's tensors to write to. `status` is for the caller to look at
     when it next waits for the GPU: unless status[0] is 0 (PLAN_STATUS), nothing
     was changed and the round has no rows."""
-    device = _tensor("table", table, _I32, 2).device
-    requests, width = table.shape
-    stride = _table(table, None, device)
+    requests, width, stride = _table(table, None)
+    device = table.device
     cached, lengths = _flat("cached", cached, _I32, requests, device), _flat("lengths", lengths, _I32, requests, device)
     pages = free_pages.numel() if isinstance(free_pages, torch.Tensor) else 0
     free_pages = _flat("free_pages", free_pages, _I32, pages, device)
@@ -159,8 +159,10 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     sizes = (requests + 1, rows, rows, 1, 2)
     if out is None:
         with under:
-            out = PagePlan(*table.new_empty(requests + 2 * rows + 4).split_with_sizes(sizes))
-        at = [t.data_ptr() for t in out]
+            one = table.new_empty(requests + 2 * rows + 4)
+        out = PagePlan(*one.split_with_sizes(sizes))
+        base = one.data_ptr()
+        at = [base + 4 * n for n in (0, requests + 1, requests + 1 + rows, requests + 1 + 2 * rows, requests + 2 + 2 * rows)]
     else:
         at = [_flat("out." + name, t, _I32, n, device) for name, t, n in zip(PagePlan._fields, out, sizes)]
     check(_lib.load().cq35_page_plan(table.data_ptr(), stride, requests, width, cached, lengths, free_pages, pages, free_count,
@@ -226,7 +228,7 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
     requests = lengths.numel() if isinstance(lengths, torch.Tensor) else 0
     lengths = _flat("lengths", lengths, _I32, requests, device)
     row_start = _flat("row_start", row_start, _I32, requests + 1, device)
-    stride = _table(table, requests, device)
+    _, width, stride = _table(table, requests, device)
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
     max_rows, max_keys = int(max_rows), int(max_keys)
     raw, under = _stream(device, stream)
@@ -244,7 +246,7 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
             out, ho = _new_like(q, shape)
         else:
             ho = _heads("out", out, shape, device)
-    check(_lib.load().cq35_paged_attention(cache, hq, hg, ho, rows, q_heads, table.data_ptr(), stride, requests, table.shape[1],
+    check(_lib.load().cq35_paged_attention(cache, hq, hg, ho, rows, q_heads, table.data_ptr(), stride, requests, width,
                                            row_start, lengths, scale, max_rows, max_keys, at, have, raw))
     return out
 

@@ -845,12 +845,15 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
         if (a.gate) write(std::true_type{});
         else write(std::false_type{});
       } else {
+        // the addresses made here: kept over the loop they are spilled, and each
+        // reload waits for the stores in front of it
         float* part = a.part + (item.slot * (kManyRows / 32) + wave) * PartSlot<HD>::kFloats;
+        const uint32_t own = 4 * lane_here();
 #pragma unroll
         for (int i = 0; i < R::kChannelTiles * 4; ++i) {
           const f32x16_t& o = rows.o[i >> 2];
           const int r = 4 * (i & 3);
-          reinterpret_cast<float4*>(part)[i * 64 + lane] = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+          *reinterpret_cast<float4*>(part + 256 * i + own) = make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
         }
         if (h == 0) part[32 * HD + c] = rows.max, part[32 * HD + 32 + c] = sum;
       }

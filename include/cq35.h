@@ -276,8 +276,10 @@ int cq35_session_matrix_prefill(const cq35_session* session, int* components);
  * kept in F32 where the reference's matrix-core path rounds them to BF16 (the
  * unnormalised weights enter the second product as BF16), keys split over the
  * device where a chunk has few rows (so a call's chunks change its rounding).
- * Tolerance-level, as the component is; 0 (the default) keeps the reference's rounding points. head_dim 64, 128 or 256.
- * Prompt buffers hold up to 135 MB more. Copied by cq35_session_copy. */
+ * Tolerance-level, as the component is; 0 (the default) keeps the reference's
+ * rounding points. head_dim 64, 128 or 256; sessions of more than 2^22 positions
+ * keep the two passes. Prompt buffers hold up to 135 MB more. Copied by
+ * cq35_session_copy. */
 int cq35_session_set_online_attention(cq35_session* session, int enabled);
 int cq35_session_online_attention(const cq35_session* session, int* enabled);
 
@@ -393,11 +395,12 @@ typedef struct cq35_heads {
  * pages); *free_left (the count after; not free_count itself); status[2]: 0, or
  * 1 pages are missing (status[1] of them), 2 `rows` is too small (by
  * status[1]), 3 a length is negative or longer than a table, 4 the stack's
- * count is negative or above `pages`. Unless status[0] is 0 the tables and
- * the stack are left as they were, row_start is 0 and every slot -1: later
- * operators of the round then do nothing. Outputs overlap neither each other
- * nor inputs, the tables and free_pages apart. requests: 1 to 8192. With the
- * same free_count the call can be repeated with the same results. */
+ * count is negative or, with the pages given back, above `pages`. Unless
+ * status[0] is 0 the tables and the stack are left as they were, row_start is 0
+ * and every slot -1: later operators of the round then do nothing. Outputs
+ * overlap neither each other nor inputs, the tables and free_pages apart.
+ * requests: 1 to 8192. With the same free_count the call can be repeated with
+ * the same results. */
 int cq35_page_plan(int32_t* table, int64_t table_stride, int64_t requests, int64_t width,
                    const int32_t* cached, const int32_t* lengths, int32_t* free_pages, int64_t pages,
                    const int32_t* free_count, int32_t page_size, int64_t rows, int32_t* row_start,
