@@ -490,12 +490,13 @@ struct RowWriter {
     gate = a.gate ? a.gate + row * a.gate_row + head * a.gate_head : nullptr;
     inverse = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
   }
-  // four channels from `ch`
+  // Four channels from `ch` and their gates. The gates of several calls are read
+  // in front of the first: behind it, each would wait for the store before it.
+  __device__ __forceinline__ uint2 gates(int ch) const { return *reinterpret_cast<const uint2*>(gate + ch); }
   template <bool kGate>
-  __device__ __forceinline__ void write(int ch, float x0, float x1, float x2, float x3) const {
+  __device__ __forceinline__ void write(int ch, uint2 g, float x0, float x1, float x2, float x3) const {
     float x[4] = {x0 * inverse, x1 * inverse, x2 * inverse, x3 * inverse};
     if (kGate) {
-      const uint2 g = *reinterpret_cast<const uint2*>(gate + ch);
       const float gv[4] = {lo2f(g.x), hi2f(g.x), lo2f(g.y), hi2f(g.y)};
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= __builtin_amdgcn_rcpf(1.0f + exp2_fast(gv[i] * -1.44269504f));
@@ -681,11 +682,14 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
       if (!item.parts) {
         const RowWriter to(a, req, kvh, m0 + c, sum);
         auto write = [&](auto gate) {
+          constexpr bool kGate = decltype(gate)::value;
+          uint2 g[kQuads / 4] = {};
+          if (kGate)
 #pragma unroll
-          for (int n = 0; n < kQuads / 4; ++n) {
-            const int i = wave + 4 * n;
-            to.template write<decltype(gate)::value>(8 * i + 4 * h, joined[n][0], joined[n][1], joined[n][2], joined[n][3]);
-          }
+            for (int n = 0; n < kQuads / 4; ++n) g[n] = to.gates(8 * (wave + 4 * n) + 4 * h);
+#pragma unroll
+          for (int n = 0; n < kQuads / 4; ++n)
+            to.template write<kGate>(8 * (wave + 4 * n) + 4 * h, g[n], joined[n][0], joined[n][1], joined[n][2], joined[n][3]);
         };
         if (a.gate) write(std::true_type{});
         else write(std::false_type{});
@@ -749,7 +753,6 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
   const int m0 = kManyRows * item.row_tile + 32 * wave;
   const int64_t kv_offset = kvh * a.head_stride;
   R rows;
-  rows.load(a, req, kvh, m0);
   const int least = m0 + 32 > req.packed ? -1 : visible_keys(packed_position(a.cut, req, m0), req.length) - 1;
   const bool idle = m0 >= req.packed;  // no rows: the wave only requests tiles
   const bool late = wave >= 4;
@@ -761,6 +764,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
   const int own_run = 2 * own_tile + (own_row >> 4);
   bool open = m0 + c < req.packed;
   for (int limit = item.last_key;;) {
+    rows.load(a, req, kvh, m0);  // again with each pass: not kept over the results' writing
     rows.clear();
     const int t1 = min(item.t1, key_tiles_of(limit + 1)), stages = (t1 - item.t0 + N - 1) / N;
     Window runs;
@@ -835,11 +839,20 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
       if (!item.parts) {
         const RowWriter to(a, req, kvh, m0 + c, sum);
         auto write = [&](auto gate) {
+          constexpr bool kGate = decltype(gate)::value;
+          constexpr int kBatch = 8;
 #pragma unroll
-          for (int i = 0; i < R::kChannelTiles * 4; ++i) {
-            const f32x16_t& o = rows.o[i >> 2];
-            const int r = 4 * (i & 3);
-            to.template write<decltype(gate)::value>(8 * i + 4 * h, o[r], o[r + 1], o[r + 2], o[r + 3]);
+          for (int i0 = 0; i0 < R::kChannelTiles * 4; i0 += kBatch) {
+            uint2 g[kBatch] = {};
+            if (kGate)
+#pragma unroll
+              for (int n = 0; n < kBatch; ++n) g[n] = to.gates(8 * (i0 + n) + 4 * h);
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+              const f32x16_t& o = rows.o[(i0 + n) >> 2];
+              const int r = 4 * (n & 3);
+              to.template write<kGate>(8 * (i0 + n) + 4 * h, g[n], o[r], o[r + 1], o[r + 2], o[r + 3]);
+            }
           }
         };
         if (a.gate) write(std::true_type{});
@@ -904,6 +917,10 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   };
   read(0, 0);
+  uint2 g[kTiles] = {};
+  if (a.gate)
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) g[j] = to.gates(8 * (quad0 + 4 * j) + 4 * h);
   float most = -INFINITY, sum = 0.0f;
   if (row)
 #pragma unroll 4
@@ -938,8 +955,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
       }
     }
     if (!row) continue;
-    if (a.gate) to.template write<true>(8 * (quad0 + 4 * j) + 4 * h, v.x, v.y, v.z, v.w);
-    else to.template write<false>(8 * (quad0 + 4 * j) + 4 * h, v.x, v.y, v.z, v.w);
+    if (a.gate) to.template write<true>(8 * (quad0 + 4 * j) + 4 * h, g[j], v.x, v.y, v.z, v.w);
+    else to.template write<false>(8 * (quad0 + 4 * j) + 4 * h, g[j], v.x, v.y, v.z, v.w);
   }
 }
 
