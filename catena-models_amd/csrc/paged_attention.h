@@ -727,8 +727,9 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
 // cycles of a clock that falls from 2.3 to 1.8 - 2.0 GHz. In step, scores in a
 // run of their own: 1.08 ms; a phase apart with that run: 1.15 ms; values'
 // products and scores in one run without places in the lanes (table and strides
-// worked on every stage): 1.26 ms. Short prompts are bound by an item's start
-// and end (about 12 us with the partial results' write) and the softmax.
+// worked on every stage): 1.26 ms. 16 mixed requests (500, 300, 223 and single
+// tokens over up to 4096 keys of 256 channels) take 67 us, 16 more for the join:
+// 26 stages, then 36 MB of partial results by all items at once.
 constexpr int kManyThreads = 512;
 constexpr int kManyRows = 256;
 constexpr int kManyStages = 4;
@@ -964,15 +965,15 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
 
 // How a call of paged attention is cut. k_paged_few reads the keys again for
 // every 32 packed rows (rows times query heads of a KV head), k_paged_many for
-// every 256 but with an item's start and end, about 12 us. Requests of up to 32
-// packed rows, and calls whose 32-row tiles of a KV head times keys times
+// every 256, but its items are longer and have more to write. Requests of up to
+// 32 packed rows, and calls whose 32-row tiles of a KV head times keys times
 // channels stay below kFewWork, go to the first. Measured in us, few and many,
-// at tiles x keys: 256 channels 512 x 600 42, 52; 128 x 4000 57, 61; 1024 x 600
-// 82, 68; 256 x 4000 90, 77; 64 x 16000 85, 76. 128 channels 256 x 4000 40, 43;
-// 512 x 4000 61, 59; 256 x 16000 116, 92. 64 channels 2048 x 600 31, 38; 512 x
-// 4000 46, 43; 256 x 16000 84, 67. max_rows and max_keys tell without the
-// lengths, a call without max_keys counts as one of kKeysAssumed; max_keys also
-// spares the join where no request can be split.
+// at tiles x keys: 256 channels 512 x 600 45, 46; 64 x 4000 42, 42; 128 x 4000
+// 56, 55; 1024 x 600 81, 60; 256 x 4000 91, 73; 64 x 16000 84, 70. 128 channels
+// 256 x 4000 40, 44; 512 x 4000 61, 59; 256 x 16000 115, 93. 64 channels 2048 x
+// 600 31, 38; 512 x 4000 46, 44; 256 x 16000 84, 67. max_rows and max_keys tell
+// without the lengths, a call without max_keys counts as one of kKeysAssumed;
+// max_keys also spares the join where no request can be split.
 constexpr int64_t kFewWork = 1 << 27;
 constexpr int64_t kKeysAssumed = 4096;
 constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
