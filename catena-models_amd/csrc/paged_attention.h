@@ -107,7 +107,7 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, uint32_t at, Foun
     if (r < R) q = cut_request(a.cut, a.row_start[r], a.row_start[r + 1], a.lengths[r]);
     return q;
   };
-  auto pairs_of = [](const CutRequest& q) { return (int64_t)q.tiles * q.key_tiles; };
+  auto work_of = [&](const CutRequest& q) { return request_work(a.cut, q); };
   auto items_of = [&](const CutRequest& q, int n) { return kTiles ? q.tiles : (int64_t)q.tiles * n; };
   auto parts_of = [](const CutRequest& q, int n) { return n > 1 ? (int64_t)q.tiles * n : 0; };
   CutRequest q;
@@ -115,12 +115,12 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, uint32_t at, Foun
   int64_t before = 0, parts_before = 0;  // of earlier slices
   if (slices == 1) {
     q = shape(0);
-    chunk = cut_chunk(a.cut, lane_value(wave_sums(pairs_of(q)), 63), [&](int32_t x) {
+    chunk = cut_chunk(a.cut, lane_value(wave_sums(work_of(q)), 63), [&](int32_t x) {
       return lane_value(wave_sums((int64_t)q.tiles * cut_splits(a.cut, q, x)), 63);
     });
   } else {
     for (int s = wave; s < slices; s += W) {
-      const int64_t x = wave_sums(pairs_of(shape(s)));
+      const int64_t x = wave_sums(work_of(shape(s)));
       if (lane == 63) sums[0][s] = x;
     }
     __syncthreads();
@@ -575,25 +575,23 @@ constexpr int kFewRows = 32;
 template <int HD>
 constexpr size_t few_lds_bytes() { return 4 * 2 * KvTile<HD>::kBytes; }
 
-template <int HD>
-__global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(AttendArgs a) {
+// An item by a block's first four waves, the others gone; kUnits: parts of a
+// slot. In k_paged_many's block the scores are one chain: two spill.
+template <int HD, int kUnits>
+__device__ __forceinline__ void few_rows_item(const AttendArgs& a, int kvh, const Item& item, const CutRequest& req,
+                                              uint8_t* lds) {
   typedef KvTile<HD> T;
   typedef Rows<HD> R;
-  extern __shared__ __align__(1024) uint8_t attend_lds[];
   __shared__ float stat[2][4][32];
   __shared__ int open_at[4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
-  const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
-  Item item;
-  CutRequest req;
-  if (!find_item<kFewThreads>(a, kvh, &item, &req)) return;
   const int m0 = kFewRows * item.row_tile;
   const int64_t kv_offset = kvh * a.head_stride;
   R rows;
   rows.load(a, req, kvh, m0);
   // up to this key every column sees all: none where a column is no row
   const int least = m0 + kFewRows > req.packed ? -1 : visible_keys(packed_position(a.cut, req, m0), req.length) - 1;
-  const uint32_t keys = lds_address(attend_lds) + wave * 2 * T::kBytes, values = keys + T::kBytes;
+  const uint32_t keys = lds_address(lds) + wave * 2 * T::kBytes, values = keys + T::kBytes;
   bool open = m0 + c < req.packed;  // this column's result is not written yet
   for (int limit = item.last_key;;) {
     rows.clear();
@@ -620,7 +618,7 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
       const int gone = (int)(runs.bad >> ((t - window) / 2)) & 3;
       arrived_but<T::kLoads>();
       f32x16_t sc[1];
-      rows.template scores<2>(keys, sc[0]);
+      rows.template scores<kUnits == 1 ? 2 : 1>(keys, sc[0]);
       __builtin_amdgcn_sched_barrier(0);
       if (more) {
         if (t + 4 == window + 128) {
@@ -648,7 +646,7 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
 #pragma unroll
     for (int w = 0; w < 4; ++w) sum += stat[1][w][c] * exp2_fast(stat[0][w][c] - base);
     const float keep = exp2_fast(rows.max - base);
-    float4* red = reinterpret_cast<float4*>(attend_lds);  // [wave][channel tile][4 registers][lane]
+    float4* red = reinterpret_cast<float4*>(lds);  // [wave][channel tile][4 registers][lane]
     constexpr int kQuads = R::kChannelTiles * 4;
 #pragma unroll
     for (int i = 0; i < kQuads; ++i) {
@@ -694,7 +692,7 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
         if (a.gate) write(std::true_type{});
         else write(std::false_type{});
       } else {
-        float* part = a.part + item.slot * PartSlot<HD>::kFloats;
+        float* part = a.part + item.slot * kUnits * PartSlot<HD>::kFloats;
 #pragma unroll
         for (int n = 0; n < kQuads / 4; ++n)
           reinterpret_cast<float4*>(part)[(wave + 4 * n) * 64 + lane] = make_float4(joined[n][0], joined[n][1], joined[n][2], joined[n][3]);
@@ -707,12 +705,22 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
   }
 }
 
+template <int HD>
+__global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(AttendArgs a) {
+  extern __shared__ __align__(1024) uint8_t attend_lds[];
+  const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
+  Item item;
+  CutRequest req;
+  if (find_item<kFewThreads>(a, kvh, &item, &req)) few_rows_item<HD, 1>(a, kvh, item, req, attend_lds);
+}
+
 // -------------------------------------------- many rows: rows over waves
 //
 // One item is 256 packed rows over one split of the keys, 32 rows a wave, two
 // waves a SIMD. The waves share rings of four stages of 32 keys (of 64 for heads
 // of up to 128 channels, whose tiles are short), half of them requesting the
-// keys, half the values, two to three stages ahead; one barrier a stage.
+// keys, half the values, two to three stages ahead; one barrier a stage. A
+// request of up to 32 packed rows is done as in k_paged_few.
 //
 // A stage is its softmax on the vector unit and a run of products (its values',
 // the next stage's scores) on the matrix cores. The first half of the waves
@@ -728,8 +736,8 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
 // run of their own: 1.08 ms; a phase apart with that run: 1.15 ms; values'
 // products and scores in one run without places in the lanes (table and strides
 // worked on every stage): 1.26 ms. 16 mixed requests (500, 300, 223 and single
-// tokens over up to 4096 keys of 256 channels) take 67 us, 16 more for the join:
-// 26 stages, then 36 MB of partial results by all items at once.
+// tokens over up to 4096 keys of 256 channels) take 62 us, 18 more for the join:
+// 19 stages, then 50 MB of partial results by all items at once.
 constexpr int kManyThreads = 512;
 constexpr int kManyRows = 256;
 constexpr int kManyStages = 4;
@@ -751,6 +759,10 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
   Item item;
   CutRequest req;
   if (!find_item<kManyThreads>(a, kvh, &item, &req)) return;
+  if (req.packed <= kFewRows) {
+    if (wave < kFewThreads / 64) few_rows_item<HD, kManyRows / 32>(a, kvh, item, req, attend_lds);
+    return;
+  }
   const int m0 = kManyRows * item.row_tile + 32 * wave;
   const int64_t kv_offset = kvh * a.head_stride;
   R rows;

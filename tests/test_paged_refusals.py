@@ -186,7 +186,7 @@ int main(int argc, char** argv) {
       int64_t pairs = 0, items = 0, parts = 0, tile_count = 0;
       for (long long r = 0; r < R; ++r) {
         const CutRequest q = cut_request(c, start[r], start[r + 1], length[r]);
-        pairs += (int64_t)q.tiles * q.key_tiles;
+        pairs += request_work(c, q);
       }
       const int32_t chunk = cut_chunk(c, pairs, [&](int32_t x) {
         int64_t n = 0;
