@@ -893,43 +893,46 @@ __global__ __launch_bounds__(kManyThreads, 2) void k_paged_many(AttendArgs a) {
 // ---------------------------------------------------- joining the splits
 //
 // Block (32 packed rows and KV head, kTiles channel tiles): each thread a
-// float4 of the fragment order per channel tile over all splits, weighted by
-// 2^(max - maximum). The splits' maxima and sums are read once, eight splits at
-// a time, each eighth of them joined as it comes; the first parts and the gate
-// are on their way meanwhile.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinKept = 128;  // splits whose maxima stay in LDS
-template <int HD, int kGroups, int kTiles>
-__global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
+// float4 of the fragment order per channel tile over all splits, or over those
+// of its group of four waves, weighted by 2^(max - maximum). The splits' maxima
+// and sums are read once, two a wave at a time, each wave's joined as they come;
+// the first parts and the gate are on their way meanwhile.
+template <int HD, int kUnits, int kTiles, int kGroups>
+__global__ __launch_bounds__(256 * kGroups) void k_paged_join(AttendArgs a) {
+  static_assert(kGroups == 1 || kTiles == 1, "groups are added once");
+  constexpr int kWaves = 4 * kGroups, kJoinKept = kGroups > 1 ? 256 : 128;  // splits whose maxima stay in LDS
   const int kvh = blockIdx.x % (uint32_t)a.cut.kv_heads;
   const uint32_t unit = blockIdx.x / (uint32_t)a.cut.kv_heads;
   Found f;
   CutRequest req;
-  if (!find_work<true, kJoinThreads>(a, unit / kGroups, &f, &req)) return;
+  if (!find_work<true, 256 * kGroups>(a, unit / kUnits, &f, &req)) return;
   const int splits = cut_splits(a.cut, req, f.chunk), chunk = split_tiles(req, splits);
   const int tile = req.tiles - 1 - f.index, seen = key_tiles_of(tile_keys(a.cut, req, tile));
   if (seen <= chunk) return;
-  const int used = (int)((uint32_t)(seen + chunk - 1) / (uint32_t)chunk), group = (int)(unit % kGroups);
+  const int used = (int)((uint32_t)(seen + chunk - 1) / (uint32_t)chunk), of = (int)(unit % kUnits);
   const int64_t first = (f.parts_before + (int64_t)f.index * splits) * a.cut.kv_heads + kvh;
   if (first + (int64_t)(used - 1) * a.cut.kv_heads >= a.cut.slots) return;
-  __shared__ float kept[kJoinKept][32], stat[2][8][32];
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
-  const int m0 = a.cut.tile_rows * tile + 32 * group, m = min(m0 + c, req.packed - 1);
+  __shared__ float kept[kJoinKept][32], stat[2][2 * kWaves][32];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = kGroups > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x >> 6;
+  const int m0 = a.cut.tile_rows * tile + 32 * of, m = min(m0 + c, req.packed - 1);
   if (m0 >= req.packed) return;
   const bool row = m0 + c < req.packed;  // other columns' parts were not written
-  const int64_t step = (int64_t)a.cut.kv_heads * kGroups * PartSlot<HD>::kFloats;
-  const float* part = a.part + (first * kGroups + group) * PartSlot<HD>::kFloats;
-  const int quad0 = 4 * kTiles * blockIdx.y + wave;  // this thread's quads: quad0 + 4 j
+  const int64_t step = (int64_t)a.cut.kv_heads * kUnits * PartSlot<HD>::kFloats;
+  const float* part = a.part + (first * kUnits + of) * PartSlot<HD>::kFloats;
+  const int quad0 = 4 * kTiles * blockIdx.y + (kGroups > 1 ? wave & 3 : wave);  // this thread's quads: quad0 + 4 j
   const RowWriter to(a, req, kvh, m, 1.0f);
+  const int each = (used + kGroups - 1) / kGroups;
+  const int begin = kGroups > 1 ? wave / 4 * each : 0, end = kGroups > 1 ? min(begin + each, used) : used;
   constexpr int kBatch = 8;
   float4 x[kBatch];
   auto read = [&](int s0, int j) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      x[i] = s0 + i < used && row ? reinterpret_cast<const float4*>(part + (s0 + i) * step)[(quad0 + 4 * j) * 64 + lane]
+      x[i] = s0 + i < end && row ? reinterpret_cast<const float4*>(part + (s0 + i) * step)[(quad0 + 4 * j) * 64 + lane]
                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   };
-  read(0, 0);
+  read(begin, 0);
   uint2 g[kTiles] = {};
   if (a.gate)
 #pragma unroll
@@ -937,7 +940,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
   float most = -INFINITY, sum = 0.0f;
   if (row)
 #pragma unroll 4
-    for (int s = 2 * wave + h; s < used; s += 8) {
+    for (int s = 2 * wave + h; s < used; s += 2 * kWaves) {
       const float x = part[s * step + 32 * HD + c], l = part[s * step + 32 * HD + 32 + c];
       if (s < kJoinKept) kept[s][c] = x;
       const float grown = fmaxf(most, x), base = grown == -INFINITY ? 0.0f : grown;
@@ -947,24 +950,35 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(AttendArgs a) {
   stat[0][2 * wave + h][c] = most, stat[1][2 * wave + h][c] = sum;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = fmaxf(most, stat[0][i][c]);
+  for (int i = 0; i < 2 * kWaves; ++i) most = fmaxf(most, stat[0][i][c]);
   const float base = most == -INFINITY ? 0.0f : most;
   sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(stat[1][i][c], exp2_fast(stat[0][i][c] - base), sum);
+  for (int i = 0; i < 2 * kWaves; ++i) sum = __builtin_fmaf(stat[1][i][c], exp2_fast(stat[0][i][c] - base), sum);
   const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < used; s0 += kBatch) {
-      if (s0 > 0 || j > 0) read(s0, j);
+    for (int s0 = begin; s0 < end; s0 += kBatch) {
+      if (s0 > begin || j > 0) read(s0, j);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int s = s0 + i;
-        if (s >= used) break;
+        if (s >= end) break;
         const float w = exp2_fast((s < kJoinKept ? kept[s][c] : part[s * step + 32 * HD + c]) - base) * inverse;
         v.x = __builtin_fmaf(w, x[i].x, v.x), v.y = __builtin_fmaf(w, x[i].y, v.y);
         v.z = __builtin_fmaf(w, x[i].z, v.z), v.w = __builtin_fmaf(w, x[i].w, v.w);
+      }
+    }
+    if (kGroups > 1) {
+      __shared__ float4 sums[kGroups][4][64];
+      sums[wave / 4][wave & 3][lane] = v;
+      __syncthreads();
+      if (wave >= 4) return;
+#pragma unroll
+      for (int o = 1; o < kGroups; ++o) {
+        const float4 y = sums[o][wave][lane];
+        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
       }
     }
     if (!row) continue;
@@ -992,10 +1006,14 @@ constexpr int kFewTarget = 9, kManyTarget = 8;  // log2 of the items wanted
 constexpr int kFewMinTiles = 4, kManyMinTiles = 8;
 constexpr int kMostSplits = 1024;
 constexpr int64_t kMostBlocks = 1 << 22;  // times 512 threads: a launch takes below 2^32
+// Few units take a channel tile a block, and four groups of waves where a row
+// tile may have kTallJoin splits, a chain of loads for one (one token over 32768 keys
+// of 2 heads of 256 in 256 splits: 48 and 84 us; over 8000 20 and 27); 32 requests
+// of 5 over 5000, of five splits, 66 and 57.5.
 constexpr int kWideJoin = 512;  // units of 32 packed rows and KV head
 
 struct AttendPlan {
-  bool few;
+  bool few, tall;        // tall: row tiles of many splits
   CutRule cut;
   int64_t items, units;  // at most: blocks of the attention, 32-row groups of the join
   int64_t floats;        // of workspace
@@ -1016,6 +1034,7 @@ inline AttendPlan cut_attention(bool few, int64_t rows, int64_t requests, int q_
   p.items = most_items(tiles, kv_heads, c.target_shift, c.max_splits);
   p.units = tiles * kv_heads * (c.tile_rows / 32);
   c.slots = most_slots(tiles, kv_heads, c.target_shift, c.max_splits);
+  p.tall = c.slots >= kTallJoin * tiles * kv_heads;
   p.floats = c.slots * (c.tile_rows / 32) * (32 * (int64_t)head_dim + 64);
   return p;
 }
@@ -1039,7 +1058,7 @@ struct AttendKernels {
   void (*attend)(AttendArgs);
   void (*join)(AttendArgs);
   dim3 grid, join_grid;
-  int threads;
+  int threads, join_threads;
   size_t lds;
 };
 
@@ -1049,8 +1068,11 @@ AttendKernels attend_kernels(const AttendPlan& p) {
   const bool wide = p.units >= kWideJoin;
   AttendKernels k;
   k.attend = p.few ? k_paged_few<HD> : k_paged_many<HD>;
-  k.join = p.few ? (wide ? k_paged_join<HD, 1, HD / 32> : k_paged_join<HD, 1, 1>)
-                 : (wide ? k_paged_join<HD, kManyRows / 32, HD / 32> : k_paged_join<HD, kManyRows / 32, 1>);
+  constexpr int kUnits = kManyRows / 32;
+  const bool tall = !wide && p.tall;
+  k.join = p.few ? (wide ? k_paged_join<HD, 1, HD / 32, 1> : tall ? k_paged_join<HD, 1, 1, 4> : k_paged_join<HD, 1, 1, 1>)
+                 : (wide ? k_paged_join<HD, kUnits, HD / 32, 1> : tall ? k_paged_join<HD, kUnits, 1, 4> : k_paged_join<HD, kUnits, 1, 1>);
+  k.join_threads = tall ? 1024 : 256;
   k.grid = dim3((unsigned)p.items), k.join_grid = dim3((unsigned)p.units, wide ? 1 : HD / 32);
   k.threads = p.few ? kFewThreads : kManyThreads;
   k.lds = p.few ? few_lds_bytes<HD>() : many_lds_bytes<HD>();

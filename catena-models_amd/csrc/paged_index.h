@@ -135,12 +135,20 @@ CQ35_BOTH int32_t split_tiles(const CutRequest& q, int32_t splits) {
 // that sum dealt evenly to the items wanted, or up to twice that (`search`)
 // where the requests' ends then make fewer rounds of items: one CU holds one,
 // and an item costs some tiles' time besides its own (kItemTiles, measured).
+// Tiles of few rows that may have many splits take up to twice min_tiles first,
+// half as many items as wanted: one token over 32768 keys of 2 heads of 256 33
+// us, with twice the splits 47 (2 requests of 3 over 17909 keys of one head 26
+// and 36).
 // items_at(chunk): the items per KV head that splits of `chunk` make.
 constexpr int kItemTiles = 6;
+constexpr int kTallJoin = 32;  // splits of a row tile from which on its join is a chain
 template <typename F>
 CQ35_BOTH int32_t cut_chunk(const CutRule& c, int64_t pairs, F items_at) {
   const int64_t even = (pairs * c.kv_heads + ((int64_t)1 << c.target_shift) - 1) >> c.target_shift;
-  const int32_t base = even > INT32_MAX / 16 ? INT32_MAX / 16 : even > c.min_tiles ? (int32_t)even : c.min_tiles;
+  const int64_t twice = 2 * even < 2 * c.min_tiles ? 2 * even : 2 * c.min_tiles;
+  const int64_t least_tiles = c.tile_rows <= kLightRows && c.max_splits >= kTallJoin && twice > c.min_tiles ? twice : c.min_tiles;
+  const int64_t wanted = even > least_tiles ? even : least_tiles;
+  const int32_t base = wanted > INT32_MAX / 16 ? INT32_MAX / 16 : (int32_t)wanted;
   if (!c.search) return base;
   int32_t best = base;
   int64_t least = INT64_MAX;

@@ -234,7 +234,7 @@ int launch_attention(const AttendArgs& a, const AttendPlan& p, hipStream_t s) {
   const AttendKernels k = attend_kernels<HD>(p);
   if (k.lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)k.attend, hipFuncAttributeMaxDynamicSharedMemorySize, (int)k.lds));
   int rc = launch_operator("paged attention", k.attend, k.grid, k.threads, k.lds, s, a);
-  if (!rc && a.cut.slots > 0) rc = launch_operator("paged attention", k.join, k.join_grid, kJoinThreads, 0, s, a);
+  if (!rc && a.cut.slots > 0) rc = launch_operator("paged attention", k.join, k.join_grid, k.join_threads, 0, s, a);
   return rc;
 }
 

@@ -1762,7 +1762,7 @@ void enqueue_prefill(cq35_session* s, int64_t n, const Prefill& pf) {
           at.cut = p.cut, at.cut.most_keys = (int32_t)cap, at.part = pf.joint;
           const AttendKernels k = attend_kernels<HD>(p);
           L(KC_ATTENTION, k.attend, k.grid, dim3(k.threads), k.lds, at);
-          if (at.cut.slots > 0) L(KC_ATTENTION, k.join, k.join_grid, dim3(kJoinThreads), 0, at);
+          if (at.cut.slots > 0) L(KC_ATTENTION, k.join, k.join_grid, dim3(k.join_threads), 0, at);
         };
         if (pf.span && d.HD == 256) online(std::integral_constant<int, 256>{});
         else if (pf.span && d.HD == 128) online(std::integral_constant<int, 128>{});
