@@ -565,7 +565,7 @@ __device__ __forceinline__ int least_open(bool open, int pos, int* shared) {
 // 64 KB and more are on their way per CU.
 //
 // Bound by the keys and values: 8 tokens over 14 to 32 thousand keys of 2 heads
-// of 256, 457 MB, 90 us or 5.1 TB/s (a large copy: 4.9), and 12 us for the join.
+// of 256, 457 MB, 90 us or 5.1 TB/s (a large copy: 4.9), and 9 us for the join.
 // 512 items: one of 256 gives 125 us in all, one of 1024 (half a split each) 129.
 // A single token over 520 keys is bound by its chain of loads (request, table,
 // keys), 10.5 us: splits of four tiles, one a wave, against two: 20.3 and 21.3.

@@ -381,6 +381,7 @@ def test_attention_rows_that_see_nothing(steered):
 
 @pytest.mark.parametrize("new,length,QH,KVH,HD,page", [
     (40, 3000, 4, 1, 256, 16), (33, 2500, 2, 2, 128, 32), (70, 2300, 1, 1, 64, 64), (1, 9000, 8, 2, 256, 16), (2, 5000, 3, 1, 64, 16),
+    (1, 140000, 2, 1, 64, 64),  # more splits than the join keeps maxima of
 ])
 def test_attention_long_splits(new, length, QH, KVH, HD, page, steered):
     """Splits of more tiles than a wave keeps places of, with pages outside the
