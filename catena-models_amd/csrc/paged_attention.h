@@ -466,14 +466,15 @@ struct Rows {
     sc = next;
   }
 
-  // Whether a result of a column that sees anything is NaN (or infinite).
+  // Whether a result is NaN (or infinite), also of a column that sees nothing:
+  // its weights of zero meet the values that later rows see.
   __device__ __forceinline__ bool any_nan() const {
     float x = 0.0f;
 #pragma unroll
     for (int ct = 0; ct < kChannelTiles; ++ct)
 #pragma unroll
       for (int r = 0; r < 16; ++r) x = __builtin_fmaf(o[ct][r], 0.0f, x);
-    return x != x && pos >= 0;
+    return x != x;
   }
 };
 
