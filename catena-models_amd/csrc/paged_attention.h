@@ -478,7 +478,8 @@ struct Rows {
   }
 };
 
-// Packed row m's results: divided by its sum, gated, rounded once.
+// Packed row m's results: divided by its sum, gated, rounded once; zeros for a
+// row without a weight above 0, whatever its values and its gate.
 struct RowWriter {
   uint16_t* out;
   const uint16_t* gate;
@@ -489,7 +490,7 @@ struct RowWriter {
     const int64_t row = r.begin + token, head = kvh * a.cut.group + m - token * a.cut.group;
     out = a.out + row * a.out_row + head * a.out_head;
     gate = a.gate ? a.gate + row * a.gate_row + head * a.gate_head : nullptr;
-    inverse = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+    inverse = sum == 0.0f ? 0.0f : 1.0f / sum;  // 0: zeros
   }
   // Four channels from `ch` and their gates. The gates of several calls are read
   // in front of the first: behind it, each would wait for the store before it.
@@ -502,6 +503,8 @@ struct RowWriter {
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= __builtin_amdgcn_rcpf(1.0f + exp2_fast(gv[i] * -1.44269504f));
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = inverse == 0.0f ? 0.0f : x[i];
     *reinterpret_cast<uint2*>(out + ch) = make_uint2(pack_weights(x[0], x[1]), pack_weights(x[2], x[3]));
   }
 };
@@ -922,7 +925,7 @@ __global__ __launch_bounds__(256 * kGroups) void k_paged_join(AttendArgs a) {
   const int64_t step = (int64_t)a.cut.kv_heads * kUnits * PartSlot<HD>::kFloats;
   const float* part = a.part + (first * kUnits + of) * PartSlot<HD>::kFloats;
   const int quad0 = 4 * kTiles * blockIdx.y + (kGroups > 1 ? wave & 3 : wave);  // this thread's quads: quad0 + 4 j
-  const RowWriter to(a, req, kvh, m, 1.0f);
+  RowWriter to(a, req, kvh, m, 1.0f);
   const int each = (used + kGroups - 1) / kGroups;
   const int begin = kGroups > 1 ? wave / 4 * each : 0, end = kGroups > 1 ? min(begin + each, used) : used;
   constexpr int kBatch = 8;
@@ -956,7 +959,8 @@ __global__ __launch_bounds__(256 * kGroups) void k_paged_join(AttendArgs a) {
   sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < 2 * kWaves; ++i) sum = __builtin_fmaf(stat[1][i][c], exp2_fast(stat[0][i][c] - base), sum);
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inverse = 1.0f / sum;
+  if (sum == 0.0f) to.inverse = 0.0f;
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

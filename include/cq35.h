@@ -438,7 +438,8 @@ int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const
  * the second product as BF16 (off by at most 2^-8 each, as the values they
  * meet), the sums and the running maximum stay F32, the result is rounded to
  * BF16 once. The same call gives the same bits.
- * A row that sees no key (p < 0), or none with a score above -inf, gets zeros.
+ * A row that sees no key (p < 0), or none with a score above -inf, gets zeros,
+ * whatever its values and its gate.
  * Keys in pages whose number is outside the cache are not seen; lengths are
  * cut to what the table holds (at most 2^30 keys). Rows outside every request
  * are left alone. Up to 8192 requests; rows * q_heads below about 2^27. out may be
