@@ -1089,19 +1089,25 @@ inline void attend_scale(AttendArgs* a, float scale) {
   a->q_and = scale == 0.0f ? 0u : ~0u, a->q_xor = scale < 0.0f ? 0x80008000u : 0u;
 }
 
-// One request over a contiguous cache: its rows, length and a table of pages
-// that follow each other, for attention over the session's own cache.
+// A request over a contiguous cache: its rows, length and a table of pages
+// that follow each other, for attention over the session's own cache. A chunk of
+// a prompt is a request for every kSpanRows of its rows, attended by a call of
+// its own: how a call is cut, and so its rounding, follows from its rows, and
+// chunks of any whole number of kSpanRows (fewer rows are taken where memory is
+// short) then give the same bits.
 constexpr int kSpanShift = 16, kSpanTable = 64;  // rows of a page (log2), pages
+constexpr int kSpanRows = 1024;
 struct PromptSpan {
   int32_t row_start[2], length, pad;
   int32_t table[kSpanTable];
 };
-__global__ void k_prompt_span(const uint64_t* __restrict__ params, int t, int rows_n, PromptSpan* __restrict__ span) {
-  const int i = threadIdx.x;
+__global__ void k_prompt_span(const uint64_t* __restrict__ params, int t, int rows_n, PromptSpan* __restrict__ spans) {
+  const int i = threadIdx.x, before = kSpanRows * blockIdx.x, rows = min(kSpanRows, rows_n - before);
+  PromptSpan* span = spans + blockIdx.x;
   if (i < kSpanTable) span->table[i] = i;
   if (i == 0) {
-    span->row_start[0] = 0, span->row_start[1] = rows_n;
-    span->length = (int32_t)(step_position(params, t) + rows_n);
+    span->row_start[0] = 0, span->row_start[1] = rows;
+    span->length = (int32_t)(step_position(params, t) + before + rows);
   }
 }
 

@@ -1535,8 +1535,8 @@ struct Prefill {
   int *eoff = nullptr, *order = nullptr;    // experts: buckets
   int* tiles = nullptr;                     // matrix-core experts: tiles that hold work
   int* ids = nullptr;
-  PromptSpan* span = nullptr;  // one-pass attention: the chunk as a request
-  float* joint = nullptr;      // its splits' partial results
+  PromptSpan* span = nullptr;  // one-pass attention: the chunk as requests
+  float* joint = nullptr;      // the partial results of one's splits
   uint32_t* ranges = nullptr;  // k_bgemm: magnitude ranges of a launch's weight and token tiles
   int attn_tokens = 0;         // tokens per staged-attention launch (scratch rows)
   int rows = 0;                // tokens per chunk
@@ -1588,8 +1588,8 @@ size_t prefill_layout(const cq35_session* s, int64_t rows, unsigned char* base, 
     take(&pf->spart, m * d.H);
   }
   if (online_attention(s)) {
-    take(&pf->span, 1);
-    take(&pf->joint, most_attend_floats(m, (int)d.Q, (int)d.KVH, (int)d.HD, s->capacity));
+    take(&pf->span, (m + kSpanRows - 1) / kSpanRows);
+    take(&pf->joint, most_attend_floats(std::min<int64_t>(m, kSpanRows), (int)d.Q, (int)d.KVH, (int)d.HD, s->capacity));
   }
   // staged attention scratch rows, at most 64 MiB
   const int64_t per_token = d.Q * (int64_t)s->attn_stride;
@@ -1654,6 +1654,9 @@ void enqueue_prefill(cq35_session* s, int64_t n, const Prefill& pf) {
   int last_rows = 1;
   // The chunk size changes no result: every per-token operation is
   // independent of the other rows, the scan carries its state in the shadow.
+  // One-pass attention alone is cut by its rows; it takes them kSpanRows at a
+  // time, so that this holds for chunks of a whole number of those.
+  static_assert(kMChunk % kSpanRows == 0 && kMFewRows % kSpanRows == 0, "chunks of whole spans");
   const int64_t chunk = pf.rows;
   for (int64_t c0 = 0; c0 < n; c0 += chunk) {
     const int rows_n = (int)std::min<int64_t>(chunk, n - c0);
@@ -1661,7 +1664,8 @@ void enqueue_prefill(cq35_session* s, int64_t n, const Prefill& pf) {
     const unsigned tiles = (unsigned)((rows_n + 4 * kBTokens - 1) / (4 * kBTokens));
     L(KC_EMBED, k_bembed, dim3(rows_n), dim3(kBlock), 0, params, first, (const uint16_t*)Wt(0), H,
       pf.h, c0 + rows_n == n ? s->d_best : (unsigned long long*)nullptr);
-    if (pf.span) L(KC_EMBED, k_prompt_span, dim3(1), dim3(64), 0, params, first, rows_n, pf.span);
+    const int spans = (rows_n + kSpanRows - 1) / kSpanRows;
+    if (pf.span) L(KC_EMBED, k_prompt_span, dim3(spans), dim3(64), 0, params, first, rows_n, pf.span);
     // matrix-core projections when selected (K a multiple of the MFMA step)
     const bool mp = (s->matrix & CQ35_MATRIX_PROJECTIONS) != 0;
     // matrix-core projections: LDS-staged tiles for widths of whole 128-column
@@ -1748,21 +1752,25 @@ void enqueue_prefill(cq35_session* s, int64_t n, const Prefill& pf) {
         const bool ma = (s->matrix & CQ35_MATRIX_ATTENTION) != 0;
         auto online = [&](auto hd) {
           constexpr int HD = decltype(hd)::value;
-          const AttendPlan p = plan_attention(rows_n, 1, (int)d.Q, (int)d.KVH, HD, rows_n,
-                                              (int64_t)s->h_params[0] + first + rows_n);
-          AttendArgs at{};
-          at.q = qr, at.q_row = d.QS, at.q_head = HD;
-          at.gate = qg + HD, at.gate_row = 2 * d.QS, at.gate_head = 2 * HD;
-          at.out = ctx, at.out_row = d.QS, at.out_head = HD;
-          at.keys = s->cache + key_base, at.values = s->cache + value_base;
-          at.pages = (cap + (1 << kSpanShift) - 1) >> kSpanShift, at.page_stride = d.KVS << kSpanShift;
-          at.row_stride = d.KVS, at.head_stride = HD, at.shift = kSpanShift;
-          at.table = pf.span->table, at.row_start = pf.span->row_start, at.lengths = &pf.span->length, at.requests = 1;
-          attend_scale(&at, scale);
-          at.cut = p.cut, at.cut.most_keys = (int32_t)cap, at.part = pf.joint;
-          const AttendKernels k = attend_kernels<HD>(p);
-          L(KC_ATTENTION, k.attend, k.grid, dim3(k.threads), k.lds, at);
-          if (at.cut.slots > 0) L(KC_ATTENTION, k.join, k.join_grid, dim3(k.join_threads), 0, at);
+          for (int i = 0; i < spans; ++i) {
+            const int64_t before = (int64_t)kSpanRows * i, n_i = std::min<int64_t>(kSpanRows, rows_n - before);
+            const AttendPlan p = plan_attention(n_i, 1, (int)d.Q, (int)d.KVH, HD, n_i,
+                                                (int64_t)s->h_params[0] + first + before + n_i);
+            const PromptSpan* span = pf.span + i;
+            AttendArgs at{};
+            at.q = qr + before * d.QS, at.q_row = d.QS, at.q_head = HD;
+            at.gate = qg + before * 2 * d.QS + HD, at.gate_row = 2 * d.QS, at.gate_head = 2 * HD;
+            at.out = ctx + before * d.QS, at.out_row = d.QS, at.out_head = HD;
+            at.keys = s->cache + key_base, at.values = s->cache + value_base;
+            at.pages = (cap + (1 << kSpanShift) - 1) >> kSpanShift, at.page_stride = d.KVS << kSpanShift;
+            at.row_stride = d.KVS, at.head_stride = HD, at.shift = kSpanShift;
+            at.table = span->table, at.row_start = span->row_start, at.lengths = &span->length, at.requests = 1;
+            attend_scale(&at, scale);
+            at.cut = p.cut, at.cut.most_keys = (int32_t)cap, at.part = pf.joint;
+            const AttendKernels k = attend_kernels<HD>(p);
+            L(KC_ATTENTION, k.attend, k.grid, dim3(k.threads), k.lds, at);
+            if (at.cut.slots > 0) L(KC_ATTENTION, k.join, k.join_grid, dim3(k.join_threads), 0, at);
+          }
         };
         if (pf.span && d.HD == 256) online(std::integral_constant<int, 256>{});
         else if (pf.span && d.HD == 128) online(std::integral_constant<int, 128>{});

@@ -275,7 +275,8 @@ int cq35_session_matrix_prefill(const cq35_session* session, int* components);
  * maximum and sum instead of two passes over the keys, scores and probabilities
  * kept in F32 where the reference's matrix-core path rounds them to BF16 (the
  * unnormalised weights enter the second product as BF16), keys split over the
- * device where a chunk has few rows (so a call's chunks change its rounding).
+ * device where a call has few rows: how a prompt is divided into calls changes
+ * its rounding, how much device memory is free does not.
  * Tolerance-level, as the component is; 0 (the default) keeps the reference's
  * rounding points. head_dim 64, 128 or 256; sessions of more than 2^22 positions
  * keep the two passes. Prompt buffers hold up to 135 MB more. Copied by

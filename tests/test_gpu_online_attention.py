@@ -126,3 +126,25 @@ def test_long_context_chunk(held):
     r = rel_rms(out[1], out[0])
     say("long chunk: relative logit RMS %.4f" % r)
     assert r <= 0.05
+
+
+@pytest.mark.parametrize("name,components,sizes", [("mini", ATT, [2065, 300]), ("mini", ATT | Session.MATRIX_PROJECTIONS, [40, 4100]),
+                                                   ("mini-moe", ATT | Session.MATRIX_EXPERTS, [3, 2500])])
+def test_chunk_rows_of_short_memory_change_no_bit(monkeypatch, name, components, sizes):
+    """Chunks of 2048 rows and of 1024, as where memory is short: which of them
+    a call gets follows from what else is allocated, its results must not. The
+    layers behind the fourth, whose attention is compared, keep what every row
+    of it left in their state."""
+    cfg = dict(cc.preset(name), layers=8)
+    m = cq35.Model.synthetic(cfg, seed=10)
+    out = []
+    for rows in (0, 1024):
+        monkeypatch.setenv("CQ35_PREFILL_ROWS", str(rows))
+        s = m.session(sum(sizes) + 5)
+        s.set_matrix_prefill(components)
+        s.set_online_attention(True)
+        say("one-pass attention, chunk rows", name, rows)
+        logits = [s.step_raw(p)[0] for p in prompts(cfg, sizes, seed=11)]
+        out.append(logits + [s.export_state(0)])
+    for a, b in zip(*out):
+        assert np.array_equal(a, b)
