@@ -136,6 +136,17 @@ def _table(table, requests, device=None):
     return count, width, row if count > 1 else width
 
 
+def _pair_axis(pair_axis, pairs, axes):
+    """One byte a pair, from a sequence, an array or a tensor of whole numbers."""
+    try:
+        named = bytes(list(pair_axis))  # an array's own bytes are not its values
+    except (TypeError, ValueError, OverflowError) as e:
+        raise (TypeError if isinstance(e, TypeError) else ValueError)(f"pair_axis must hold whole numbers from 0 to {axes - 1}: {e}") from None
+    if len(named) != pairs or not named or max(named) >= axes:
+        raise ValueError(f"pair_axis must name one of {axes} axes for each of {pairs} pairs")
+    return named
+
+
 def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows, out=None, stream=None) -> PagePlan:
     """Pages, positions and slots of a round (cq35_page_plan): request r holds
     cached[r] tokens and is to hold lengths[r] (int32 [requests]). `table` (int32
@@ -195,9 +206,7 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
         raise ValueError(f"positions must be [axes, {rows}] with contiguous rows, not {tuple(positions.shape)}")
     slots = _flat("slots", slots, _I32, rows, device)
     if pair_axis is not None:
-        if len(pair_axis) != pairs or not 0 <= min(pair_axis) <= max(pair_axis) < axes:
-            raise ValueError(f"pair_axis must name one of {axes} axes for each of {pairs} pairs")
-        pair_axis = bytes(pair_axis)
+        pair_axis = _pair_axis(pair_axis, pairs, axes)
     raw, under = _stream(device, stream)
     if out is None:
         with under:

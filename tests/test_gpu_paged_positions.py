@@ -1,0 +1,31 @@
+"""Positions of several axes as callers hold them, and heads at the ends of the
+number range, through cq35.paged_prepare."""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+from test_gpu_paged import cache_tensors, check_prepare, i32, ops, prepare_case, say
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+
+def call(s, k, v, T, **kw):
+    qg, kv = s["qg"].cuda(), s["kv"].cuda()
+    HD, KVH = kv.shape[2], kv.shape[1] // 2
+    args = dict(positions=s["positions"].cuda(), pair_axis=s["axis"], slots=i32(np.arange(T)).cuda())
+    args.update(kw)
+    return ops().paged_prepare(qg[:, :, :HD], kv[:, :KVH], kv[:, KVH:], s["qw"].cuda(), s["kw"].cuda(), s["freq"].cuda(),
+                               args.pop("positions"), args.pop("slots"), k, v, **args)
+
+
+@pytest.mark.parametrize("kind", [np.int64, np.int32, np.uint8, "tensor", bytes, tuple])
+def test_pair_axis_in_any_container(kind):
+    say("pair_axis", kind)
+    T, QH, KVH, HD = 9, 4, 2, 64
+    s = prepare_case(4, T, QH, KVH, HD, 32, 3)
+    k, v = cache_tensors(1, 16, KVH, HD)
+    before = k.cpu().clone(), v.cpu().clone()
+    axis = torch.tensor(s["axis"]) if kind == "tensor" else kind(s["axis"]) if kind in (bytes, tuple) else np.array(s["axis"], kind)
+    check_prepare(s, call(s, k, v, T, pair_axis=axis), k, v, before, list(range(T)), 16)

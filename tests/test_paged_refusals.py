@@ -306,3 +306,27 @@ def test_cut_covers_every_tile_once(index_program):
             int(rng.choice([1, 2, 7, 1024])), int(R <= 64 and i % 2), R, " ".join(map(str, np.concatenate([[0], np.cumsum(new)]))),
             " ".join(map(str, length))))
     assert len(ask(index_program, lines)) == len(lines) > 300
+
+
+@pytest.mark.parametrize("kind", ["list", "tuple", "bytes", "int64", "int32", "uint8", "tensor", "range"])
+def test_pair_axis_in_any_container(kind):
+    """The axes of the pairs as a user may hold them: their values count, not
+    the bytes that hold them."""
+    torch = pytest.importorskip("torch")
+    from cq35 import paged
+    want = [0, 1, 2, 1, 0, 2, 2, 1] if kind != "range" else [0, 1, 2]
+    given = {"list": list, "tuple": tuple, "bytes": bytes, "int64": lambda x: np.array(x, np.int64),
+             "int32": lambda x: np.array(x, np.int32), "uint8": lambda x: np.array(x, np.uint8), "tensor": torch.tensor,
+             "range": lambda x: range(3)}[kind](want)
+    assert list(paged._pair_axis(given, len(want), 3)) == want
+    for bad, pairs, axes in ((given, len(want), 2), (given, len(want) + 1, 3), (given, 0, 3)):
+        with pytest.raises(ValueError, match="pair_axis"):
+            paged._pair_axis(bad, pairs, axes)
+
+
+def test_pair_axis_refusals():
+    pytest.importorskip("torch")
+    from cq35 import paged
+    for bad in ([0, -1], [0, 256], [0, 2**40], [0, 2**80], [0.0, 1.0], np.array([0.0, 1.0]), "01", [None, 0], 3):
+        with pytest.raises((ValueError, TypeError), match="pair_axis"):
+            paged._pair_axis(bad, 2, 2)
