@@ -183,7 +183,7 @@ extern "C" int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_head
   if (rows == 0) return CQ35_OK;
   if (!q_weight || !k_weight || !inv_freq || !positions || !slots) return fail(CQ35_EINVAL, "paged prepare: null argument");
   if (!aligned16(q_weight) || !aligned16(k_weight)) return fail(CQ35_EINVAL, "paged prepare: norm weights not at a 16-byte address");
-  if (axes > 1 && position_stride < rows) return fail(CQ35_EINVAL, "paged prepare: position axes overlap");
+  if (axes > 1 && position_stride != 0 && position_stride < rows) return fail(CQ35_EINVAL, "paged prepare: position axes overlap");
   rc = check_heads("paged prepare: queries", q, rows, q_heads, cache->head_dim, false);
   if (!rc) rc = check_heads("paged prepare: keys", k, rows, cache->kv_heads, cache->head_dim, false);
   if (!rc) rc = check_heads("paged prepare: values", v, rows, cache->kv_heads, cache->head_dim, false);

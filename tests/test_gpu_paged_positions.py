@@ -29,3 +29,18 @@ def test_pair_axis_in_any_container(kind):
     before = k.cpu().clone(), v.cpu().clone()
     axis = torch.tensor(s["axis"]) if kind == "tensor" else kind(s["axis"]) if kind in (bytes, tuple) else np.array(s["axis"], kind)
     check_prepare(s, call(s, k, v, T, pair_axis=axis), k, v, before, list(range(T)), 16)
+
+
+@pytest.mark.parametrize("T,axes", [(1, 3), (2, 2), (33, 3), (700, 4)])
+def test_one_row_of_positions_for_every_axis(T, axes):
+    """Text beside images has one position on all axes: an expanded view of it
+    gives what a copy for each axis gives."""
+    say("expanded positions", T, axes)
+    QH, KVH, HD = 4, 2, 128
+    s = prepare_case(6, T, QH, KVH, HD, 64, axes)
+    s["positions"] = s["positions"][:1].expand(axes, T).contiguous()
+    page = ref.ceil(T, 16)
+    k, v = cache_tensors(page, 16, KVH, HD)
+    before = k.cpu().clone(), v.cpu().clone()
+    out = call(s, k, v, T, positions=s["positions"][:1].cuda().expand(axes, T))
+    check_prepare(s, out, k, v, before, list(range(T)), 16)

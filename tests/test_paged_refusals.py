@@ -330,3 +330,9 @@ def test_pair_axis_refusals():
     for bad in ([0, -1], [0, 256], [0, 2**40], [0, 2**80], [0.0, 1.0], np.array([0.0, 1.0]), "01", [None, 0], 3):
         with pytest.raises((ValueError, TypeError), match="pair_axis"):
             paged._pair_axis(bad, 2, 2)
+
+
+def test_positions_repeated_on_every_axis_are_no_overlap():
+    refused(prepare(axes=2, stride=0, pair_axis=(ctypes.c_uint8 * 8)(0, 1)), -1, "not device memory")
+    for stride in (1, 2, -3):
+        refused(prepare(axes=2, stride=stride, pair_axis=(ctypes.c_uint8 * 8)(0, 1)), -1, "axes overlap")
