@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import operator
 from typing import NamedTuple
 
 import torch
@@ -136,6 +137,14 @@ def _table(table, requests, device=None):
     return count, width, row if count > 1 else width
 
 
+def _int32(name, x):
+    """A number as the library's 32 bits hold it; others would be taken modulo 2^32."""
+    x = operator.index(x)
+    if not -1 << 31 <= x < 1 << 31:
+        raise ValueError(f"{name} is out of range: {x}")
+    return x
+
+
 def _pair_axis(pair_axis, pairs, axes):
     """One byte a pair, from a sequence, an array or a tensor of whole numbers."""
     try:
@@ -157,6 +166,7 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     earlier plan's tensors to write to. `status` is for the caller to look at
     when it next waits for the GPU: unless status[0] is 0 (PLAN_STATUS), nothing
     was changed and the round has no rows."""
+    page_size = _int32("page_size", page_size)
     requests, width, stride = _table(table, None)
     device = table.device
     cached, lengths = _flat("cached", cached, _I32, requests, device), _flat("lengths", lengths, _I32, requests, device)
@@ -264,6 +274,7 @@ def paged_attention(q, key_cache, value_cache, table, row_start, lengths, *, gat
 def paged_attention_workspace(rows, requests, q_heads, kv_heads, head_dim, max_rows=0, max_keys=0) -> int:
     """Bytes of workspace that paged_attention needs for these sizes."""
     b = ctypes.c_int64()
+    q_heads, kv_heads, head_dim = _int32("q_heads", q_heads), _int32("kv_heads", kv_heads), _int32("head_dim", head_dim)
     check(_lib.load().cq35_paged_attention_workspace(rows, requests, q_heads, kv_heads, head_dim, max_rows, max_keys,
                                                      ctypes.byref(b)))
     return b.value

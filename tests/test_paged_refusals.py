@@ -336,3 +336,21 @@ def test_positions_repeated_on_every_axis_are_no_overlap():
     refused(prepare(axes=2, stride=0, pair_axis=(ctypes.c_uint8 * 8)(0, 1)), -1, "not device memory")
     for stride in (1, 2, -3):
         refused(prepare(axes=2, stride=stride, pair_axis=(ctypes.c_uint8 * 8)(0, 1)), -1, "axes overlap")
+
+
+def test_numbers_past_32_bits_are_refused():
+    """Not taken modulo 2^32: a page size of 2^32 + 16 is not one of 16."""
+    torch = pytest.importorskip("torch")
+    import cq35
+    i = torch.zeros(2, dtype=torch.int32)
+    for x in (2**32 + 16, -2**32 + 16, 2**64 + 16):
+        with pytest.raises(ValueError, match="page_size"):
+            cq35.page_plan(i.view(1, 2), i[:1], i[:1], i, i[:1], page_size=x, rows=1)
+    with pytest.raises(TypeError):
+        cq35.page_plan(i.view(1, 2), i[:1], i[:1], i, i[:1], page_size=16.5, rows=1)
+    for at, name in ((2, "q_heads"), (3, "kv_heads"), (4, "head_dim")):
+        sizes = [40, 2, 8, 2, 256]
+        sizes[at] += 2**32
+        with pytest.raises(ValueError, match=name):
+            cq35.paged_attention_workspace(*sizes)
+    assert cq35.paged_attention_workspace(40, 2, 8, 2, 256, 40, 3000) > 0
