@@ -354,3 +354,15 @@ def test_numbers_past_32_bits_are_refused():
         with pytest.raises(ValueError, match=name):
             cq35.paged_attention_workspace(*sizes)
     assert cq35.paged_attention_workspace(40, 2, 8, 2, 256, 40, 3000) > 0
+
+
+def test_star_import_with_and_without_torch():
+    """The package's public names come without torch too, the operators' then aside."""
+    import sys
+    path = os.path.join(ROOT, "catena-models_amd")
+    for hide in ("", "sys.modules['torch'] = None; "):
+        code = ("import sys; sys.path.insert(0, %r); %sfrom cq35 import *; import cq35; assert Model is cq35.Model; "
+                "assert ('page_plan' in globals()) is %s; assert hasattr(cq35, '__all__') and 'page_plan' in dir(cq35)"
+                % (path, hide, not hide))
+        p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+        assert p.returncode == 0, p.stderr
