@@ -417,8 +417,9 @@ int cq35_page_plan(int32_t* table, int64_t table_stride, int64_t requests, int64
  * position that of axis pair_axis[i] (host, rope_dim / 2 entries below `axes`;
  * NULL with one axis): positions[axis * position_stride + t], up to 4 axes
  * (time, height and width of images; a stride of 0 repeats one row of positions
- * on every axis, others are at least `rows`). F32 inside, the angle modulo a turn in
- * 64 bits, each result rounded to BF16 once. q_out may be q itself, laid out
+ * on every axis, others are at least `rows`). F32 inside, the angle modulo a
+ * turn in 64 bits, each result rounded to BF16 once; a head whose mean square
+ * passes F32's range gives zeros. q_out may be q itself, laid out
  * alike. A row whose slot is negative or past the cache is left alone: neither
  * its query nor the cache is written. Slots of one call differ; of two equal
  * ones either row may end up in the cache, piece by piece. Up to 2^26 rows. */

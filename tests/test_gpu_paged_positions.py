@@ -44,3 +44,29 @@ def test_one_row_of_positions_for_every_axis(T, axes):
     before = k.cpu().clone(), v.cpu().clone()
     out = call(s, k, v, T, positions=s["positions"][:1].cuda().expand(axes, T))
     check_prepare(s, out, k, v, before, list(range(T)), 16)
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e30, -3e38])
+def test_heads_whose_squares_pass_the_range(HD, size):
+    """One channel's square passes F32: the head gives zeros, rotated or not;
+    the other heads are what they are without it."""
+    T, QH, KVH = 5, 4, 2
+    s = prepare_case(11, T, QH, KVH, HD, 32, 1)
+    huge = dict(s, qg=s["qg"].clone(), kv=s["kv"].clone())
+    huge["qg"][1, 2, HD - 1] = size
+    huge["qg"][4, 0, 3] = size
+    huge["kv"][2, 1, 7] = size
+    huge["kv"][3, KVH, 5] = size  # a value: copied as it is
+    k, v = cache_tensors(1, 16, KVH, HD)
+    say("huge heads", HD, size)
+    out = call(huge, k, v, T, positions=s["positions"][0].cuda(), pair_axis=None).cpu()
+    assert bool((out[1, 2] == 0).all()) and bool((out[4, 0] == 0).all()) and bool((k[0, 2, 1] == 0).all())
+    assert torch.equal(v[0, :T].cpu(), huge["kv"][:, KVH:])
+    k2, v2 = cache_tensors(1, 16, KVH, HD)
+    plain = call(s, k2, v2, T, positions=s["positions"][0].cuda(), pair_axis=None).cpu()
+    for t in range(T):
+        for h in range(QH):
+            assert (t, h) in ((1, 2), (4, 0)) or torch.equal(out[t, h], plain[t, h])
+        for h in range(KVH):
+            assert (t, h) == (2, 1) or torch.equal(k[0, t, h], k2[0, t, h])
