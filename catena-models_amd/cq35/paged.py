@@ -6,9 +6,11 @@ tokens over the pages (`paged_attention`).
 Tensors lie on one GPU, which need not be the current one; work goes to that
 device's current torch stream, or to `stream` (a torch.cuda.Stream). Nothing
 waits for the GPU, and every call may be captured into a graph. Results carry no
-gradients. A cache is a
-pair of BF16 tensors [pages, page_size, kv_heads, head_dim] (views with other
-strides included, head_dim contiguous).
+gradients. Rows of a result that the call leaves alone (no slot, no request) are
+uninitialised where the result is new: a round of more rows than its requests
+have, whose rows all go on into other work, passes an `out` zeroed beforehand. A
+cache is a pair of BF16 tensors [pages, page_size, kv_heads, head_dim] (views
+with other strides included, head_dim contiguous).
 """
 from __future__ import annotations
 

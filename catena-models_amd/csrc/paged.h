@@ -152,9 +152,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(PlanArgs a) {
 // i + rope_dim / 2 of the first rope_dim are turned by the angle
 // position[axis_i] * inv_freq[i]; queries go to q_out, keys and the unchanged
 // values to their cache rows. F32 throughout, each result rounded to BF16
-// once. The angle is the exact product taken modulo a turn in 64 bits: an F32
-// angle is off by up to 2^-24 of itself, a sixteenth of a turn at position
-// 10^6, where the 64-bit one is within 2^-32 of a turn at any position.
+// once. The angle is the product taken modulo a turn in 64 bits: an F32 angle is
+// off by up to 2^-24 of itself, a sixteenth of a radian at position 10^6. Here
+// the product (exact below position 2^29), 1 / (2 pi) and their product are each
+// off by at most 2^-53 of the turns, the remainder's rounding to F32 by 2^-26 of
+// a turn: together 2^-26 up to 2^20 turns or so, below 2^-22 of a turn at
+// position 2^31 - 1 with a frequency of 1.
 //
 // A head is head_dim / 8 lanes of 16 bytes; a block takes `tokens` rows, makes
 // their cosines and sines once in LDS (one pair per thread) and deals the

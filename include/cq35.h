@@ -445,7 +445,9 @@ int cq35_paged_prepare(const cq35_paged_cache* cache, const cq35_heads* q, const
  * whatever its values and its gate.
  * Keys in pages whose number is outside the cache are not seen; lengths are
  * cut to what the table holds (at most 2^30 keys). Rows outside every request
- * are left alone. Up to 8192 requests; rows * q_heads below about 2^27. out may be
+ * are left alone. row_start ascends from 0 or more: where it does not, rows of a
+ * request that overlaps another's hold either's results or are left alone, as are
+ * those of later requests; rows past `rows` are not read or written. Up to 8192 requests; rows * q_heads below about 2^27. out may be
  * q itself, laid out alike; it overlaps no other operand.
  * max_rows and max_keys are what the caller knows of the most rows and keys of
  * any request, 0 for nothing: they steer how the work is cut and the launches
