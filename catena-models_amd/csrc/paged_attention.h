@@ -740,8 +740,8 @@ __global__ __launch_bounds__(kFewThreads, HD == 256 ? 1 : 2) void k_paged_few(At
 // run of their own: 1.08 ms; a phase apart with that run: 1.15 ms; values'
 // products and scores in one run without places in the lanes (table and strides
 // worked on every stage): 1.26 ms. 16 mixed requests (500, 300, 223 and single
-// tokens over up to 4096 keys of 256 channels) take 62 us, 18 more for the join:
-// 19 stages, then 50 MB of partial results by all items at once.
+// tokens over up to 4096 keys of 256 channels) take 59 to 62 us, 18 more for the
+// join: 19 stages, then 44 MB of partial results by all items at once.
 constexpr int kManyThreads = 512;
 constexpr int kManyRows = 256;
 constexpr int kManyStages = 4;
