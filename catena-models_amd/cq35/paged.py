@@ -168,7 +168,8 @@ def page_plan(table, cached, lengths, free_pages, free_count, *, page_size, rows
     earlier plan's tensors to write to. `status` is for the caller to look at
     when it next waits for the GPU: unless status[0] is 0 (PLAN_STATUS), nothing
     was changed and the round has no rows."""
-    page_size = _int32("page_size", page_size)
+    if type(page_size) is not int or not 0 < page_size < 1 << 31:
+        page_size = _int32("page_size", page_size)
     requests, width, stride = _table(table, None)
     device = table.device
     cached, lengths = _flat("cached", cached, _I32, requests, device), _flat("lengths", lengths, _I32, requests, device)
