@@ -148,7 +148,8 @@ def _int32(name, x):
 
 
 def _pair_axis(pair_axis, pairs, axes):
-    """One byte a pair, from a sequence, an array or a tensor of whole numbers."""
+    """One byte a pair, from a sequence, an array or a tensor of whole numbers in
+    host memory (one on the GPU would be waited for)."""
     try:
         named = bytes(list(pair_axis))  # an array's own bytes are not its values
     except (TypeError, ValueError, OverflowError) as e:
@@ -202,8 +203,8 @@ def paged_prepare(q, k, v, q_weight, k_weight, inv_freq, positions, slots, key_c
     q_heads, head_dim], k and v [rows, kv_heads, head_dim] BF16 with any row and
     head strides (the query half of a query/gate projection is such a view);
     weights F32 [head_dim]; inv_freq F32 [rope_dim / 2]; positions int32 [rows],
-    or [axes, rows] (an expanded row included) with pair_axis[i] the axis of
-    rotated pair i. `out`: the tensor for the queries, q itself allowed."""
+    or [axes, rows] (an expanded row included) with pair_axis[i] (held
+    on the host) the axis of rotated pair i. `out`: the tensor for the queries, q itself allowed."""
     device, cache = _cache(key_cache, value_cache)
     shape, rows, q_heads = _query_shape(q, cache, device)
     kv_shape = (rows, cache.kv_heads, cache.head_dim)
