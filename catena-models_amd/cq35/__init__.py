@@ -20,20 +20,25 @@ __all__ = [
     "CQ35Error", "LIBRARY", "load", "SPLIT_KEYS_DEFAULT",
 ]
 
-# the operators over torch tensors (paged.py), loaded on first use: the rest of
-# the package runs without torch, and a star import takes them where torch is
+# the operators over torch tensors (paged.py, int8.py, logprobs.py), loaded on
+# first use: the rest of the package runs without torch, and a star import takes
+# them where torch is
 _PAGED = ("PLAN_STATUS", "PagePlan", "page_plan", "paged_prepare", "paged_attention", "paged_attention_workspace")
+_INT8 = ("Int8Rows", "NormRows", "quantize_rows", "norm_quantize", "gated_quantize", "int8_linear")
+_LOGPROBS = ("TokenLogprobs", "token_logprobs", "token_logprobs_workspace")
+_TENSOR = _PAGED + _INT8 + _LOGPROBS
 if sys.modules["torch"] is not None if "torch" in sys.modules else importlib.util.find_spec("torch") is not None:
-    __all__ += _PAGED
+    __all__ += _TENSOR
 
 
 def __dir__():
-    return sorted({*globals(), *_PAGED})
+    return sorted({*globals(), *_TENSOR})
 
 
 def __getattr__(name):
-    if name in _PAGED:
-        from . import paged
-        globals().update((n, getattr(paged, n)) for n in _PAGED)
+    if name in _TENSOR:
+        from . import int8, logprobs, paged
+        globals().update((n, getattr(m, n)) for m, names in ((paged, _PAGED), (int8, _INT8), (logprobs, _LOGPROBS))
+                         for n in names)
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -36,6 +36,16 @@ class Heads(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
+class Rows(ctypes.Structure):
+    """Mirror of ``cq35_rows``."""
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class Int8Rows(ctypes.Structure):
+    """Mirror of ``cq35_int8_rows``."""
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("scale", ctypes.c_void_p)]
+
+
 def load():
     """Load the in-tree library; raise loudly when it has not been built."""
     global _lib
@@ -49,6 +59,7 @@ def load():
     P, I64, I32, U64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_uint64
     PC = ctypes.POINTER(CConfig)
     PG, PH = ctypes.POINTER(PagedCache), ctypes.POINTER(Heads)
+    PR, P8 = ctypes.POINTER(Rows), ctypes.POINTER(Int8Rows)
     sig = {
         "cq35_last_error": ([], ctypes.c_char_p),
         "cq35_abi_version": ([], ctypes.c_int),
@@ -108,6 +119,12 @@ def load():
         "cq35_paged_attention_workspace": ([I64, I64, I32, I32, I32, I64, I64, ctypes.POINTER(I64)], ctypes.c_int),
         "cq35_paged_attention": ([PG, PH, PH, PH, I64, I32, P, I64, I64, I64, P, P, ctypes.c_float, I64, I64, P, I64, P],
                                  ctypes.c_int),
+        "cq35_quantize_rows": ([PR, I64, I64, P8, P], ctypes.c_int),
+        "cq35_norm_quantize": ([PR, PR, P, ctypes.c_float, I64, I64, PR, P8, P], ctypes.c_int),
+        "cq35_gated_quantize": ([PR, PR, I64, I64, P8, P], ctypes.c_int),
+        "cq35_int8_linear": ([P8, P8, I64, I64, I64, PR, P], ctypes.c_int),
+        "cq35_token_logprobs_workspace": ([I64, I64, I64, I32, ctypes.POINTER(I64)], ctypes.c_int),
+        "cq35_token_logprobs": ([PR, I64, I64, P, I64, I32, P, P, P, P, P, I64, P], ctypes.c_int),
         "cq35_session_phase_trace": ([P, P, I64, ctypes.POINTER(I64), ctypes.POINTER(I64)], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
@@ -141,4 +158,6 @@ EXPORTED = [
     "cq35_session_attention_split", "cq35_session_phase_trace",
     "cq35_session_set_online_attention", "cq35_session_online_attention",
     "cq35_page_plan", "cq35_paged_prepare", "cq35_paged_attention_workspace", "cq35_paged_attention",
+    "cq35_quantize_rows", "cq35_norm_quantize", "cq35_gated_quantize", "cq35_int8_linear",
+    "cq35_token_logprobs_workspace", "cq35_token_logprobs",
 ]

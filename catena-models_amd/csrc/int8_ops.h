@@ -1,0 +1,192 @@
+// C entry points of the 8-bit rows and products and of the log probabilities:
+// argument checks, then the launches on the caller's stream, as the paged-cache
+// operators' are.
+#pragma once
+
+#include "int8_product.h"
+#include "int8_rows.h"
+#include "logprobs.h"
+#include "operator_call.h"
+
+namespace {
+
+constexpr int64_t kMostRows = 1 << 21;  // times 1024 threads: a launch takes below 2^32
+constexpr int64_t kMostResults = 1ll << 34;  // in tiles of 64 x 64 by 256 threads as well
+
+bool row_type(int32_t dtype) { return dtype == CQ35_BF16 || dtype == CQ35_F32; }
+
+// Rows read or written in 16-byte pieces.
+int check_rows(const char* what, const cq35_rows* r, int64_t rows, int64_t channels, bool written) {
+  if (!r || !r->data) return fail(CQ35_EINVAL, "%s: null argument", what);
+  if (!row_type(r->dtype)) return fail(CQ35_EUNSUPPORTED, "%s: type %d is neither BF16 nor F32", what, r->dtype);
+  const int unit = r->dtype == CQ35_BF16 ? 8 : 4;
+  if (!aligned16(r->data)) return fail(CQ35_EINVAL, "%s: not at a 16-byte address", what);
+  if (r->row_stride < 0 || r->row_stride % unit)
+    return fail(CQ35_EINVAL, "%s: rows %lld elements apart, not a multiple of %d", what, (long long)r->row_stride, unit);
+  if (written && !distinct({{rows, r->row_stride}}, channels)) return fail(CQ35_EINVAL, "%s: rows overlap", what);
+  return CQ35_OK;
+}
+
+int check_int8_rows(const char* what, const cq35_int8_rows* r, int64_t rows, int64_t channels, bool written) {
+  if (!r || !r->data || !r->scale) return fail(CQ35_EINVAL, "%s: null argument", what);
+  if (!aligned16(r->data)) return fail(CQ35_EINVAL, "%s: not at a 16-byte address", what);
+  if (r->row_stride < 0 || r->row_stride % 16)
+    return fail(CQ35_EINVAL, "%s: rows %lld bytes apart, not a multiple of 16", what, (long long)r->row_stride);
+  if (written && !distinct({{rows, r->row_stride}}, channels)) return fail(CQ35_EINVAL, "%s: rows overlap", what);
+  return CQ35_OK;
+}
+
+int check_row_sizes(const char* what, int64_t rows, int64_t channels) {
+  if (rows < 0 || rows > kMostRows) return fail(CQ35_ERANGE, "%s: %lld rows, not up to 2^21", what, (long long)rows);
+  if (channels < 16 || channels > kProductMostChannels || channels % 16)
+    return fail(CQ35_ERANGE, "%s: %lld channels, not a multiple of 16 up to 65536", what, (long long)channels);
+  return CQ35_OK;
+}
+
+template <typename T, RowSource kSource>
+int launch_rows(const char* what, const RowArgs& a, hipStream_t s) {
+  constexpr int E = RowPiece<T>::kValues;
+  if (a.channels <= 2048)
+    return launch_operator(what, k_int8_rows<T, kSource, 64, 32 / E>, dim3((unsigned)((a.rows + 3) / 4)), 256, 0, s, a);
+  if (a.channels <= 8192) return launch_operator(what, k_int8_rows<T, kSource, 256, 32 / E>, dim3((unsigned)a.rows), 256, 0, s, a);
+  return launch_operator(what, k_int8_rows<T, kSource, 1024, 64 / E>, dim3((unsigned)a.rows), 1024, 0, s, a);
+}
+
+template <RowSource kSource>
+int launch_rows(const char* what, int32_t dtype, const RowArgs& a, hipStream_t s) {
+  return dtype == CQ35_BF16 ? launch_rows<uint16_t, kSource>(what, a, s) : launch_rows<float, kSource>(what, a, s);
+}
+
+RowArgs row_args(const cq35_rows* x, int64_t rows, int64_t channels, const cq35_int8_rows* out) {
+  RowArgs a{};
+  a.a = x->data, a.a_stride = x->row_stride, a.rows = rows, a.channels = (int)channels;
+  a.data = out->data, a.data_stride = out->row_stride, a.scale = out->scale;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int cq35_quantize_rows(const cq35_rows* x, int64_t rows, int64_t channels, const cq35_int8_rows* out,
+                                  void* stream) {
+  int rc = check_row_sizes("quantize rows", rows, channels);
+  if (rc || rows == 0) return rc;
+  rc = check_rows("quantize rows: input", x, rows, channels, false);
+  if (!rc) rc = check_int8_rows("quantize rows: output", out, rows, channels, true);
+  if (rc) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  OperatorDevice on;
+  rc = on.enter({x->data, out->data, out->scale}, s);
+  if (rc) return rc;
+  return launch_rows<RowSource::kPlain>("quantize rows", x->dtype, row_args(x, rows, channels, out), s);
+}
+
+extern "C" int cq35_norm_quantize(const cq35_rows* x, const cq35_rows* residual, const float* weight, float eps,
+                                  int64_t rows, int64_t channels, const cq35_rows* summed, const cq35_int8_rows* out,
+                                  void* stream) {
+  int rc = check_row_sizes("norm quantize", rows, channels);
+  if (rc) return rc;
+  if (!(eps >= 0.0f)) return fail(CQ35_EINVAL, "norm quantize: eps %g", (double)eps);
+  if (rows == 0) return CQ35_OK;
+  if (!weight) return fail(CQ35_EINVAL, "norm quantize: null argument");
+  if (!aligned16(weight)) return fail(CQ35_EINVAL, "norm quantize: weights not at a 16-byte address");
+  rc = check_rows("norm quantize: input", x, rows, channels, false);
+  if (!rc && residual) rc = check_rows("norm quantize: residual", residual, rows, channels, false);
+  if (!rc && residual) rc = check_rows("norm quantize: sum", summed, rows, channels, true);
+  if (!rc) rc = check_int8_rows("norm quantize: output", out, rows, channels, true);
+  if (rc) return rc;
+  if (residual && (residual->dtype != x->dtype || summed->dtype != x->dtype))
+    return fail(CQ35_EINVAL, "norm quantize: input, residual and sum of types %d, %d and %d", x->dtype, residual->dtype, summed->dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  OperatorDevice on;
+  rc = on.enter({x->data, weight, residual ? residual->data : nullptr, residual ? summed->data : nullptr, out->data, out->scale}, s);
+  if (rc) return rc;
+  RowArgs a = row_args(x, rows, channels, out);
+  a.weight = weight, a.eps = eps;
+  if (residual) a.b = residual->data, a.b_stride = residual->row_stride, a.sum = summed->data, a.sum_stride = summed->row_stride;
+  return launch_rows<RowSource::kNorm>("norm quantize", x->dtype, a, s);
+}
+
+extern "C" int cq35_gated_quantize(const cq35_rows* gate, const cq35_rows* up, int64_t rows, int64_t channels,
+                                   const cq35_int8_rows* out, void* stream) {
+  int rc = check_row_sizes("gated quantize", rows, channels);
+  if (rc || rows == 0) return rc;
+  rc = check_rows("gated quantize: gate", gate, rows, channels, false);
+  if (!rc) rc = check_rows("gated quantize: up", up, rows, channels, false);
+  if (!rc) rc = check_int8_rows("gated quantize: output", out, rows, channels, true);
+  if (rc) return rc;
+  if (gate->dtype != up->dtype) return fail(CQ35_EINVAL, "gated quantize: gate and up of types %d and %d", gate->dtype, up->dtype);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  OperatorDevice on;
+  rc = on.enter({gate->data, up->data, out->data, out->scale}, s);
+  if (rc) return rc;
+  RowArgs a = row_args(gate, rows, channels, out);
+  a.b = up->data, a.b_stride = up->row_stride;
+  return launch_rows<RowSource::kGated>("gated quantize", gate->dtype, a, s);
+}
+
+extern "C" int cq35_int8_linear(const cq35_int8_rows* x, const cq35_int8_rows* w, int64_t rows, int64_t outputs,
+                                int64_t channels, const cq35_rows* out, void* stream) {
+  int rc = check_row_sizes("int8 linear", rows, channels);
+  if (rc) return rc;
+  if (outputs < 1 || outputs > kMostRows) return fail(CQ35_ERANGE, "int8 linear: %lld outputs, not 1 to 2^21", (long long)outputs);
+  if (rows * outputs > kMostResults)
+    return fail(CQ35_ERANGE, "int8 linear: too many results for one call: %lld x %lld", (long long)rows, (long long)outputs);
+  if (rows == 0) return CQ35_OK;
+  rc = check_int8_rows("int8 linear: input", x, rows, channels, false);
+  if (!rc) rc = check_int8_rows("int8 linear: weights", w, outputs, channels, false);
+  if (rc) return rc;
+  if (!out || !out->data) return fail(CQ35_EINVAL, "int8 linear: output: null argument");
+  if (!row_type(out->dtype)) return fail(CQ35_EUNSUPPORTED, "int8 linear: output: type %d is neither BF16 nor F32", out->dtype);
+  if ((uintptr_t)out->data % (out->dtype == CQ35_BF16 ? 2 : 4)) return fail(CQ35_EINVAL, "int8 linear: output: misaligned");
+  if (out->row_stride < 0 || !distinct({{rows, out->row_stride}}, outputs)) return fail(CQ35_EINVAL, "int8 linear: output: rows overlap");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  OperatorDevice on;
+  rc = on.enter({x->data, x->scale, w->data, w->scale, out->data}, s);
+  if (rc) return rc;
+  const ProductArgs a{x->data, w->data, x->row_stride, w->row_stride, x->scale, w->scale, rows, outputs, (int)channels,
+                      out->data, out->row_stride};
+  const dim3 grid((unsigned)(((outputs + 63) / 64) * ((rows + 63) / 64)));
+  return launch_operator("int8 linear", out->dtype == CQ35_BF16 ? k_int8_product<uint16_t> : k_int8_product<float>, grid, 256, 0, s, a);
+}
+
+namespace {
+
+int check_logprob_sizes(const char* what, int64_t rows, int64_t vocab, int64_t given, int32_t top) {
+  if (rows < 0 || rows > kMostRows || vocab < 1 || vocab > 1 << 30)
+    return fail(CQ35_ERANGE, "%s: %lld rows of %lld logits", what, (long long)rows, (long long)vocab);
+  if (given < 0 || given > kLogprobsMostGiven)
+    return fail(CQ35_ERANGE, "%s: %lld given tokens a row, not up to %d", what, (long long)given, kLogprobsMostGiven);
+  if (top < 0 || top > kLogprobsMostTop || top > vocab)
+    return fail(CQ35_ERANGE, "%s: %d alternatives, not up to %d", what, top, (int)std::min<int64_t>(vocab, kLogprobsMostTop));
+  return CQ35_OK;
+}
+
+}  // namespace
+
+extern "C" int cq35_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t given, int32_t top, int64_t* bytes) {
+  if (!bytes) return fail(CQ35_EINVAL, "token logprobs workspace: null argument");
+  const int rc = check_logprob_sizes("token logprobs workspace", rows, vocab, given, top);
+  if (!rc) *bytes = 0;
+  return rc;
+}
+
+extern "C" int cq35_token_logprobs(const cq35_rows* logits, int64_t rows, int64_t vocab, const int64_t* tokens,
+                                   int64_t given, int32_t top, float* logprobs, float* entropy, int64_t* top_tokens,
+                                   float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_logprob_sizes("token logprobs", rows, vocab, given, top);
+  if (rc || rows == 0) return rc;
+  if (!logits || !logits->data || !entropy || (given > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_tokens || !top_logprobs)))
+    return fail(CQ35_EINVAL, "token logprobs: null argument");
+  if (!row_type(logits->dtype)) return fail(CQ35_EUNSUPPORTED, "token logprobs: type %d is neither BF16 nor F32", logits->dtype);
+  if ((uintptr_t)logits->data % (logits->dtype == CQ35_BF16 ? 2 : 4) || logits->row_stride < 0)
+    return fail(CQ35_EINVAL, "token logprobs: logits misaligned, or rows %lld apart", (long long)logits->row_stride);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  OperatorDevice on;
+  rc = on.enter({logits->data, entropy, given ? tokens : nullptr, given ? logprobs : nullptr, top ? top_tokens : nullptr,
+                 top ? top_logprobs : nullptr}, s);
+  if (rc) return rc;
+  const LogprobArgs a{logits->data, logits->row_stride, rows, (int)vocab, tokens, (int)given, top, logprobs, entropy, top_tokens,
+                      top_logprobs};
+  return launch_operator("token logprobs", logits->dtype == CQ35_BF16 ? k_logprobs<uint16_t> : k_logprobs<float>,
+                         dim3((unsigned)rows), kLogprobThreads, 0, s, a);
+}

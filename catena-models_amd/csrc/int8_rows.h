@@ -1,0 +1,166 @@
+// Rows of 8-bit integers with a scale each: plain rows (k_int8_rows of
+// RowSource::kPlain), the norm of rows with the residual's addition (RowSource::kNorm) and the
+// gated product of a feed-forward (RowSource::kGated).
+#pragma once
+
+#include "layers.h"
+
+namespace cq35 {
+
+// With a = max |y_i| of a row: scale = a / 127, q_i = rint(y_i * (127 / a)), half
+// to even, so |q_i| is at most 127. A row with a value that is not finite gets the
+// scale NaN, one without a magnitude of 127 * 2^-126 (whose scale would lose bits
+// in the subnormals) the scale 0, both zeros.
+enum class RowSource { kPlain, kNorm, kGated };
+constexpr float kLeastAmax = 127.0f * 1.17549435e-38f;
+
+struct RowArgs {
+  const void *a, *b;  // rows, and the residual or the up projection
+  int64_t a_stride, b_stride;
+  void* sum;
+  int64_t sum_stride;
+  const float* weight;
+  float eps;
+  int64_t rows;
+  int channels;
+  int8_t* data;
+  int64_t data_stride;
+  float* scale;
+};
+
+// A 16-byte piece of a row of T.
+template <typename T>
+struct RowPiece;
+template <>
+struct RowPiece<uint16_t> {
+  static constexpr int kValues = 8;
+  static __device__ __forceinline__ void widen(const u32x4& raw, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = lo2f(raw[i]), x[2 * i + 1] = hi2f(raw[i]);
+  }
+  static __device__ __forceinline__ u32x4 narrow(const float* x) {
+    u32x4 raw;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = (uint32_t)f2bf(x[2 * i]) | (uint32_t)f2bf(x[2 * i + 1]) << 16;
+    return raw;
+  }
+};
+template <>
+struct RowPiece<float> {
+  static constexpr int kValues = 4;
+  static __device__ __forceinline__ void widen(const u32x4& raw, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = bitsf(raw[i]);
+  }
+  static __device__ __forceinline__ u32x4 narrow(const float* x) {
+    return u32x4{fbits(x[0]), fbits(x[1]), fbits(x[2]), fbits(x[3])};
+  }
+};
+
+// Four values, already times 127 / a, rounded half to even: the sum with 1.5 * 2^23 has
+// the integer in its low bits.
+__device__ __forceinline__ uint32_t pack_int8(const float* v) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = fbits(v[i] + 12582912.0f);
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+  return lo | hi << 16;
+}
+
+// kLanes threads a row, kPieces pieces of 16 bytes a thread.
+template <typename T, RowSource kSource, int kLanes, int kPieces>
+__global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowArgs a) {
+  typedef RowPiece<T> P;
+  constexpr int E = P::kValues, kThreads = kLanes < 256 ? 256 : kLanes, kWaves = kLanes / 64;
+  __shared__ float sums[kWaves];
+  __shared__ uint32_t most[kWaves];
+  const int tid = threadIdx.x, lane = tid % kLanes, wave = lane >> 6;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + tid / kLanes;
+  if (row >= a.rows) return;  // whole waves; only where a wave is a row
+  const T *xa = (const T*)a.a + row * a.a_stride, *xb = (const T*)a.b + row * a.b_stride;
+  float y[kPieces][E];
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = (p * kLanes + lane) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[p][e] = 0.0f;
+    if (i >= a.channels) continue;
+    P::widen(*reinterpret_cast<const u32x4*>(xa + i), y[p]);
+    if (kSource == RowSource::kNorm && a.b) {
+      float r[E];
+      P::widen(*reinterpret_cast<const u32x4*>(xb + i), r);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[p][e] += r[e];
+      // the sum in the stream's type is what the norm sees
+      const u32x4 raw = P::narrow(y[p]);
+      *reinterpret_cast<u32x4*>((T*)a.sum + row * a.sum_stride + i) = raw;
+      P::widen(raw, y[p]);
+    }
+    if (kSource == RowSource::kGated) {
+      float u[E];
+      P::widen(*reinterpret_cast<const u32x4*>(xb + i), u);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        y[p][e] = y[p][e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y[p][e] * -1.44269504f)) * u[e];
+    }
+  }
+  if (kSource == RowSource::kNorm) {
+    float s = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int e = 0; e < E; ++e) s = __builtin_fmaf(y[p][e], y[p][e], s);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+    if (kWaves > 1) {
+      if ((tid & 63) == 0) sums[wave] = s;
+      __syncthreads();
+      s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) s += sums[w];
+    }
+    const float inverse = 1.0f / sqrtf(s / (float)a.channels + a.eps);
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int i = (p * kLanes + lane) * E;
+      if (i >= a.channels) continue;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const float4 w = *reinterpret_cast<const float4*>(a.weight + i + e);
+        y[p][e] = y[p][e] * inverse * w.x, y[p][e + 1] = y[p][e + 1] * inverse * w.y;
+        y[p][e + 2] = y[p][e + 2] * inverse * w.z, y[p][e + 3] = y[p][e + 3] * inverse * w.w;
+      }
+    }
+  }
+  // magnitudes as integers: infinity and NaN are the largest
+  uint32_t m = 0;
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = max(m, fbits(y[p][e]) & 0x7fffffffu);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+  if (kWaves > 1) {
+    if ((tid & 63) == 0) most[wave] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = max(m, most[w]);
+  }
+  const float amax = bitsf(m);
+  const bool zeros = m >= 0x7f800000u || amax < kLeastAmax;
+  const float up = 127.0f / amax;
+  if (lane == 0) a.scale[row] = m >= 0x7f800000u ? bitsf(0x7fc00000u) : amax < kLeastAmax ? 0.0f : amax / 127.0f;
+  int8_t* to = a.data + row * a.data_stride;
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = (p * kLanes + lane) * E;
+    if (i >= a.channels) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[p][e] = zeros ? 0.0f : y[p][e] * up;
+    if (E == 8) *reinterpret_cast<uint2*>(to + i) = make_uint2(pack_int8(y[p]), pack_int8(y[p] + E / 2));
+    else *reinterpret_cast<uint32_t*>(to + i) = pack_int8(y[p]);
+  }
+}
+
+}  // namespace cq35

@@ -465,6 +465,79 @@ int cq35_paged_attention(const cq35_paged_cache* cache, const cq35_heads* q, con
                          int64_t max_rows, int64_t max_keys, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------ 8-bit rows and products
+ * Operators over device memory for what a round runs before, between and behind
+ * the paged-cache operators: a layer's projections in 8-bit integers
+ * (cq35_quantize_rows, cq35_norm_quantize, cq35_gated_quantize make their inputs,
+ * cq35_quantize_rows their weights once; cq35_int8_linear is the product) and the
+ * log probabilities of what is answered (cq35_token_logprobs). No reference
+ * counterpart (its products take BF16 weights). Pointers, streams, errors and
+ * capture are as with the paged cache. */
+
+/* Rows of CQ35_BF16 or CQ35_F32 values: row t starts at t * row_stride elements
+ * (0 repeats one row of an input). Unless said otherwise the base is a 16-byte
+ * address and the stride a multiple of 16 bytes. */
+typedef struct cq35_rows {
+  void* data;
+  int64_t row_stride;
+  int32_t dtype;
+} cq35_rows;
+
+/* Rows of 8-bit integers with a scale each: element i of row t stands for
+ * data[t * row_stride + i] * scale[t]. The base is a 16-byte address, the stride a
+ * multiple of 16; channels are a multiple of 16, at most 65536. */
+typedef struct cq35_int8_rows {
+  int8_t* data;
+  int64_t row_stride;
+  float* scale;
+} cq35_int8_rows;
+
+/* 8-bit rows of y: with a = max |y_i| of a row scale = a / 127 and q_i = y_i * (127 / a)
+ * rounded to the nearest integer, half to even (-127 to 127). A row with a value that
+ * is not finite gets the scale NaN and zeros, so that what is made of it is NaN; a
+ * row without a magnitude of 127 * 2^-126 or more gets the scale 0 and zeros.
+ *   cq35_quantize_rows:  y = x
+ *   cq35_norm_quantize:  y = h w / sqrt(mean(h^2) + eps) with h = x + residual, rounded to
+ *     their type and written to `summed` (x or residual itself allowed, laid out
+ *     alike); without a residual (NULL) h = x and nothing is written. w: F32, at a
+ *     16-byte address. A row whose mean square passes F32's range gives zeros. x,
+ *     residual and summed have one type.
+ *   cq35_gated_quantize: y = gate / (1 + e^-gate) * up, of one type
+ * F32 inside. Outputs overlap no input, summed apart. Up to 2^21 rows. */
+int cq35_quantize_rows(const cq35_rows* x, int64_t rows, int64_t channels, const cq35_int8_rows* out,
+                       void* stream);
+int cq35_norm_quantize(const cq35_rows* x, const cq35_rows* residual, const float* weight, float eps,
+                       int64_t rows, int64_t channels, const cq35_rows* summed, const cq35_int8_rows* out,
+                       void* stream);
+int cq35_gated_quantize(const cq35_rows* gate, const cq35_rows* up, int64_t rows, int64_t channels,
+                        const cq35_int8_rows* out, void* stream);
+
+/* out[m][n] = (sum_k x[m][k] w[n][k]) * x.scale[m] * w.scale[n] for `rows` rows of x and
+ * `outputs` rows of w: the sum exact, rounded to F32, each product rounded to F32, the
+ * result to out's type. All values of an 8-bit integer are taken, -128 too. Rows
+ * of out may lie anywhere that its elements may (no 16-byte rule), row_stride at least
+ * `outputs`. Up to 2^21 rows and outputs, 2^34 results. */
+int cq35_int8_linear(const cq35_int8_rows* x, const cq35_int8_rows* w, int64_t rows, int64_t outputs,
+                     int64_t channels, const cq35_rows* out, void* stream);
+
+/* Of each row of `vocab` logits x (any stride, at addresses of their type), in F32, with
+ * m = max x and s = sum e^(x - m):
+ *   logprobs[rows][given]:   (x[t] - m) - log s of the tokens t = tokens[rows][given]
+ *                            (contiguous); NaN where t is no index of the row
+ *   entropy[rows]:           log s - sum e^(x - m) (x - m) / s, a logit of -inf adding nothing
+ *   top_tokens, top_logprobs [rows][top]: the `top` largest logits in descending order,
+ *                            among equal ones the lowest index first (-0 equals 0)
+ * A row that holds NaN or +inf, or nothing above -inf, gets NaN for every log
+ * probability and the entropy; its top tokens are in the same order, NaN before
+ * +inf. given: 0 to 1024; top: 0 to 32, at most vocab; vocab up to 2^30, rows to 2^21.
+ * workspace: cq35_token_logprobs_workspace bytes (of the same arguments) at a 16-byte
+ * address, used during the call's work only and by no other work at that time; NULL
+ * where 0 bytes are needed. The same call gives the same bits. */
+int cq35_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t given, int32_t top, int64_t* bytes);
+int cq35_token_logprobs(const cq35_rows* logits, int64_t rows, int64_t vocab, const int64_t* tokens,
+                        int64_t given, int32_t top, float* logprobs, float* entropy, int64_t* top_tokens,
+                        float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
