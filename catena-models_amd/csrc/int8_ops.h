@@ -11,6 +11,7 @@
 namespace {
 
 constexpr int64_t kMostRows = 1 << 21;  // times 1024 threads: a launch takes below 2^32
+constexpr int64_t kLogprobBlocks = 1024;  // four a CU; more rows take a block each
 constexpr int64_t kMostResults = 1ll << 34;  // in tiles of 64 x 64 by 256 threads as well
 
 bool row_type(int32_t dtype) { return dtype == CQ35_BF16 || dtype == CQ35_F32; }
@@ -161,12 +162,33 @@ int check_logprob_sizes(const char* what, int64_t rows, int64_t vocab, int64_t g
   return CQ35_OK;
 }
 
+// Blocks of a row, and the bytes of workspace they need.
+struct LogprobPlan {
+  int splits;
+  int64_t keys_at, bytes;
+};
+LogprobPlan plan_logprobs(int64_t rows, int64_t vocab, int32_t top) {
+  const int64_t tiles = (vocab + LogitTile<uint16_t>::kLogits - 1) / LogitTile<uint16_t>::kLogits;  // of BF16, half as many as of F32
+  const int64_t wanted = std::max<int64_t>(1, kLogprobBlocks / std::max<int64_t>(rows, 1));
+  LogprobPlan p{(int)std::min<int64_t>({tiles, wanted, (int64_t)kLogprobMostSplits}), 0, 0};
+  if (p.splits > 1) p.keys_at = 16 * rows * p.splits, p.bytes = p.keys_at + 8 * rows * p.splits * top;
+  return p;
+}
+
+template <typename T>
+int launch_logprobs(const LogprobArgs& a, hipStream_t s) {
+  const int rc = launch_operator("token logprobs", a.top ? k_logprobs<T, true> : k_logprobs<T, false>, dim3((unsigned)(a.rows * a.splits)),
+                                 kLogprobThreads, 0, s, a);
+  if (rc || a.splits == 1) return rc;
+  return launch_operator("token logprobs", k_logprobs_join<T>, dim3((unsigned)a.rows), kLogprobThreads, 0, s, a);
+}
+
 }  // namespace
 
 extern "C" int cq35_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t given, int32_t top, int64_t* bytes) {
   if (!bytes) return fail(CQ35_EINVAL, "token logprobs workspace: null argument");
   const int rc = check_logprob_sizes("token logprobs workspace", rows, vocab, given, top);
-  if (!rc) *bytes = 0;
+  if (!rc) *bytes = rows ? plan_logprobs(rows, vocab, top).bytes : 0;
   return rc;
 }
 
@@ -180,13 +202,16 @@ extern "C" int cq35_token_logprobs(const cq35_rows* logits, int64_t rows, int64_
   if (!row_type(logits->dtype)) return fail(CQ35_EUNSUPPORTED, "token logprobs: type %d is neither BF16 nor F32", logits->dtype);
   if ((uintptr_t)logits->data % (logits->dtype == CQ35_BF16 ? 2 : 4) || logits->row_stride < 0)
     return fail(CQ35_EINVAL, "token logprobs: logits misaligned, or rows %lld apart", (long long)logits->row_stride);
+  const LogprobPlan p = plan_logprobs(rows, vocab, top);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !aligned16(workspace)))
+    return fail(CQ35_EINVAL, "token logprobs: %lld bytes of workspace at a 16-byte address needed, %lld given", (long long)p.bytes,
+                (long long)(workspace ? workspace_bytes : 0));
   hipStream_t s = static_cast<hipStream_t>(stream);
   OperatorDevice on;
   rc = on.enter({logits->data, entropy, given ? tokens : nullptr, given ? logprobs : nullptr, top ? top_tokens : nullptr,
-                 top ? top_logprobs : nullptr}, s);
+                 top ? top_logprobs : nullptr, p.bytes ? workspace : nullptr}, s);
   if (rc) return rc;
   const LogprobArgs a{logits->data, logits->row_stride, rows, (int)vocab, tokens, (int)given, top, logprobs, entropy, top_tokens,
-                      top_logprobs};
-  return launch_operator("token logprobs", logits->dtype == CQ35_BF16 ? k_logprobs<uint16_t> : k_logprobs<float>,
-                         dim3((unsigned)rows), kLogprobThreads, 0, s, a);
+                      top_logprobs, p.splits, (float*)workspace, (uint64_t*)((char*)workspace + p.keys_at)};
+  return logits->dtype == CQ35_BF16 ? launch_logprobs<uint16_t>(a, s) : launch_logprobs<float>(a, s);
 }

@@ -3,6 +3,7 @@
 // gated product of a feed-forward (RowSource::kGated).
 #pragma once
 
+#include "lanes.h"
 #include "layers.h"
 
 namespace cq35 {
@@ -110,8 +111,7 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
     for (int p = 0; p < kPieces; ++p)
 #pragma unroll
       for (int e = 0; e < E; ++e) s = __builtin_fmaf(y[p][e], y[p][e], s);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+    s = lanes_sum(s);
     if (kWaves > 1) {
       if ((tid & 63) == 0) sums[wave] = s;
       __syncthreads();
@@ -138,8 +138,7 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
   for (int p = 0; p < kPieces; ++p)
 #pragma unroll
     for (int e = 0; e < E; ++e) m = max(m, fbits(y[p][e]) & 0x7fffffffu);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+  m = lanes_max(m);
   if (kWaves > 1) {
     if ((tid & 63) == 0) most[wave] = m;
     __syncthreads();
