@@ -53,12 +53,12 @@ __device__ __forceinline__ float widened(float x) { return x; }
 
 // Larger for larger logits (NaN above infinity, -0 as 0), among equal ones for lower indices;
 // never 0.
-__device__ __forceinline__ uint32_t logit_order(float x) {
+__device__ __forceinline__ uint32_t order_of_logit(float x) {
   const uint32_t b = fbits(x + 0.0f);
   return x != x ? 0xffffffffu : b >> 31 ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t logit_key(float x, int index) {
-  return (uint64_t)logit_order(x) << 32 | (0xffffffffu - (uint32_t)index);
+  return (uint64_t)order_of_logit(x) << 32 | (0xffffffffu - (uint32_t)index);
 }
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 __device__ __forceinline__ float key_logit(uint64_t key) {
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void k_logprobs(LogprobArgs a) 
         for (int e = 0; e < Tile::E; ++e) r.add(v.value(j, e) - from);
       if (!kTop) continue;
       if (threshold == 0 && tile == start) {
-        const uint32_t order = group_bound(l, logit_order(most), a.top);
+        const uint32_t order = group_bound(l, order_of_logit(most), a.top);
         above = below_order(order), limit = below_logit(order);
       }
       if (!(most <= limit) || r.s != r.s) {
