@@ -27,6 +27,13 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor  # float32 [rows, top]
 
 
+def _results(out, given, rows, top, device):
+    for name, t, shape, dtype in zip(TokenLogprobs._fields, out, (given, (rows,), (rows, top), (rows, top)), (_F32, _F32, _I64, _F32)):
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()):
+            _why("out." + name, t, dtype, len(shape), device)
+            raise ValueError(f"out.{name} must be contiguous {tuple(shape)}, not {tuple(t.shape)}")
+
+
 def token_logprobs(logits, tokens, *, top=0, out=None, workspace=None, stream=None) -> TokenLogprobs:
     """Log probabilities (cq35_token_logprobs) under each row of logits (BF16 or F32
     [rows, vocab], rows of any stride) of its tokens (int64 [rows] or [rows, given],
@@ -64,11 +71,8 @@ def token_logprobs(logits, tokens, *, top=0, out=None, workspace=None, stream=No
             parts = whole.split_with_sizes((2 * rows * top, rows * top, rows * given, rows))
             out = TokenLogprobs(parts[2].view(tokens.shape), parts[3], parts[0].view(_I64).view(rows, top),
                                 parts[1].view(rows, top))
-    shapes = (tokens.shape, (rows,), (rows, top), (rows, top))
-    for name, t, shape, dtype in zip(TokenLogprobs._fields, out, shapes, (_F32, _F32, _I64, _F32)):
-        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()):
-            _why("out." + name, t, dtype, len(shape), device)
-            raise ValueError(f"out.{name} must be contiguous {tuple(shape)}, not {tuple(t.shape)}")
+        else:
+            _results(out, tokens.shape, rows, top, device)
     check(_lib.load().cq35_token_logprobs(hl, rows, vocab, tokens.data_ptr(), given, top, out[0].data_ptr(), out[1].data_ptr(),
                                           out[2].data_ptr(), out[3].data_ptr(), at, have, raw))
     return TokenLogprobs(*out)

@@ -12,7 +12,7 @@ namespace {
 
 constexpr int64_t kMostRows = 1 << 21;  // times 1024 threads: a launch takes below 2^32
 constexpr int64_t kLogprobBlocks = 1024;  // four a CU; more rows take a block each
-constexpr int64_t kMostResults = 1ll << 34;  // in tiles of 64 x 64 by 256 threads as well
+constexpr int64_t kMostResults = 1ll << 34;  // in tiles of 16 x 16 by 512 threads as well
 
 bool row_type(int32_t dtype) { return dtype == CQ35_BF16 || dtype == CQ35_F32; }
 
@@ -63,6 +63,60 @@ RowArgs row_args(const cq35_rows* x, int64_t rows, int64_t channels, const cq35_
   a.a = x->data, a.a_stride = x->row_stride, a.rows = rows, a.channels = (int)channels;
   a.data = out->data, a.data_stride = out->row_stride, a.scale = out->scale;
   return a;
+}
+
+template <typename T, int BM, int BN>
+int launch_tiles(const ProductArgs& a, hipStream_t s) {
+  constexpr size_t lds = ProductTile<T, BM, BN>::kLds;
+  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)k_int8_tiles<T, BM, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  const int64_t blocks = ((a.rows + BM - 1) / BM) * ((a.outputs + BN - 1) / BN);
+  return launch_operator("int8 linear", k_int8_tiles<T, BM, BN>, dim3((unsigned)blocks), 256, lds, s, a);
+}
+
+template <typename T, int MT>
+int launch_few(const ProductArgs& a, hipStream_t s) {
+  return launch_operator("int8 linear", k_int8_few<T, MT>, dim3((unsigned)((a.outputs + 15) / 16)), 512, 0, s, a);
+}
+
+// The kernels and what a block of each takes, in ns: alone on its compute unit, and each further one there, by
+// the stages of 64 channels. Fitted to measured times; for 2048 channels to 9216 outputs (us, tiles of 64 x 64,
+// 128 x 128, 256 x 128, 256 x 256): 65 rows 10.5, 12.3, 18.4, 28.2; 300 rows 17.3, 13.9, 20.0, 30.7; 512 rows 25.7,
+// 21.6, 20.7, 31.1; 4096 rows 163, 105, 93, 103; 8192 rows to 12288 outputs -, 280, 251, 234. Up to 16 rows the
+// kernel of few rows takes 4.1 to 2048 outputs (64 x 64: 8.4) and 7.8 to 12288 (9.0), but 124 to 248320 (93).
+struct ProductKernel {
+  int rows, outputs;  // of a block
+  int most_rows;
+  int64_t start, stage, more_start, more_stage;
+};
+constexpr ProductKernel kProductKernels[] = {
+    {16, 16, 16, 3000, 40, 700, 39},          {32, 16, 32, 3300, 81, 1000, 62},      {64, 64, INT32_MAX, 3500, 154, 1200, 110},
+    {128, 128, INT32_MAX, 4900, 224, 1500, 310}, {256, 128, INT32_MAX, 6700, 360, 1800, 553}, {256, 256, INT32_MAX, 10400, 560, 11000, 867},
+};
+
+int product_kernel(int64_t rows, int64_t outputs, int64_t channels) {
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int i = 0; i < (int)(sizeof(kProductKernels) / sizeof(kProductKernels[0])); ++i) {
+    const ProductKernel& k = kProductKernels[i];
+    if (rows > k.most_rows) continue;
+    const int64_t blocks = ((rows + k.rows - 1) / k.rows) * ((outputs + k.outputs - 1) / k.outputs);
+    const int64_t stages = (channels + 63) / 64, more = (blocks + 255) / 256 - 1;
+    const int64_t time = k.start + stages * k.stage + more * (k.more_start + stages * k.more_stage);
+    if (time < least) best = i, least = time;
+  }
+  return best;
+}
+
+template <typename T>
+int launch_product(const ProductArgs& a, hipStream_t s) {
+  switch (product_kernel(a.rows, a.outputs, a.channels)) {
+    case 0: return launch_few<T, 1>(a, s);
+    case 1: return launch_few<T, 2>(a, s);
+    case 2: return launch_tiles<T, 64, 64>(a, s);
+    case 3: return launch_tiles<T, 128, 128>(a, s);
+    case 4: return launch_tiles<T, 256, 128>(a, s);
+    default: return launch_tiles<T, 256, 256>(a, s);
+  }
 }
 
 }  // namespace
@@ -146,8 +200,7 @@ extern "C" int cq35_int8_linear(const cq35_int8_rows* x, const cq35_int8_rows* w
   if (rc) return rc;
   const ProductArgs a{x->data, w->data, x->row_stride, w->row_stride, x->scale, w->scale, rows, outputs, (int)channels,
                       out->data, out->row_stride};
-  const dim3 grid((unsigned)(((outputs + 63) / 64) * ((rows + 63) / 64)));
-  return launch_operator("int8 linear", out->dtype == CQ35_BF16 ? k_int8_product<uint16_t> : k_int8_product<float>, grid, 256, 0, s, a);
+  return out->dtype == CQ35_BF16 ? launch_product<uint16_t>(a, s) : launch_product<float>(a, s);
 }
 
 namespace {
