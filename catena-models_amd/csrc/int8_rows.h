@@ -68,97 +68,124 @@ __device__ __forceinline__ uint32_t pack_int8(const float* v) {
   return lo | hi << 16;
 }
 
-// kLanes threads a row, kPieces pieces of 16 bytes a thread.
+// kLanes threads a row, kPieces pieces of 16 bytes a thread. Where a wave is a row it goes on to others, the next
+// one's pieces asked for under the current one's arithmetic and the norm's weights kept in registers.
 template <typename T, RowSource kSource, int kLanes, int kPieces>
 __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowArgs a) {
   typedef RowPiece<T> P;
-  constexpr int E = P::kValues, kThreads = kLanes < 256 ? 256 : kLanes, kWaves = kLanes / 64;
+  constexpr int E = P::kValues, kThreads = kLanes < 256 ? 256 : kLanes, kWaves = kLanes / 64, kRows = kThreads / kLanes;
   __shared__ float sums[kWaves];
   __shared__ uint32_t most[kWaves];
   const int tid = threadIdx.x, lane = tid % kLanes, wave = lane >> 6;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + tid / kLanes;
+  const bool two = kSource == RowSource::kGated || (kSource == RowSource::kNorm && a.b);
+  struct Row {
+    u32x4 a[kPieces], b[kSource == RowSource::kPlain ? 1 : kPieces];
+  } next;
+  auto load = [&](Row& r, int64_t row) {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int i = (p * kLanes + lane) * E;
+      if (i >= a.channels) continue;
+      r.a[p] = *reinterpret_cast<const u32x4*>((const T*)a.a + row * a.a_stride + i);
+      if (kSource != RowSource::kPlain && two) r.b[p] = *reinterpret_cast<const u32x4*>((const T*)a.b + row * a.b_stride + i);
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * kRows + tid / kLanes;
   if (row >= a.rows) return;  // whole waves; only where a wave is a row
-  const T *xa = (const T*)a.a + row * a.a_stride, *xb = (const T*)a.b + row * a.b_stride;
-  float y[kPieces][E];
-#pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
-    const int i = (p * kLanes + lane) * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[p][e] = 0.0f;
-    if (i >= a.channels) continue;
-    P::widen(*reinterpret_cast<const u32x4*>(xa + i), y[p]);
-    if (kSource == RowSource::kNorm && a.b) {
-      float r[E];
-      P::widen(*reinterpret_cast<const u32x4*>(xb + i), r);
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[p][e] += r[e];
-      // the sum in the stream's type is what the norm sees
-      const u32x4 raw = P::narrow(y[p]);
-      *reinterpret_cast<u32x4*>((T*)a.sum + row * a.sum_stride + i) = raw;
-      P::widen(raw, y[p]);
-    }
-    if (kSource == RowSource::kGated) {
-      float u[E];
-      P::widen(*reinterpret_cast<const u32x4*>(xb + i), u);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        y[p][e] = y[p][e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y[p][e] * -1.44269504f)) * u[e];
-    }
-  }
-  if (kSource == RowSource::kNorm) {
-    float s = 0.0f;
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p)
-#pragma unroll
-      for (int e = 0; e < E; ++e) s = __builtin_fmaf(y[p][e], y[p][e], s);
-    s = lanes_sum(s);
-    if (kWaves > 1) {
-      if ((tid & 63) == 0) sums[wave] = s;
-      __syncthreads();
-      s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) s += sums[w];
-    }
-    const float inverse = 1.0f / sqrtf(s / (float)a.channels + a.eps);
+  load(next, row);
+  float w[kSource == RowSource::kNorm ? kPieces : 1][E];
+  if (kSource == RowSource::kNorm)
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
       const int i = (p * kLanes + lane) * E;
       if (i >= a.channels) continue;
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
-        const float4 w = *reinterpret_cast<const float4*>(a.weight + i + e);
-        y[p][e] = y[p][e] * inverse * w.x, y[p][e + 1] = y[p][e + 1] * inverse * w.y;
-        y[p][e + 2] = y[p][e + 2] * inverse * w.z, y[p][e + 3] = y[p][e + 3] * inverse * w.w;
+        const float4 v = *reinterpret_cast<const float4*>(a.weight + i + e);
+        w[p][e] = v.x, w[p][e + 1] = v.y, w[p][e + 2] = v.z, w[p][e + 3] = v.w;
       }
     }
-  }
-  // magnitudes as integers: infinity and NaN are the largest
-  uint32_t m = 0;
+  for (;;) {
+    const Row now = next;
+    const int64_t after = row + (int64_t)gridDim.x * kRows;
+    if (kLanes == 64 && after < a.rows) load(next, after);
+    float y[kPieces][E];
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p)
+    for (int p = 0; p < kPieces; ++p) {
+      const int i = (p * kLanes + lane) * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = max(m, fbits(y[p][e]) & 0x7fffffffu);
-  m = lanes_max(m);
-  if (kWaves > 1) {
-    if ((tid & 63) == 0) most[wave] = m;
-    __syncthreads();
-    m = 0;
+      for (int e = 0; e < E; ++e) y[p][e] = 0.0f;
+      if (i >= a.channels) continue;
+      P::widen(now.a[p], y[p]);
+      if (kSource == RowSource::kNorm && two) {
+        float r[E];
+        P::widen(now.b[p], r);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = max(m, most[w]);
-  }
-  const float amax = bitsf(m);
-  const bool zeros = m >= 0x7f800000u || amax < kLeastAmax;
-  const float up = 127.0f / amax;
-  if (lane == 0) a.scale[row] = m >= 0x7f800000u ? bitsf(0x7fc00000u) : amax < kLeastAmax ? 0.0f : amax / 127.0f;
-  int8_t* to = a.data + row * a.data_stride;
+        for (int e = 0; e < E; ++e) y[p][e] += r[e];
+        // the sum in the stream's type is what the norm sees
+        const u32x4 raw = P::narrow(y[p]);
+        *reinterpret_cast<u32x4*>((T*)a.sum + row * a.sum_stride + i) = raw;
+        P::widen(raw, y[p]);
+      }
+      if (kSource == RowSource::kGated) {
+        float u[E];
+        P::widen(now.b[p], u);
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
-    const int i = (p * kLanes + lane) * E;
-    if (i >= a.channels) continue;
+        for (int e = 0; e < E; ++e)
+          y[p][e] = y[p][e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y[p][e] * -1.44269504f)) * u[e];
+      }
+    }
+    if (kSource == RowSource::kNorm) {
+      float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[p][e] = zeros ? 0.0f : y[p][e] * up;
-    if (E == 8) *reinterpret_cast<uint2*>(to + i) = make_uint2(pack_int8(y[p]), pack_int8(y[p] + E / 2));
-    else *reinterpret_cast<uint32_t*>(to + i) = pack_int8(y[p]);
+      for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = __builtin_fmaf(y[p][e], y[p][e], s);
+      s = lanes_sum(s);
+      if (kWaves > 1) {
+        if ((tid & 63) == 0) sums[wave] = s;
+        __syncthreads();
+        s = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) s += sums[v];
+      }
+      const float inverse = 1.0f / sqrtf(s / (float)a.channels + a.eps);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+        if ((p * kLanes + lane) * E < a.channels)
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[p][e] = y[p][e] * inverse * w[p][e];
+    }
+    // magnitudes as integers: infinity and NaN are the largest
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int e = 0; e < E; ++e) m = max(m, fbits(y[p][e]) & 0x7fffffffu);
+    m = lanes_max(m);
+    if (kWaves > 1) {
+      if ((tid & 63) == 0) most[wave] = m;
+      __syncthreads();
+      m = 0;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) m = max(m, most[v]);
+    }
+    const float amax = bitsf(m);
+    const bool zeros = m >= 0x7f800000u || amax < kLeastAmax;
+    const float up = 127.0f / amax;
+    if (lane == 0) a.scale[row] = m >= 0x7f800000u ? bitsf(0x7fc00000u) : zeros ? 0.0f : amax / 127.0f;
+    int8_t* to = a.data + row * a.data_stride;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int i = (p * kLanes + lane) * E;
+      if (i >= a.channels) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[p][e] = zeros ? 0.0f : y[p][e] * up;
+      if (E == 8) *reinterpret_cast<uint2*>(to + i) = make_uint2(pack_int8(y[p]), pack_int8(y[p] + E / 2));
+      else *reinterpret_cast<uint32_t*>(to + i) = pack_int8(y[p]);
+    }
+    if (kLanes != 64 || after >= a.rows) return;
+    row = after;
   }
 }
 

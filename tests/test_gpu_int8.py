@@ -86,6 +86,25 @@ def test_gated(rows, channels, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(8195, 64), (20001, 272), (9001, 2048)])
+def test_more_rows_than_waves(rows, channels, dtype):
+    """Waves that go on to other rows."""
+    say("many rows", rows, channels, dtype)
+    x, r = normal(1, rows, channels, dtype=dtype), normal(2, rows, channels, dtype=dtype)
+    w = 1 + 0.1 * normal(3, channels)
+    q = ops().quantize_rows(x)
+    ref.check_rows(q.data, q.scale, x.double(), 0.0)
+    h = (x.float() + r.float()).to(dtype)
+    q = ops().norm_quantize(x, w, residual=r, summed=r)
+    assert torch.equal(r, h)
+    ref.check_rows(q.data, q.scale, ref.norm(h, w, 1e-6), ref.NORM_REL)
+    q = ops().norm_quantize(x, w)
+    ref.check_rows(q.data, q.scale, ref.norm(x, w, 1e-6), ref.NORM_REL)
+    q = ops().gated_quantize(x, h)
+    ref.check_rows(q.data, q.scale, ref.gated(x, h), ref.gated_rel(x))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("channels", [48, 2048, 6144, 16384])
 def test_rows_of_extremes(dtype, channels):
     """Zeros, magnitudes at the ends of the range, single values, values that are not finite."""
