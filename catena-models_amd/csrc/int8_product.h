@@ -86,8 +86,10 @@ __global__ __launch_bounds__(256, BM * BN > 256 * 128 ? 1 : 2) void k_int8_tiles
                                    : a.w + min(n0 + (q - BM / 16) * 16 + from_row, a.outputs - 1) * a.w_stride);
   }
   float* scales = reinterpret_cast<float*>(product_lds + P::kScales);
-  for (int n = threadIdx.x; n < BN; n += 256) scales[n] = a.sw[min(n0 + n, a.outputs - 1)];
-  for (int m = threadIdx.x; m < BM; m += 256) scales[BN + m] = a.sx[min(m0 + m, a.rows - 1)];
+  // the thread's share of the scales, under way with the first stages
+  float sw = 0.0f, sx = 0.0f;
+  if (threadIdx.x < BN) sw = a.sw[min(n0 + threadIdx.x, a.outputs - 1)];
+  if (threadIdx.x < BM) sx = a.sx[min(m0 + threadIdx.x, a.rows - 1)];
   const int stages = (a.channels + 63) / 64;
   // Zeros behind the last channel, and for stages behind the last: the loop has one body and no other way
   // through it, as the compiler would copy the sums where ways meet.
@@ -154,6 +156,8 @@ __global__ __launch_bounds__(256, BM * BN > 256 * 128 ? 1 : 2) void k_int8_tiles
              [&](int u) { request(i + P::kStages, u); });
   }
   arrived_but<0>();
+  if (threadIdx.x < BN) scales[threadIdx.x] = sw;
+  if (threadIdx.x < BM) scales[BN + threadIdx.x] = sx;
   __syncthreads();
   // Results by rows: 32 rows of the wave's part at a time through LDS, so that a store is of whole lines.
   uint8_t* slab = product_lds + wave * 32 * P::kSlabRow;
@@ -164,15 +168,15 @@ __global__ __launch_bounds__(256, BM * BN > 256 * 128 ? 1 : 2) void k_int8_tiles
   const T* in = reinterpret_cast<const T*>(slab + lr * P::kSlabRow) + at;
 #pragma unroll
   for (int t = 0; t < P::TM; ++t) {
-    const float sx = scales[BN + wm + 32 * t + c];
+    const float row = scales[BN + wm + 32 * t + c];
 #pragma unroll
     for (int n = 0; n < P::TN; ++n)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 sw = *reinterpret_cast<const float4*>(scales + wn + 32 * n + 8 * g + 4 * h);
+        const float4 s = *reinterpret_cast<const float4*>(scales + wn + 32 * n + 8 * g + 4 * h);
         const i32x16& v = acc[t][n];
-        store_four((float)v[4 * g] * sx * sw.x, (float)v[4 * g + 1] * sx * sw.y, (float)v[4 * g + 2] * sx * sw.z,
-                   (float)v[4 * g + 3] * sx * sw.w, reinterpret_cast<T*>(slab + c * P::kSlabRow) + 32 * n + 8 * g + 4 * h);
+        store_four((float)v[4 * g] * row * s.x, (float)v[4 * g + 1] * row * s.y, (float)v[4 * g + 2] * row * s.z,
+                   (float)v[4 * g + 3] * row * s.w, reinterpret_cast<T*>(slab + c * P::kSlabRow) + 32 * n + 8 * g + 4 * h);
       }
     __builtin_amdgcn_wave_barrier();
     if (whole) {

@@ -205,6 +205,19 @@ def test_linear(rows, channels, outputs, dtype):
     assert torch.equal(got, ref.linear(x, w, dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels,outputs,front", [(2300, 2064, 12300, 0), (2049, 4112, 6200, 8), (1030, 6160, 12501, 0), (700, 1040, 9000, 0),
+                                                         (700, 1040, 9003, 3), (520, 16, 20000, 16), (300, 80, 20001, 1), (40, 2048, 30000, 0)])
+def test_linear_many_tiles(rows, channels, outputs, front, dtype):
+    """More tiles than compute units, of every size: ragged at their ends, in rows of whole lines and not."""
+    say("many tiles", rows, channels, outputs, front, dtype)
+    x, w = ints(1, rows, channels), ints(2, outputs, channels)
+    whole = torch.full((rows, outputs + 2 * front), 77, dtype=dtype, device="cuda")
+    got = ops().int8_linear(x, w, out=whole[:, front:front + outputs])
+    assert torch.equal(got, ref.linear(x, w, dtype))
+    assert bool((whole[:, :front] == 77).all()) and bool((whole[:, front + outputs:] == 77).all())
+
+
 @pytest.mark.parametrize("rows,outputs", [(1, 7), (40, 70), (300, 520)])
 def test_linear_sums_at_their_largest(rows, outputs):
     """-128 times -128 over every channel."""

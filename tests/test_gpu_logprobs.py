@@ -221,6 +221,40 @@ def test_captured_and_on_another_stream(rows, vocab):
     assert all(torch.equal(a, b) for a, b in zip(other, want))
 
 
+def test_two_graphs_that_share_a_workspace():
+    """Replayed one after the other, in any order."""
+    say("shared workspace")
+    o = ops()
+    cases = [(2, 100000, 7), (1, 248320, 32)]
+    work = torch.empty(max(o.token_logprobs_workspace(r, v, 1, k) for r, v, k in cases), dtype=torch.uint8, device="cuda")
+    held = []
+    side = torch.cuda.Stream()
+    for rows, vocab, top in cases:
+        x, t = logits(rows, rows, vocab, BF), tokens(2, rows, 1, vocab)
+        n = o.token_logprobs_workspace(rows, vocab, 1, top)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                got = o.token_logprobs(x, t, top=top, workspace=work[:n])
+        torch.cuda.current_stream().wait_stream(side)
+        held.append((graph, got, x, t, top))
+    for i in (0, 1, 1, 0, 1, 0, 0):
+        graph, got, x, t, top = held[i]
+        x.copy_(logits(30 + i, *x.shape, BF))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, o.token_logprobs(x, t, top=top)))
+
+
+@pytest.mark.parametrize("given", [300, 1024])
+def test_many_given_tokens(given):
+    say("given", given)
+    for rows, vocab in ((2, 70000), (600, 900)):
+        x, t = logits(1, rows, vocab, F32), tokens(2, rows, given, vocab)
+        check(x, t, 2, ops().token_logprobs(x, t, top=2))
+
+
 def test_empty_and_refused():
     say("empty and refused")
     o = ops()
