@@ -2,6 +2,14 @@
 // exact in 32-bit integers (channels <= 2^16, so they stay below 2^30), the two
 // products and the rounding of the sum to F32 one rounding each, the result rounded once
 // more where it is BF16.
+//
+// Few rows are bound by the weights' bytes and by latency: one row of 2048 channels to 12288 outputs 7.8 us (3.2
+// TB/s), to 2048 outputs 4.1. Large products are bound by the card's power: 8192 rows of 8192 channels to 8192
+// outputs 490 us, 2.2 POP/s, the matrix cores busy 0.61 of the cycles at 1.65 to 1.8 GHz; with nothing fetched the
+// same loop keeps them busy 0.76 at 2.2 GHz. Those of fewer channels add a tile's start and end, 10 us of
+// 256 x 256 results: 8192 rows of 2048 to 12288 outputs 245 us, 1.68 POP/s. In between LDS is the bound: the
+// waves' reads and the requests' writes share its port, 64 channels of a 128 x 128 tile take about 550
+// cycles there and 256 on the matrix cores.
 #pragma once
 
 #include "layers.h"
@@ -37,9 +45,17 @@ __device__ __forceinline__ void store_four(float a, float b, float c, float d, f
 
 // Block = BM rows x BN outputs, four waves of half by half. Channels go through LDS 64 a stage by
 // DMA, kStages stages, one barrier a stage; a stage holds BM + BN rows of 64 bytes whose
-// 16-byte pieces are swapped so that eight neighbouring rows' same piece lie in different banks.
-// Weights are the first operand of the matrix instruction, so that a lane's results are four
-// neighbouring outputs of one row.
+// 16-byte pieces are swapped so that sixteen neighbouring rows' same piece lie in different ones of the 64
+// banks (swapped by the next lower bit of the row half of the reads' cycles were conflicts). Weights are the
+// first operand of the matrix instruction, so that a lane's results are four neighbouring outputs of one row.
+//
+// Measured and not kept (8192 rows of 2048 channels to 12288 outputs unless said otherwise): products of 16 x 16
+// with whole stages in registers, spilled at 256 x 256 (397 us) and 10 % faster at 64 x 64; requests all behind the
+// barrier instead of spread (259 against 248); two groups of waves with half the channels each, joined in LDS (300
+// rows to 9216 17.1 us against 14.6); rings of 8 or 16 stages (no change); a block that goes on to further tiles,
+// their first stages requested under the stores (250 to 274 against 245: the compiler copies the sums); stores past
+// the caches (238 against 232); tiles of 64 x 128
+// (4096 rows: 182 us against 138 of 128 x 128).
 template <typename T, int BM, int BN>
 struct ProductTile {
   static constexpr int kStage = (BM + BN) * 64, kStages = BM * BN == 256 * 128 ? 3 : 4;  // two blocks of 256 x 128 a CU

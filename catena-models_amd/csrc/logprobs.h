@@ -20,16 +20,22 @@ namespace cq35 {
 // are found changes nothing. A block keeps candidates in LDS and a threshold, the
 // top-th best key so far, for the next kEpoch tiles; a thread looks at its logits of a
 // tile one by one only if the largest passes it. Without a threshold yet one is taken
-// from the largest logits of the threads: the least maximum of 4 to 32 groups of
-// threads, at least `top` of them, which as many logits reach. Where more candidates
-// pass than the list holds (rows that ascend, or of equal logits), the tiles are looked
-// at again one by one over the top-th of the 256 threads' largest keys: at most 32
-// logits of each of top threads reach it.
+// from the threads' largest logits (group_bound). Where more candidates pass than the
+// list holds (rows that ascend, or of equal logits), the tiles are looked at again one by
+// one over the top-th of the 256 threads' largest keys: at most 32 logits of each of top
+// threads reach it.
+//
+// Bound by the logits' bytes where there are many rows: 1000 rows of 248320 BF16 logits with one
+// alternative 101 us (4.9 TB/s), with 20 139; 64 rows of F32 with 20 19.7, without any 12.2. One row is
+// latency: 6.5 us in 31 blocks, then 4 us for the join. A barrier a tile instead of one in four: 205 us
+// for the 1000 rows; a thread's logits kept in registers for the candidates instead of read again: 168
+// registers instead of 127, half the waves; tiles of 32 F32 logits a thread instead of 16: spilled, 31 us
+// for the 64 rows; 512 or 2048 blocks wanted instead of 1024: 75 and 56 us for 300 rows, 53.
 constexpr int kLogprobsMostTop = 32;
 constexpr int kLogprobsMostGiven = 1024;
 constexpr int kLogprobThreads = 256;
 constexpr int kLogprobPieces = 4;                                 // of 16 bytes, a thread's share of a tile
-constexpr int kCandidates = 2048;                                 // of the list, half of them kept from tile to tile
+constexpr int kCandidates = 2048;                                 // of the list
 constexpr int kLogprobMostSplits = kCandidates / kLogprobsMostTop;  // of a row, so that the join's list holds them
 constexpr int kEpoch = 4;                                         // tiles between two looks at the list
 constexpr int kLogprobPrune = 128;                                // candidates that are cut down to the best

@@ -91,6 +91,22 @@ pub struct cq35_heads {
     pub head_stride: i64,
 }
 
+/// Rows of BF16 or F32 values in device memory (cq35_rows).
+#[repr(C)]
+pub struct cq35_rows {
+    pub data: *mut c_void,
+    pub row_stride: i64,
+    pub dtype: i32,
+}
+
+/// Rows of 8-bit integers with a scale each in device memory (cq35_int8_rows).
+#[repr(C)]
+pub struct cq35_int8_rows {
+    pub data: *mut i8,
+    pub row_stride: i64,
+    pub scale: *mut f32,
+}
+
 extern "C" {
     pub fn cq35_last_error() -> *const c_char;
     pub fn cq35_abi_version() -> c_int;
@@ -139,6 +155,19 @@ extern "C" {
                                 requests: i64, width: i64, row_start: *const i32, lengths: *const i32, scale: f32,
                                 max_rows: i64, max_keys: i64, workspace: *mut c_void, workspace_bytes: i64,
                                 stream: *mut c_void) -> c_int;
+    pub fn cq35_quantize_rows(x: *const cq35_rows, rows: i64, channels: i64, out: *const cq35_int8_rows,
+                              stream: *mut c_void) -> c_int;
+    pub fn cq35_norm_quantize(x: *const cq35_rows, residual: *const cq35_rows, weight: *const f32, eps: f32, rows: i64,
+                              channels: i64, summed: *const cq35_rows, out: *const cq35_int8_rows,
+                              stream: *mut c_void) -> c_int;
+    pub fn cq35_gated_quantize(gate: *const cq35_rows, up: *const cq35_rows, rows: i64, channels: i64,
+                               out: *const cq35_int8_rows, stream: *mut c_void) -> c_int;
+    pub fn cq35_int8_linear(x: *const cq35_int8_rows, w: *const cq35_int8_rows, rows: i64, outputs: i64, channels: i64,
+                            out: *const cq35_rows, stream: *mut c_void) -> c_int;
+    pub fn cq35_token_logprobs_workspace(rows: i64, vocab: i64, given: i64, top: i32, bytes: *mut i64) -> c_int;
+    pub fn cq35_token_logprobs(logits: *const cq35_rows, rows: i64, vocab: i64, tokens: *const i64, given: i64, top: i32,
+                               logprobs: *mut f32, entropy: *mut f32, top_tokens: *mut i64, top_logprobs: *mut f32,
+                               workspace: *mut c_void, workspace_bytes: i64, stream: *mut c_void) -> c_int;
 }
 
 /// `Ok(())` for CQ35_OK, else the code with the library's message for this thread.

@@ -516,7 +516,7 @@ int cq35_gated_quantize(const cq35_rows* gate, const cq35_rows* up, int64_t rows
  * `outputs` rows of w: the sum exact, rounded to F32, each product rounded to F32, the
  * result to out's type. All values of an 8-bit integer are taken, -128 too. Rows
  * of out may lie anywhere that its elements may (no 16-byte rule), row_stride at least
- * `outputs`. Up to 2^21 rows and outputs, 2^34 results. */
+ * `outputs`; they overlap no input. Up to 2^21 rows and outputs, 2^34 results. */
 int cq35_int8_linear(const cq35_int8_rows* x, const cq35_int8_rows* w, int64_t rows, int64_t outputs,
                      int64_t channels, const cq35_rows* out, void* stream);
 
