@@ -103,6 +103,31 @@ def test_rows_of_all_shapes(vocab, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [1, 20])
+def test_rows_of_all_shapes_in_one_block_each(top, dtype):
+    """So many rows that none is cut: a block goes over many tiles, with the front of some masked for a while."""
+    say("one block", top, dtype)
+    vocab, rows = 70001, 620
+    x = [shaped(k, vocab, dtype) for k in KINDS]
+    ordinary = logits(5, 12, vocab, dtype)
+    for i, front in enumerate((30, 4096, 4097, 8192, 8200, 16384, 16500, 33000, 40960, 65600, vocab - 21, vocab - 3)):
+        ordinary[i, :front] = (-INF, torch.finfo(dtype).min, 0.0)[i % 3]
+    x = torch.cat([torch.stack(x), ordinary])
+    n = len(x)
+    t = tokens(4, n, 2, vocab)
+    again = torch.arange(rows, device="cuda") % n
+    got = ops().token_logprobs(x[again], t[again], top=top)
+    for at in (0, n):
+        check(x, t, top, type(got)(*(a[at:at + n] for a in got)))
+    assert torch.equal(got.top_tokens, got.top_tokens[:n][again])
+    # the order of a row's sums follows from its place within 16 bytes, the same every 8 rows (2 n is a multiple)
+    assert 2 * n % 8 == 0
+    again = torch.arange(rows, device="cuda") % (2 * n)
+    for a in got:
+        assert torch.equal(a.view(torch.uint8), a[:2 * n].contiguous()[again].view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("vocab", [40, 9001, 100003])
 def test_not_finite(vocab, dtype):
     """NaN and infinity make a row's numbers NaN, wherever they lie; its order stays."""
