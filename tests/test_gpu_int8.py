@@ -362,6 +362,26 @@ def test_captured(rows):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_products(dtype):
+    """Tiles of every size in one graph, LDS of more than 64 KB among them, without a call in front of it."""
+    sizes = [(5, 512, 700), (24, 512, 700), (70, 256, 300), (300, 2048, 9216), (1030, 2064, 6300), (2300, 2064, 12300)]
+    say("captured products", dtype)
+    made = [(ints(r, r, c), ints(o, o, c)) for r, c, o in sizes]
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            got = [ops().int8_linear(x, w, dtype=dtype) for x, w in made]
+    for i in range(3):
+        for (x, _), _ in made:
+            x.copy_(x.flip(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, (x, w) in zip(got, made):
+            assert torch.equal(g, ref.linear(x, w, dtype)), (i, g.shape)
+
+
 @pytest.mark.parametrize("rows", [1, 33])
 def test_layer_near_the_exact_products(rows):
     """The layer in 8 bits against its definition in 64 bits: each operator's output follows from
