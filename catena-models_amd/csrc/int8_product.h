@@ -55,7 +55,9 @@ __device__ __forceinline__ void store_four(float a, float b, float c, float d, f
 // rows to 9216 17.1 us against 14.6); rings of 8 or 16 stages (no change); a block that goes on to further tiles,
 // their first stages requested under the stores (250 to 274 against 245: the compiler copies the sums); stores past
 // the caches (238 against 232); tiles of 64 x 128
-// (4096 rows: 182 us against 138 of 128 x 128).
+// (4096 rows: 182 us against 138 of 128 x 128); the waves side by side along the outputs, 32 each, whose weights go
+// from memory straight to registers eight stages ahead and only rows through LDS (300 rows to 9216 17.6 against 15.2,
+// 8192 rows 337 to 364: 16 bytes from each of 32 rows are 64 requests to the caches, four times those of 1 KB by DMA).
 template <typename T, int BM, int BN>
 struct ProductTile {
   static constexpr int kStage = (BM + BN) * 64, kStages = BM * BN == 256 * 128 ? 3 : 4;  // two blocks of 256 x 128 a CU
