@@ -78,22 +78,27 @@ int launch_tiles(const ProductArgs& a, hipStream_t s) {
 
 template <typename T, int MT>
 int launch_few(const ProductArgs& a, hipStream_t s) {
-  return launch_operator("int8 linear", k_int8_few<T, MT>, dim3((unsigned)((a.outputs + 15) / 16)), 512, 0, s, a);
+  const unsigned blocks = (unsigned)((a.outputs + 15) / 16);
+  // more than two blocks a compute unit: the kernel of which four fit
+  const bool many = MT > 1 || blocks > 512;
+  return launch_operator("int8 linear", many ? k_int8_few<T, MT, 2> : k_int8_few<T, MT, (MT > 1 ? 2 : 4)>, dim3(blocks), 512, 0, s, a);
 }
 
 // The kernels and what a block of each takes, in ns: alone on its compute unit, and each further one there, by
 // the stages of 64 channels. Fitted to measured times; for 2048 channels to 9216 outputs (us, tiles of 64 x 64,
 // 128 x 128, 256 x 128, 256 x 256): 65 rows 10.5, 12.3, 18.4, 28.2; 300 rows 17.3, 13.9, 20.0, 30.7; 512 rows 25.7,
 // 21.6, 20.7, 31.1; 4096 rows 163, 105, 93, 103; 8192 rows to 12288 outputs -, 280, 251, 234. Up to 16 rows the
-// kernel of few rows takes 4.1 to 2048 outputs (64 x 64: 8.4) and 7.8 to 12288 (9.0), but 124 to 248320 (93).
+// kernel of few rows takes 4.1 to 4.8 to 2048 outputs (64 x 64: 7.8); one row 6.9 to 12288 (8.1) and 83 to 248320 (90),
+// but sixteen 8.6 (8.2) and 140 (111).
 struct ProductKernel {
   int rows, outputs;  // of a block
   int most_rows;
   int64_t start, stage, more_start, more_stage;
+  int64_t more_row;  // of each row, by the stage
 };
 constexpr ProductKernel kProductKernels[] = {
-    {16, 16, 16, 3000, 40, 700, 39},          {32, 16, 32, 3300, 81, 1000, 62},      {64, 64, INT32_MAX, 3500, 154, 1200, 110},
-    {128, 128, INT32_MAX, 4900, 224, 1500, 310}, {256, 128, INT32_MAX, 6700, 360, 1800, 553}, {256, 256, INT32_MAX, 10400, 560, 11000, 867},
+    {16, 16, 16, 3000, 40, 500, 18, 2},             {32, 16, 32, 3300, 81, 1000, 62, 0},            {64, 64, INT32_MAX, 3500, 154, 1200, 110, 0},
+    {128, 128, INT32_MAX, 4900, 224, 1500, 310, 0}, {256, 128, INT32_MAX, 6700, 360, 1800, 553, 0}, {256, 256, INT32_MAX, 10400, 560, 11000, 867, 0},
 };
 
 int product_kernel(int64_t rows, int64_t outputs, int64_t channels) {
@@ -104,7 +109,7 @@ int product_kernel(int64_t rows, int64_t outputs, int64_t channels) {
     if (rows > k.most_rows) continue;
     const int64_t blocks = ((rows + k.rows - 1) / k.rows) * ((outputs + k.outputs - 1) / k.outputs);
     const int64_t stages = (channels + 63) / 64, more = (blocks + 255) / 256 - 1;
-    const int64_t time = k.start + stages * k.stage + more * (k.more_start + stages * k.more_stage);
+    const int64_t time = k.start + stages * k.stage + more * (k.more_start + stages * (k.more_stage + rows * k.more_row));
     if (time < least) best = i, least = time;
   }
   return best;

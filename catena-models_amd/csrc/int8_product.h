@@ -3,7 +3,7 @@
 // products and the rounding of the sum to F32 one rounding each, the result rounded once
 // more where it is BF16.
 //
-// Few rows are bound by the weights' bytes and by latency: one row of 2048 channels to 12288 outputs 7.8 us (3.2
+// Few rows are bound by the weights' bytes and by latency: one row of 2048 channels to 12288 outputs 6.9 us (3.6
 // TB/s), to 2048 outputs 4.1. Large products are bound by the card's power: 8192 rows of 8192 channels to 8192
 // outputs 490 us, 2.2 POP/s, the matrix cores busy 0.61 of the cycles at 1.65 to 1.8 GHz; with nothing fetched the
 // same loop keeps them busy 0.76 at 2.2 GHz. Those of fewer channels add a tile's start and end, 10 us of
@@ -219,9 +219,12 @@ __global__ __launch_bounds__(256, BM * BN > 256 * 128 ? 1 : 2) void k_int8_tiles
 // Few rows: the weights' bytes are the time, so they go from memory straight to registers. Block = 16 MT
 // rows x 16 outputs, the channels dealt to its eight waves 128 at a time (a line of memory); a wave keeps
 // kAhead runs of 128 under way. The waves' sums meet in LDS by integer additions, whose order changes nothing.
-template <typename T, int MT>
+// Two runs leave room for four blocks on a compute unit instead of two, four are longer under way where there are
+// fewer blocks: one row of 2048 channels to 12288 outputs 6.9 us with two, 7.8 with four, of 6144 channels to 2048
+// outputs 6.5 and 6.3, of 4096 to 4096 6.65 and 6.25. Blocks of four waves: 7.0, 7.6, 7.1 at best.
+template <typename T, int MT, int kAhead>
 __global__ __launch_bounds__(512) void k_int8_few(ProductArgs a) {
-  constexpr int kWaves = 8, kAhead = MT > 1 ? 3 : 4, kRow = 20;
+  constexpr int kWaves = 8, kRow = 20;
   __shared__ int32_t sums[16 * MT * kRow];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, h = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;

@@ -218,6 +218,17 @@ def test_linear_many_tiles(rows, channels, outputs, front, dtype):
     assert bool((whole[:, :front] == 77).all()) and bool((whole[:, front + outputs:] == 77).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels,outputs", [(1, 16, 8193), (1, 2048, 12300), (2, 1040, 33000), (7, 4112, 9217), (3, 144, 50001), (16, 304, 8200)])
+def test_linear_few_rows_many_outputs(rows, channels, outputs, dtype):
+    say("few rows, many outputs", rows, channels, outputs, dtype)
+    x, w = ints(1, rows, channels), ints(2, outputs, channels)
+    whole = torch.full((rows, outputs + 5), 77, dtype=dtype, device="cuda")
+    got = ops().int8_linear(x, w, out=whole[:, :outputs])
+    assert torch.equal(got, ref.linear(x, w, dtype))
+    assert bool((whole[:, outputs:] == 77).all())
+
+
 @pytest.mark.parametrize("rows,outputs", [(1, 7), (40, 70), (300, 520)])
 def test_linear_sums_at_their_largest(rows, outputs):
     """-128 times -128 over every channel."""
