@@ -224,8 +224,9 @@ __global__ __launch_bounds__(256, BM * BN > 256 * 128 ? 1 : 2) void k_int8_tiles
 // outputs 6.5 and 6.3, of 4096 to 4096 6.65 and 6.25. Blocks of four waves: 7.0, 7.6, 7.1 at best.
 template <typename T, int MT, int kAhead>
 __global__ __launch_bounds__(512) void k_int8_few(ProductArgs a) {
-  constexpr int kWaves = 8, kRow = 20;
-  __shared__ int32_t sums[16 * MT * kRow];
+  constexpr int kWaves = 8, kFourth = 64 * MT + 16;
+  // [e][row][h] of output 4 h + e, so that a wave's 64 sums lie in different banks
+  __shared__ int32_t sums[4 * kFourth];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, h = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int8_t* x[MT];
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(512) void k_int8_few(ProductArgs a) {
   i32x4 acc[MT] = {};
 #pragma unroll
   for (int d = 0; d < kAhead; ++d) load(run[d], 128 * (wave + kWaves * d));
-  for (int i = threadIdx.x; i < 16 * MT * kRow; i += 512) sums[i] = 0;
+  for (int i = threadIdx.x; i < 4 * kFourth; i += 512) sums[i] = 0;
   for (int k = 128 * wave; k < a.channels; k += 128 * kWaves * kAhead) {
 #pragma unroll
     for (int d = 0; d < kAhead; ++d) {
@@ -263,11 +264,12 @@ __global__ __launch_bounds__(512) void k_int8_few(ProductArgs a) {
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) atomicAdd(&sums[(16 * m + c) * kRow + 4 * h + e], acc[m][e]);
+    for (int e = 0; e < 4; ++e) atomicAdd(&sums[e * kFourth + 4 * (16 * m + c) + h], acc[m][e]);
   __syncthreads();
   for (int i = threadIdx.x; i < 256 * MT; i += 512) {
     const int64_t m = i / 16, n = n0 + i % 16;
-    if (m < a.rows && n < a.outputs) store_one((float)sums[m * kRow + i % 16] * a.sx[m] * a.sw[n], (T*)a.out + m * a.out_stride + n);
+    const int32_t sum = sums[i % 4 * kFourth + 4 * m + i % 16 / 4];
+    if (m < a.rows && n < a.outputs) store_one((float)sum * a.sx[m] * a.sw[n], (T*)a.out + m * a.out_stride + n);
   }
 }
 
