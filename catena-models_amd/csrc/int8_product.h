@@ -221,7 +221,8 @@ __global__ __launch_bounds__(256, BM * BN > 256 * 128 ? 1 : 2) void k_int8_tiles
 // kAhead runs of 128 under way. The waves' sums meet in LDS by integer additions, whose order changes nothing.
 // Two runs leave room for four blocks on a compute unit instead of two, four are longer under way where there are
 // fewer blocks: one row of 2048 channels to 12288 outputs 6.9 us with two, 7.8 with four, of 6144 channels to 2048
-// outputs 6.5 and 6.3, of 4096 to 4096 6.65 and 6.25. Blocks of four waves: 7.0, 7.6, 7.1 at best.
+// outputs 6.5 and 6.3, of 4096 to 4096 6.65 and 6.25. Blocks of four waves: 7.0, 7.6, 7.1 at best; of sixteen as of
+// eight (16384 channels to 1024 outputs 11.5 both: a compute unit takes in its 16 rows of weights no faster).
 template <typename T, int MT, int kAhead>
 __global__ __launch_bounds__(512) void k_int8_few(ProductArgs a) {
   constexpr int kWaves = 8, kFourth = 64 * MT + 16;
