@@ -22,18 +22,19 @@ namespace cq35 {
 // tile one by one only if the largest passes it. Without a threshold yet one is taken
 // from the threads' largest logits (group_bound). Where more candidates pass than the
 // list holds (rows that ascend), the tiles are looked at again one by
-// one over the top-th of the 256 threads' largest keys: at most 32 logits of each of top
-// threads reach it. So is a tile alone whose bound many groups' largest logits equal (a mask's
+// one, where many threads have any over the top-th of the 256 threads' largest keys: at most 32 logits of each of
+// top threads reach it. So is a tile alone whose bound many groups' largest logits equal (a mask's
 // lowest value, rows of equal logits): its keys' threshold serves the rest.
-// 64 rows of F32 with 20, 99.9 of 100 logits masked, 34 us in all instead of 24, and 90 with each
+// 64 rows of F32 with 20, 99.9 of 100 logits masked, 34 us in all instead of 23, and 90 with each
 // such tile's equal logits as candidates; whole keys instead of orders in group_bound 28, but then 27.5 for rows
 // without a mask.
 //
 // Bound by the logits' bytes where there are many rows: 1000 rows of 248320 BF16 logits with one
-// alternative 101 us (4.9 TB/s), with 20 139; 64 rows of F32 with 20 19.7, without any 12.2. One row is
-// latency: 6.5 us in 31 blocks, then 4 us for the join. A barrier a tile instead of one in four: 205 us
-// for the 1000 rows; a thread's logits kept in registers for the candidates instead of read again: 168
-// registers instead of 127, half the waves; tiles of 32 F32 logits a thread instead of 16: spilled, 31 us
+// alternative 99 us (5.0 TB/s), with 20 112; 64 rows of F32 with 20 19, without any 12.2. One row is
+// latency: 6.7 us in 31 blocks, then 4 us for the join. A barrier a tile: 205 us for the 1000 rows, one in two 8 %
+// and one in four 2 % more than one in eight, one in sixteen as much as in eight. A candidate's logit read again where
+// it is found, and not all of them at once in front of best_keys: 102 us; a thread's logits kept in registers for
+// them: 168 registers instead of 127, half the waves; tiles of 32 F32 logits a thread instead of 16: spilled, 31 us
 // for the 64 rows; 512 or 2048 blocks wanted instead of 1024: 75 and 56 us for 300 rows, 53.
 constexpr int kLogprobsMostTop = 32;
 constexpr int kLogprobsMostGiven = 1024;
@@ -41,7 +42,7 @@ constexpr int kLogprobThreads = 256;
 constexpr int kLogprobPieces = 4;                                 // of 16 bytes, a thread's share of a tile
 constexpr int kCandidates = 2048;                                 // of the list
 constexpr int kLogprobMostSplits = kCandidates / kLogprobsMostTop;  // of a row, so that the join's list holds them
-constexpr int kEpoch = 4;                                         // tiles between two looks at the list
+constexpr int kEpoch = 8;                                         // tiles between two looks at the list
 constexpr int kMoreGroups = 8;                                    // that may pass a bound beside those needed
 constexpr int kLogprobPrune = 128;                                // candidates that are cut down to the best
 
@@ -289,9 +290,9 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void k_logprobs(LogprobArgs a) 
   if (a.splits == 1) given.load(a, row);
   RowStats r;
   r.clear();
-  uint64_t threshold = 0, above = 0;  // the top-th best key so far; keys above `above` are candidates
-  float limit = 0.0f;                 // their logits are not at or below it
-  int n = 0, turn = 0;                // candidates, and which count is in use
+  uint64_t threshold = 0;         // the top-th best key so far
+  float limit = 0.0f;             // logits not at or below it are candidates
+  int n = 0, keys = 0, turn = 0;  // in the list; of them keys, the others still places; which count is in use
   auto put = [&](uint64_t key) {
     const int at = n + atomicAdd(&l.count[turn], 1);
     if (at < kCandidates) l.list[at] = key;
@@ -328,12 +329,12 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void k_logprobs(LogprobArgs a) 
       if (threshold == 0 && tile == start) {
         int passed;
         const uint32_t order = group_bound(l, order_of_logit(most), a.top, (end - tile * Tile::kLogits + 4 * Tile::E - 1) / (4 * Tile::E), passed);
-        above = below_order(order), limit = below_logit(order);
+        limit = below_logit(order);
         // of equal logits far more would pass than are wanted: none is taken, and the tile is looked at again at once
         if (passed > a.top + kMoreGroups) limit = __builtin_inff(), stop = tile + 1;
       }
       if (!(most <= limit) || r.s != r.s) {
-        // which of the logits pass; each is read again, as few do
+        // which of the logits pass: their places, as few do and a wait for one read again would be the tile's
         uint32_t pass = 0;
 #pragma unroll
         for (int j = Tile::kPieces - 1; j >= 0; --j) {
@@ -346,47 +347,55 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void k_logprobs(LogprobArgs a) 
         }
         for (; pass; pass &= pass - 1) {
           const int at = __builtin_ctz(pass), i = Tile::first(tile, at / Tile::E) + at % Tile::E;
-          if (i < before || i >= end) continue;
-          const uint64_t key = logit_key(widened(base[i]), i - before);
-          if (key > above) put(key);
+          if (i >= before && i < end) put(i);
         }
       }
     }
     if (!kTop) continue;
     if (tid == 0 && limit == __builtin_inff()) l.count[turn] = kCandidates + 1;
     const int c = added();
-    if (n + c > kCandidates) {
+    const bool many = n + c > kCandidates;
+    if (!many) n += c;
+    if (many || tile == t1 || n >= kLogprobPrune || (threshold == 0 && n >= a.top)) {
+      // all of the places' logits at once
+      for (int i = tid; i < n; i += kLogprobThreads)
+        if (i >= keys) l.list[i] = logit_key(widened(base[l.list[i]]), (int)l.list[i] - before);
+      __syncthreads();
+      if (!many) {
+        threshold = best_keys(l, n, a.top);
+        n = min(n, a.top);
+      } else {
 #pragma unroll 1
-      for (int again = start; again < stop; ++again) {
-        // the top-th of the threads' largest keys
-        uint64_t own = 0;
-        Tile::each(base, before, end, again, [&](float x, int i) { own = max(own, logit_key(x, i)); });
-        l.per_thread[tid] = own;
-        if (tid == 0) l.exact = 0;
-        __syncthreads();
-        uint64_t mine[kShare];
-        int rank[kShare];
-        mine[0] = own;
-        ranks<1>(l.per_thread, kLogprobThreads, mine, rank);
-        if (own && rank[0] == a.top - 1) l.exact = own - 1;
-        __syncthreads();
-        above = max(l.exact, threshold);
-        Tile::each(base, before, end, again, [&](float x, int i) {
-          const uint64_t key = logit_key(x, i);
-          if (key > above) put(key);
-        });
-        n += added();
-        threshold = best_keys(l, n, a.top);
-        n = min(n, a.top);
+        for (int again = start; again < stop; ++again) {
+          uint64_t own = 0;
+          Tile::each(base, before, end, again, [&](float x, int i) { own = max(own, logit_key(x, i)); });
+          l.per_thread[tid] = own;
+          if (tid == 0) l.exact = 0;
+          const int over = __syncthreads_count(own > threshold);
+          if (over == 0) continue;
+          uint64_t above = threshold;
+          if (n + over * Tile::kPieces * Tile::E > kCandidates) {  // the list might not hold what these threads have
+            // the top-th of the threads' largest keys
+            uint64_t mine[kShare];
+            int rank[kShare];
+            mine[0] = own;
+            ranks<1>(l.per_thread, kLogprobThreads, mine, rank);
+            if (own && rank[0] == a.top - 1) l.exact = own - 1;
+            __syncthreads();
+            above = max(l.exact, threshold);
+          }
+          Tile::each(base, before, end, again, [&](float x, int i) {
+            const uint64_t key = logit_key(x, i);
+            if (key > above) put(key);
+          });
+          n += added();
+          threshold = best_keys(l, n, a.top);
+          n = min(n, a.top);
+        }
       }
-    } else {
-      n += c;
-      if (tile == t1 || n >= kLogprobPrune || (threshold == 0 && n >= a.top)) {
-        threshold = best_keys(l, n, a.top);
-        n = min(n, a.top);
-      }
+      keys = n;
     }
-    if (threshold) above = threshold, limit = key_logit(threshold);
+    if (threshold) limit = key_logit(threshold);
   }
   r.over_wave();
   if ((tid & 63) == 0) l.stats[tid >> 6] = r;

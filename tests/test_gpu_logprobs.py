@@ -128,6 +128,32 @@ def test_rows_of_all_shapes_in_one_block_each(top, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("threads", [40, 56, 60, 63, 64, 65])
+def test_a_crowd_behind_candidates(threads, dtype):
+    """Some candidates in the list, then nearly as many at once as it holds: all the logits of some threads."""
+    say("crowd", threads, dtype)
+    piece = 16 // dtype.itemsize
+    tile = 4 * 256 * piece
+    if dtype is F32:
+        threads *= 2  # half as many logits each
+    n, rows, vocab = 10, 520, 20 * tile
+    x = logits(6, n, vocab, dtype, std=0.5)
+    g = torch.Generator(device="cuda").manual_seed(threads)
+    # few logits above the first tiles' best, fewer than are sorted out at once
+    few = 9 * tile + 61 * torch.arange(100, device="cuda")
+    x[:, few] = (5 + torch.rand(n, 100, device="cuda", generator=g)).to(dtype)
+    for j in range(4):
+        at = 16 * tile + j * 256 * piece
+        x[:, at:at + threads * piece] = (10 + 4 * torch.rand(n, threads * piece, device="cuda", generator=g)).to(dtype)
+    t = tokens(4, n, 1, vocab)
+    again = torch.arange(rows, device="cuda") % n
+    got = ops().token_logprobs(x[again], t[again], top=20)
+    check(x, t, 20, type(got)(*(a[:n] for a in got)))
+    for a in got:  # rows of whole 16 bytes: the same bits
+        assert torch.equal(a.view(torch.uint8), a[:n].contiguous()[again].view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("vocab", [40, 9001, 100003])
 def test_not_finite(vocab, dtype):
     """NaN and infinity make a row's numbers NaN, wherever they lie; its order stays."""
