@@ -170,7 +170,7 @@ __device__ __forceinline__ uint64_t best_keys(LogprobShared& l, int n, int top) 
   int rank[kShare];
 #pragma unroll
   for (int b = 0; b < kShare; ++b) mine[b] = b * kLogprobThreads + tid < n ? l.list[b * kLogprobThreads + tid] : 0;
-  if (n > 64) {  // most are below a bound that is sooner had than their ranks
+  if (n > 128) {  // most are below a bound that is sooner had than their ranks (with 64, 0.5 us more for 64 rows with 20)
     uint32_t most = 0;
 #pragma unroll
     for (int b = 0; b < kShare; ++b) most = max(most, (uint32_t)(mine[b] >> 32));
