@@ -177,7 +177,10 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
     }
     const float amax = bitsf(m);
     const bool zeros = m >= 0x7f800000u || amax < kLeastAmax;
-    const float up = 127.0f / amax;
+    // 127 / a in two parts: with the second one y (127 / a) rounds once. Without it the values of a / 2, common among
+    // BF16 and 63.5 exactly, were 63 under 14 of the 128 mantissas of a. (2048 channels 9.8 -> 10.0 us for 8192 rows,
+    // 6144 29.4 both.)
+    const float up = 127.0f / amax, rest = __builtin_fmaf(-up, amax, 127.0f) * up * (1.0f / 127.0f);
     if (lane == 0) a.scale[row] = m >= 0x7f800000u ? bitsf(0x7fc00000u) : zeros ? 0.0f : amax / 127.0f;
     int8_t* to = a.data + row * a.data_stride;
 #pragma unroll
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
       const int i = (p * kLanes + lane) * E;
       if (i >= a.channels) continue;
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[p][e] = zeros ? 0.0f : y[p][e] * up;
+      for (int e = 0; e < E; ++e) y[p][e] = zeros ? 0.0f : __builtin_fmaf(y[p][e], up, y[p][e] * rest);
       if (E == 8) *reinterpret_cast<uint2*>(to + i) = make_uint2(pack_int8(y[p]), pack_int8(y[p] + E / 2));
       else *reinterpret_cast<uint32_t*>(to + i) = pack_int8(y[p]);
     }

@@ -1,0 +1,60 @@
+"""Where the roundings of the 8-bit rows lie: integers at exact halves, and gated
+values far out, against the definitions in 64 bits."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+def ops():
+    import cq35
+    return cq35
+
+
+def mantissas(channels, power):
+    """A row for each of the 128 mantissas that a largest magnitude can have in BF16: the
+    magnitude, its halves of both signs, and values of all sizes below it."""
+    g = torch.Generator().manual_seed(channels)
+    a = (torch.arange(128, 256, dtype=torch.float64) * 2.0 ** power)[:, None]
+    x = (torch.rand(128, channels, dtype=torch.float64, generator=g) * 2 - 1) * 2.0 ** -torch.randint(12, (128, channels), generator=g)
+    x = (x * a).to(BF).double().clamp(-a, a)
+    x[:, 3:4], x[:, 5:6], x[:, channels - 2:channels - 1] = -a, a / 2, -a / 2
+    return x, a
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("power", [-120, -7, 100, 119])
+@pytest.mark.parametrize("channels", [16, 272, 2064, 9008])
+def test_integers_of_exact_halves(channels, power, dtype):
+    """y (127 / a) of values of 8 bits is a half exactly or at least 2^-16 of itself away from one, so
+    that one rounding to F32 decides nothing: every integer is the definition's. 64 bits hold 127 y
+    exactly and divide with far less than that."""
+    say("halves", channels, power, dtype)
+    x, a = mantissas(channels, power)
+    q = ops().quantize_rows(x.to(dtype).cuda())
+    assert torch.equal(q.data.cpu().double(), torch.round(127 * x / a))
+    assert torch.equal(q.scale.cpu(), (a[:, 0] / 127).float())
+    assert bool((q.data[:, 5] == 64).all()) and bool((q.data[:, channels - 2] == -64).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_halves_of_a_norm_and_a_gated_product(dtype):
+    """The same behind the norm of a row of ones, whose values are its weights, and behind gates so far
+    out that their sigmoid is 1."""
+    say("halves behind others", dtype)
+    x, a = mantissas(272, -7)
+    one = torch.ones(1, 272, device="cuda", dtype=dtype)
+    want = torch.round(127 * x / a)
+    for r in range(128):
+        q = ops().norm_quantize(one, x[r].float().cuda(), eps=0.0)
+        assert torch.equal(q.data[0].cpu().double(), want[r]), r
+    gate = torch.full((128, 272), 128.0, dtype=dtype, device="cuda")
+    q = ops().gated_quantize(gate, x.to(dtype).cuda())
+    assert torch.equal(q.data.cpu().double(), want)
