@@ -5,7 +5,8 @@
 // One pass: a row stays in registers between its sums and its integers. Bound by bytes where there are
 // many rows: 8192 rows of 4096 channels 21.5 us (4.7 TB/s; a large copy: 5.1), of 2048 with residual and
 // norm 25.9 (4.5), of 6144 gated 48.5 (5.2). A row or a few are latency, 2.6 to 3.5 us. With the norm's
-// weights read for every row behind its sum, and no next row under way, the second took 30 us.
+// weights read for every row behind its sum, and no next row under way, the second took 30 us. Rows beyond 8192
+// channels: 4096 of 12288 normed with residual 86 us (4.1 TB/s; F32 145, 4.5), gated 63 (4.0; F32 92, 4.9).
 #pragma once
 
 #include "lanes.h"
@@ -74,22 +75,29 @@ __device__ __forceinline__ uint32_t pack_int8(const float* v) {
 }
 
 // kLanes threads a row, kPieces pieces of 16 bytes a thread. Where a wave is a row it goes on to others, the next
-// one's pieces asked for under the current one's arithmetic and the norm's weights kept in registers.
+// one's pieces asked for under the current one's arithmetic and the norm's weights kept in registers. Sixteen waves
+// have 128 registers a thread and 64 values in them: what does not fit beside those is asked for piece by piece, the
+// weights behind the sum of squares. Held as in the other widths it went to scratch memory: 4096 rows of 12288
+// channels normed with residual 167 us instead of 86 (F32 393, 143), gated F32 132 instead of 92.
 template <typename T, RowSource kSource, int kLanes, int kPieces>
 __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowArgs a) {
   typedef RowPiece<T> P;
   constexpr int E = P::kValues, kThreads = kLanes < 256 ? 256 : kLanes, kWaves = kLanes / 64, kRows = kThreads / kLanes;
+  // registers for a row's pieces and the weights at once, beside its values
+  constexpr int kBeside = kPieces * (kSource == RowSource::kPlain ? 4 : 8) + (kSource == RowSource::kNorm ? kPieces * E : 0);
+  constexpr bool kHeld = kLanes < 1024 || kBeside <= 64;
+  constexpr int kBatch = kHeld ? kPieces : 1;
   __shared__ float sums[kWaves];
   __shared__ uint32_t most[kWaves];
   const int tid = threadIdx.x, lane = tid % kLanes, wave = lane >> 6;
   const bool two = kSource == RowSource::kGated || (kSource == RowSource::kNorm && a.b);
   struct Row {
-    u32x4 a[kPieces], b[kSource == RowSource::kPlain ? 1 : kPieces];
+    u32x4 a[kBatch], b[kSource == RowSource::kPlain ? 1 : kBatch];
   } next;
-  auto load = [&](Row& r, int64_t row) {
+  auto load = [&](Row& r, int64_t row, int first) {
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-      const int i = (p * kLanes + lane) * E;
+    for (int p = 0; p < kBatch; ++p) {
+      const int i = ((first + p) * kLanes + lane) * E;
       if (i >= a.channels) continue;
       r.a[p] = *reinterpret_cast<const u32x4*>((const T*)a.a + row * a.a_stride + i);
       if (kSource != RowSource::kPlain && two) r.b[p] = *reinterpret_cast<const u32x4*>((const T*)a.b + row * a.b_stride + i);
@@ -97,34 +105,37 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
   };
   int64_t row = (int64_t)blockIdx.x * kRows + tid / kLanes;
   if (row >= a.rows) return;  // whole waves; only where a wave is a row
-  load(next, row);
-  float w[kSource == RowSource::kNorm ? kPieces : 1][E];
-  if (kSource == RowSource::kNorm)
+  load(next, row, 0);
+  auto load_weights = [&](float* w, int i) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(a.weight + i + e);
+      w[e] = v.x, w[e + 1] = v.y, w[e + 2] = v.z, w[e + 3] = v.w;
+    }
+  };
+  float w[kHeld && kSource == RowSource::kNorm ? kPieces : 1][E];
+  if (kHeld && kSource == RowSource::kNorm)
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
       const int i = (p * kLanes + lane) * E;
-      if (i >= a.channels) continue;
-#pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(a.weight + i + e);
-        w[p][e] = v.x, w[p][e + 1] = v.y, w[p][e + 2] = v.z, w[p][e + 3] = v.w;
-      }
+      if (i < a.channels) load_weights(w[p], i);
     }
   for (;;) {
-    const Row now = next;
+    Row now = next;
     const int64_t after = row + (int64_t)gridDim.x * kRows;
-    if (kLanes == 64 && after < a.rows) load(next, after);
+    if (kLanes == 64 && after < a.rows) load(next, after, 0);
     float y[kPieces][E];
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
       const int i = (p * kLanes + lane) * E;
+      if (p > 0 && p % kBatch == 0) load(now, row, p);
 #pragma unroll
       for (int e = 0; e < E; ++e) y[p][e] = 0.0f;
       if (i >= a.channels) continue;
-      P::widen(now.a[p], y[p]);
+      P::widen(now.a[p % kBatch], y[p]);
       if (kSource == RowSource::kNorm && two) {
         float r[E];
-        P::widen(now.b[p], r);
+        P::widen(now.b[p % kBatch], r);
 #pragma unroll
         for (int e = 0; e < E; ++e) y[p][e] += r[e];
         // the sum in the stream's type is what the norm sees
@@ -134,7 +145,7 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
       }
       if (kSource == RowSource::kGated) {
         float u[E];
-        P::widen(now.b[p], u);
+        P::widen(now.b[p % kBatch], u);
 #pragma unroll
         for (int e = 0; e < E; ++e)
           y[p][e] = y[p][e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y[p][e] * -1.44269504f)) * u[e];
@@ -156,10 +167,13 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
       }
       const float inverse = 1.0f / sqrtf(s / (float)a.channels + a.eps);
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p)
-        if ((p * kLanes + lane) * E < a.channels)
+      for (int p = 0; p < kPieces; ++p) {
+        const int i = (p * kLanes + lane) * E;
+        if (i >= a.channels) continue;
+        if (!kHeld) load_weights(w[0], i);
 #pragma unroll
-          for (int e = 0; e < E; ++e) y[p][e] = y[p][e] * inverse * w[p][e];
+        for (int e = 0; e < E; ++e) y[p][e] = y[p][e] * inverse * w[kHeld ? p : 0][e];
+      }
     }
     // magnitudes as integers: infinity and NaN are the largest
     uint32_t m = 0;
