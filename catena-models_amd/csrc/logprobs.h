@@ -92,7 +92,8 @@ struct RowStats {
     t = f * (t + s * fmaxf(d, -200.0f));
     s *= f, m = to;
   }
-  __device__ __forceinline__ void add(float d) {
+  // a logit's terms, d = x - m
+  static __device__ __forceinline__ void add(float d, float& s, float& t) {
     const float w = power(d);
     s += w, t = __builtin_fmaf(w, fmaxf(d, -200.0f), t);  // nothing of a logit of -inf
   }
@@ -320,11 +321,15 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void k_logprobs(LogprobArgs a) 
 #pragma unroll
         for (int e = 0; e < Tile::E; ++e) most = fmaxf(most, v.value(j, e));
       if (most > r.m) r.rebase(most);
+      // a tile's terms first among themselves: one chain over a row's logits rounds a thousand times, and
+      // loses terms below half a step of the sum
       const float from = RowStats::reference(r.m);
+      float tile_s = 0.0f, tile_t = 0.0f;
 #pragma unroll
       for (int j = 0; j < Tile::kPieces; ++j)
 #pragma unroll
-        for (int e = 0; e < Tile::E; ++e) r.add(v.value(j, e) - from);
+        for (int e = 0; e < Tile::E; ++e) RowStats::add(v.value(j, e) - from, tile_s, tile_t);
+      r.s += tile_s, r.t += tile_t;
       if (!kTop) continue;
       if (threshold == 0 && tile == start) {
         int passed;
