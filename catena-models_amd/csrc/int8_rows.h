@@ -4,9 +4,9 @@
 //
 // One pass: a row stays in registers between its sums and its integers. Bound by bytes where there are
 // many rows: 8192 rows of 4096 channels 21.5 us (4.7 TB/s; a large copy: 5.1), of 2048 with residual and
-// norm 25.9 (4.5), of 6144 gated 48.5 (5.2). A row or a few are latency, 2.6 to 3.5 us. With the norm's
+// norm 25.9 (4.5), of 6144 gated 49.7 (5.1). A row or a few are latency, 2.6 to 3.5 us. With the norm's
 // weights read for every row behind its sum, and no next row under way, the second took 30 us. Rows beyond 8192
-// channels: 4096 of 12288 normed with residual 86 us (4.1 TB/s; F32 145, 4.5), gated 63 (4.0; F32 92, 4.9).
+// channels: 4096 of 12288 normed with residual 86 us (4.1 TB/s; F32 145, 4.5), gated 67 (3.8; F32 93, 4.9).
 #pragma once
 
 #include "lanes.h"
@@ -74,11 +74,21 @@ __device__ __forceinline__ uint32_t pack_int8(const float* v) {
   return lo | hi << 16;
 }
 
+// g / (1 + e^-g), within 8 half-steps of F32 down to g = -87.3 (e^-g = 2^126), 0 below: e^-g = 2^t (1 + r ln 2) with
+// t = -g log2 e rounded and r what its rounding and that of log2 e leave out; 2^t alone was off by up to 1.5 |g|
+// half-steps more, and took 1 to 4 % less time (8192 rows of 6144 BF16 48.4 instead of 49.7 us, of 2048 17.4 and 18.0).
+__device__ __forceinline__ float gate_of(float g) {
+  const float t = g * -1.44269502f;
+  const float r = __builtin_fmaf(g, -1.92596299e-8f, __builtin_fmaf(g, -1.44269502f, -t));
+  const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, 0.693147181f, 1.0f);
+  return g * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 // kLanes threads a row, kPieces pieces of 16 bytes a thread. Where a wave is a row it goes on to others, the next
 // one's pieces asked for under the current one's arithmetic and the norm's weights kept in registers. Sixteen waves
 // have 128 registers a thread and 64 values in them: what does not fit beside those is asked for piece by piece, the
 // weights behind the sum of squares. Held as in the other widths it went to scratch memory: 4096 rows of 12288
-// channels normed with residual 167 us instead of 86 (F32 393, 143), gated F32 132 instead of 92.
+// channels normed with residual 167 us instead of 86 (F32 393, 145), gated F32 132 instead of 93.
 template <typename T, RowSource kSource, int kLanes, int kPieces>
 __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowArgs a) {
   typedef RowPiece<T> P;
@@ -147,8 +157,7 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowAr
         float u[E];
         P::widen(now.b[p % kBatch], u);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          y[p][e] = y[p][e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y[p][e] * -1.44269504f)) * u[e];
+        for (int e = 0; e < E; ++e) y[p][e] = gate_of(y[p][e]) * u[e];
       }
     }
     if (kSource == RowSource::kNorm) {

@@ -502,7 +502,8 @@ typedef struct cq35_int8_rows {
  *     alike); without a residual (NULL) h = x and nothing is written. w: F32, at a
  *     16-byte address. A row whose mean square passes F32's range gives zeros. x,
  *     residual and summed have one type.
- *   cq35_gated_quantize: y = gate / (1 + e^-gate) * up, of one type
+ *   cq35_gated_quantize: y = gate / (1 + e^-gate) * up, of one type; 0 for gates below
+ *     -87.3, where e^-gate passes 2^126
  * F32 inside. Outputs overlap no input, summed apart. Up to 2^21 rows. */
 int cq35_quantize_rows(const cq35_rows* x, int64_t rows, int64_t channels, const cq35_int8_rows* out,
                        void* stream);

@@ -58,3 +58,21 @@ def test_halves_of_a_norm_and_a_gated_product(dtype):
     gate = torch.full((128, 272), 128.0, dtype=dtype, device="cuda")
     q = ops().gated_quantize(gate, x.to(dtype).cuda())
     assert torch.equal(q.data.cpu().double(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("channels", [16, 2064, 9008])
+def test_gates_far_out(channels, dtype):
+    """A row of one gate and one factor: its scale times 127 is the product itself. In half-steps u of
+    F32: e^-g is off by 4 (2^t within a step, its correction and their product by 1 each), 1 + e^-g by 1, the
+    reciprocal by 2 (a step), two products and the scale's division by 1 each. Gates to where e^-g
+    nears 2^126."""
+    say("gates", channels, dtype)
+    gate = torch.cat([torch.linspace(-87.0, 87.0, 700), torch.tensor([-0.5, -1e-3, 1e-3, 2.0 ** -60, 100.0, 1e4])]).to(dtype)
+    up = torch.where(torch.arange(len(gate)) % 2 == 0, 1.0, -2.75).to(dtype)
+    up[gate < -40] *= 2.0 ** 60  # the product itself stays far above the least magnitude
+    q = ops().gated_quantize(*(t[:, None].expand(-1, channels).contiguous().cuda() for t in (gate, up)))
+    y = gate.double() * torch.sigmoid(gate.double()) * up.double()
+    off = (q.scale.cpu().double() * 127 / y.abs() - 1).abs() / 2.0 ** -24
+    assert off.max() <= 10.1, (off.max(), gate[off.argmax()])
+    assert torch.equal(q.data.cpu().double(), (127.0 * y.sign())[:, None].expand(-1, channels))
