@@ -13,22 +13,16 @@ __device__ __forceinline__ T lane_moved(T x) {
   return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(i, i, kCtrl, 0xf, 0xf, false));
 }
 
-// x and the other half's of each pair of rows of 16, or of the two of 32, in an order that both share. The
-// second operand is made a value of its own: given the same one twice, the compiler takes
-// the two results for one.
+// x and the other half's of each pair of rows of 16, or of the two of 32, in an order that both share.
 struct LanePair {
   int a, b;
 };
 __device__ __forceinline__ LanePair rows16_pair(int x) {
-  int y = x;
-  asm("" : "+v"(y));
-  const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
   return {(int)r[0], (int)r[1]};
 }
 __device__ __forceinline__ LanePair rows32_pair(int x) {
-  int y = x;
-  asm("" : "+v"(y));
-  const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return {(int)r[0], (int)r[1]};
 }
 
