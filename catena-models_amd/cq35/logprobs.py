@@ -28,6 +28,8 @@ class TokenLogprobs(NamedTuple):
 
 
 def _results(out, given, rows, top, device):
+    if not isinstance(out, (tuple, list)) or len(out) != len(TokenLogprobs._fields):
+        raise TypeError("out must be the four tensors of a TokenLogprobs")
     for name, t, shape, dtype in zip(TokenLogprobs._fields, out, (given, (rows,), (rows, top), (rows, top)), (_F32, _F32, _I64, _F32)):
         if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()):
             _why("out." + name, t, dtype, len(shape), device)

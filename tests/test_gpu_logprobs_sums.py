@@ -34,3 +34,14 @@ def test_small_terms_behind_large_ones(dtype, low):
     assert np.abs(got.logprobs[:, 1].cpu().double().numpy() - lp[0, 1]).max() <= limit + 2 * ref.U * abs(lp[0, 1])
     assert np.abs(got.entropy.cpu().double().numpy() - entropy[0]).max() <= limit + 0.01 * 2 * 105 * ref.U + 2 * ref.U * entropy[0]
     assert bool((got.top_tokens == 0).all())
+
+
+def test_results_of_another_number_are_refused():
+    print("results", flush=True)
+    import cq35
+    x, t = torch.zeros(3, 50, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    whole = cq35.token_logprobs(x, t, top=2)
+    for out in (whole[:3], whole[:2], (), list(whole) + [whole[0]], x, 5):
+        with pytest.raises(TypeError, match="four tensors"):
+            cq35.token_logprobs(x, t, top=2, out=out)
+    assert cq35.token_logprobs(x, t, top=2, out=list(whole)).entropy is whole.entropy
