@@ -500,8 +500,9 @@ typedef struct cq35_int8_rows {
  *   cq35_norm_quantize:  y = h w / sqrt(mean(h^2) + eps) with h = x + residual, rounded to
  *     their type and written to `summed` (x or residual itself allowed, laid out
  *     alike); without a residual (NULL) h = x and nothing is written. w: F32, at a
- *     16-byte address. A row whose mean square passes F32's range gives zeros. x,
- *     residual and summed have one type.
+ *     16-byte address. The mean square is F32's: a row where it passes F32's range gives
+ *     zeros, one where mean and eps are both 0 (eps = 0 and every |h| below 2^-75) the scale
+ *     NaN. x, residual and summed have one type.
  *   cq35_gated_quantize: y = gate / (1 + e^-gate) * up, of one type; 0 for gates below
  *     -87.3, where e^-gate passes 2^126
  * F32 inside. Outputs overlap no input, summed apart. Up to 2^21 rows. */

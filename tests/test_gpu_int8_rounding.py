@@ -76,3 +76,22 @@ def test_gates_far_out(channels, dtype):
     off = (q.scale.cpu().double() * 127 / y.abs() - 1).abs() / 2.0 ** -24
     assert off.max() <= 10.1, (off.max(), gate[off.argmax()])
     assert torch.equal(q.data.cpu().double(), (127.0 * y.sign())[:, None].expand(-1, channels))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("channels", [16, 2064, 9008])
+def test_norm_of_tiny_rows(channels, dtype):
+    """Rows of one power of two: the norm is the weights down to squares of 2^-140, exact in F32's subnormals;
+    below 2^-75 the squares are zeros, which eps decides about."""
+    say("tiny rows", channels, dtype)
+    w = torch.linspace(0.5, 2.0, channels).cuda()
+    tiny = torch.tensor([2.0 ** -30, 2.0 ** -60, 2.0 ** -70, 2.0 ** -76, 2.0 ** -100, 0.0], dtype=dtype, device="cuda")
+    x = tiny[:, None].expand(-1, channels).contiguous()
+    q = ops().norm_quantize(x, w, eps=0.0)
+    for r in range(3):
+        assert torch.equal(q.data[r].cpu().double(), torch.round(127 * w.cpu().double() / 2))
+        assert float(q.scale[r]) == float(torch.tensor(2.0) / 127)
+    assert bool(torch.isnan(q.scale[3:]).all()) and bool((q.data[3:] == 0).all())
+    q = ops().norm_quantize(x, w, eps=1e-6)
+    off = q.scale.cpu().double() * 127 / (tiny.cpu().double() * 2 / (tiny.cpu().double() ** 2 + 1e-6).sqrt()) - 1
+    assert off[:5].abs().max() < 8 * 2.0 ** -24 and float(q.scale[5]) == 0  # eps, mean and root, division, two products, the scale
