@@ -11,8 +11,9 @@
 namespace {
 
 constexpr int64_t kMostRows = 1 << 21;  // times 1024 threads: a launch takes below 2^32
-constexpr int64_t kRowBlocks = 2048;  // eight a CU; where a wave is a row, more rows share a wave
-constexpr int64_t kLogprobBlocks = 1024;  // four a CU; more rows take a block each
+constexpr int64_t kComputeUnits = 256;
+constexpr int64_t kRowBlocks = 8 * kComputeUnits;  // where a wave is a row, more rows share a wave
+constexpr int64_t kLogprobBlocks = 4 * kComputeUnits;  // more rows take a block each
 constexpr int64_t kMostResults = 1ll << 34;  // in tiles of 16 x 16 by 512 threads as well
 
 bool row_type(int32_t dtype) { return dtype == CQ35_BF16 || dtype == CQ35_F32; }
@@ -80,7 +81,7 @@ template <typename T, int MT>
 int launch_few(const ProductArgs& a, hipStream_t s) {
   const unsigned blocks = (unsigned)((a.outputs + 15) / 16);
   // more than two blocks a compute unit: the kernel of which four fit
-  const bool many = MT > 1 || blocks > 512;
+  const bool many = MT > 1 || blocks > 2 * kComputeUnits;
   return launch_operator("int8 linear", many ? k_int8_few<T, MT, 2> : k_int8_few<T, MT, (MT > 1 ? 2 : 4)>, dim3(blocks), 512, 0, s, a);
 }
 
@@ -90,6 +91,9 @@ int launch_few(const ProductArgs& a, hipStream_t s) {
 // 21.6, 20.7, 31.1; 4096 rows 163, 105, 93, 103; 8192 rows to 12288 outputs -, 280, 251, 234. Up to 16 rows the
 // kernel of few rows takes 4.1 to 4.8 to 2048 outputs (64 x 64: 7.8); one row 6.9 to 12288 (8.1) and 83 to 248320 (90),
 // but sixteen 8.6 (8.2) and 140 (111).
+// All with operands in the memory-side cache. No kernel divides the channels among blocks, so many channels to few
+// outputs leave compute units idle: 33, 64, 128 and 300 rows of 6144 channels to 2048 outputs take 17 to 18, from HBM
+// 23 to 25, one row 6.2 and 7.2, 300 rows of 3584 to 1024 11.3; a read of their bytes takes 1 to 3.
 struct ProductKernel {
   int rows, outputs;  // of a block
   int most_rows;
@@ -108,7 +112,7 @@ int product_kernel(int64_t rows, int64_t outputs, int64_t channels) {
     const ProductKernel& k = kProductKernels[i];
     if (rows > k.most_rows) continue;
     const int64_t blocks = ((rows + k.rows - 1) / k.rows) * ((outputs + k.outputs - 1) / k.outputs);
-    const int64_t stages = (channels + 63) / 64, more = (blocks + 255) / 256 - 1;
+    const int64_t stages = (channels + 63) / 64, more = (blocks + kComputeUnits - 1) / kComputeUnits - 1;
     const int64_t time = k.start + stages * k.stage + more * (k.more_start + stages * (k.more_stage + rows * k.more_row));
     if (time < least) best = i, least = time;
   }

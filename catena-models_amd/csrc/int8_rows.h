@@ -3,8 +3,8 @@
 // (RowSource::kNorm) and the gated product of a feed-forward (RowSource::kGated).
 //
 // One pass: a row stays in registers between its sums and its integers. Bound by bytes where there are
-// many rows: 8192 rows of 4096 channels 21.5 us (4.7 TB/s; a large copy: 5.1), of 2048 with residual and
-// norm 25.9 (4.5), of 6144 gated 49.7 (5.1). A row or a few are latency, 2.6 to 3.5 us. With the norm's
+// many rows: 8192 rows of 4096 channels 21.7 us (4.7 TB/s; a large copy: 5.0), of 2048 with residual and
+// norm 26.2 (4.5), of 6144 gated 49.9 (5.0); where results go to the same memory each time 19.2, 22.9 and 45.5. A row or a few are latency, 2.6 to 3.5 us. With the norm's
 // weights read for every row behind its sum, and no next row under way, the second took 30 us. Rows beyond 8192
 // channels: 4096 of 12288 normed with residual 86 us (4.1 TB/s; F32 145, 4.5), gated 67 (3.8; F32 93, 4.9).
 #pragma once
@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t pack_int8(const float* v) {
 
 // g / (1 + e^-g), within 8 half-steps of F32 down to g = -87.3 (e^-g = 2^126), 0 below: e^-g = 2^t (1 + r ln 2) with
 // t = -g log2 e rounded and r what its rounding and that of log2 e leave out; 2^t alone was off by up to 1.5 |g|
-// half-steps more, and took 1 to 4 % less time (8192 rows of 6144 BF16 48.4 instead of 49.7 us, of 2048 17.4 and 18.0).
+// half-steps more, and took 1 to 4 % less time (8192 rows of 6144 BF16 48.4 instead of 49.7, of 2048 17.4 and 18.0).
 __device__ __forceinline__ float gate_of(float g) {
   const float t = g * -1.44269502f;
   const float r = __builtin_fmaf(g, -1.92596299e-8f, __builtin_fmaf(g, -1.44269502f, -t));

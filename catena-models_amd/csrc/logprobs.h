@@ -30,12 +30,14 @@ namespace cq35 {
 // without a mask.
 //
 // Bound by the logits' bytes where there are many rows: 1000 rows of 248320 BF16 logits with one
-// alternative 99 us (5.0 TB/s), with 20 112; 64 rows of F32 with 20 19, without any 12.2. One row is
-// latency: 6.7 us in 31 blocks, then 4 us for the join. A barrier a tile: 205 us for the 1000 rows, one in two 8 %
-// and one in four 2 % more than one in eight, one in sixteen as much as in eight. A candidate's logit read again where
-// it is found, and not all of them at once in front of best_keys: 102 us; a thread's logits kept in registers for
-// them: 168 registers instead of 127, half the waves; tiles of 32 F32 logits a thread instead of 16: spilled, 31 us
-// for the 64 rows; 512 or 2048 blocks wanted instead of 1024: 75 and 56 us for 300 rows, 53.
+// alternative 95 us (5.2 TB/s), with 20 105; 64 rows of F32 with 20 18.8, without any 12.2. One row is
+// latency: 6.8 us in 31 blocks, then 4 us for the join. A row is cut into as many blocks as 1024 hold of all rows, so
+// beyond 512 rows each has one: 512 rows with 5 take 60 us, 600 take 74; a row beyond 1024 waits for a block that
+// ends: 1025 rows with one 111. A barrier a tile: 205 us for the 1000 rows, one in two 8 % and one in four 2 % more
+// than one in eight, one in sixteen as much as in eight. A candidate's logit read again where it is found, and not
+// all of them at once in front of best_keys: 102 us; a thread's logits kept in registers for them: 168 registers
+// instead of 127, half the waves; tiles of 32 F32 logits a thread instead of 16: spilled, 31 us for the 64 rows; 512
+// or 2048 blocks wanted instead of 1024: 75 and 56 us for 300 rows, 53.
 constexpr int kLogprobsMostTop = 32;
 constexpr int kLogprobsMostGiven = 1024;
 constexpr int kLogprobThreads = 256;
@@ -45,6 +47,7 @@ constexpr int kLogprobMostSplits = kCandidates / kLogprobsMostTop;  // of a row,
 constexpr int kEpoch = 8;                                         // tiles between two looks at the list
 constexpr int kMoreGroups = 8;                                    // that may pass a bound beside those needed
 constexpr int kLogprobPrune = 128;                                // candidates that are cut down to the best
+constexpr int kRankedAtOnce = 128;                                // candidates that are ranked without a bound
 
 struct LogprobArgs {
   const void* logits;
@@ -171,7 +174,7 @@ __device__ __forceinline__ uint64_t best_keys(LogprobShared& l, int n, int top) 
   int rank[kShare];
 #pragma unroll
   for (int b = 0; b < kShare; ++b) mine[b] = b * kLogprobThreads + tid < n ? l.list[b * kLogprobThreads + tid] : 0;
-  if (n > 128) {  // most are below a bound that is sooner had than their ranks (with 64, 0.5 us more for 64 rows with 20)
+  if (n > kRankedAtOnce) {  // most are below a bound that is sooner had than their ranks (with 64, 0.5 us more for 64 rows with 20)
     uint32_t most = 0;
 #pragma unroll
     for (int b = 0; b < kShare; ++b) most = max(most, (uint32_t)(mine[b] >> 32));
