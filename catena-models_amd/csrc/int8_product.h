@@ -4,12 +4,12 @@
 // more where it is BF16.
 //
 // Few rows are bound by the weights' bytes and by latency: one row of 2048 channels to 12288 outputs 6.9 us with the
-// weights in the 256 MB memory-side cache, 8.4 from HBM (3.0 TB/s), to 248320 outputs 81 (6.3), to 2048 4.1. Large products are bound by the card's power: 8192 rows of 8192 channels to 8192
-// outputs 490 us, 2.2 POP/s, the matrix cores busy 0.61 of the cycles at 1.65 to 1.8 GHz; with nothing fetched the
-// same loop keeps them busy 0.76 at 2.2 GHz. Those of fewer channels add a tile's start and end, 10 us of
-// 256 x 256 results: 8192 rows of 2048 to 12288 outputs 245 us, 1.68 POP/s. In between LDS is the bound: the
-// waves' reads and the requests' writes share its port, 64 channels of a 128 x 128 tile take about 550
-// cycles there and 256 on the matrix cores.
+// weights in the 256 MB memory-side cache, 8.4 from HBM (3.0 TB/s), to 248320 outputs 81 (6.3), to 2048 4.1. Large
+// products are bound by the card's power: 8192 rows of 8192 channels to 8192 outputs 490 us, 2.2 POP/s, the matrix
+// cores busy 0.61 of the cycles at 1.65 to 1.8 GHz; with nothing fetched the same loop keeps them busy 0.76 at 2.2
+// GHz. Those of fewer channels add a tile's start and end, 10 us of 256 x 256 results: 8192 rows of 2048 to 12288
+// outputs 245 us, 1.68 POP/s. In between LDS is the bound: the waves' reads and the requests' writes share its port,
+// 64 channels of a 128 x 128 tile take about 550 cycles there and 256 on the matrix cores.
 #pragma once
 
 #include "layers.h"

@@ -4,9 +4,10 @@
 //
 // One pass: a row stays in registers between its sums and its integers. Bound by bytes where there are
 // many rows: 8192 rows of 4096 channels 21.7 us (4.7 TB/s; a large copy: 5.0), of 2048 with residual and
-// norm 26.2 (4.5), of 6144 gated 49.9 (5.0); where results go to the same memory each time 19.2, 22.9 and 45.5. A row or a few are latency, 2.6 to 3.5 us. With the norm's
-// weights read for every row behind its sum, and no next row under way, the second took 30 us. Rows beyond 8192
-// channels: 4096 of 12288 normed with residual 86 us (4.1 TB/s; F32 145, 4.5), gated 67 (3.8; F32 93, 4.9).
+// norm 26.2 (4.5), of 6144 gated 49.9 (5.0); where results go to the same memory each time 19.2, 22.9 and 45.5. A
+// row or a few are latency, 2.4 to 4 us. With the norm's weights read for every row behind its sum, and no next row
+// under way, the second took 30 us. Rows beyond 8192 channels: 4096 of 12288 normed with residual 86 us (4.1 TB/s;
+// F32 145, 4.5), gated 67 (3.8; F32 93, 4.9).
 #pragma once
 
 #include "lanes.h"
@@ -74,23 +75,27 @@ __device__ __forceinline__ uint32_t pack_int8(const float* v) {
   return lo | hi << 16;
 }
 
-// g / (1 + e^-g), within 8 half-steps of F32 down to g = -87.3 (e^-g = 2^126), 0 below: e^-g = 2^t (1 + r ln 2) with
+// g / (1 + e^-g), within 7 half-steps of F32 down to g = -87.3 (e^-g = 2^126), 0 below: e^-g = 2^t (1 + r ln 2) with
 // t = -g log2 e rounded and r what its rounding and that of log2 e leave out; 2^t alone was off by up to 1.5 |g|
-// half-steps more, and took 1 to 4 % less time (8192 rows of 6144 BF16 48.4 instead of 49.7, of 2048 17.4 and 18.0).
+// half-steps more, and took 1 to 4 % less time (8192 rows of 6144 BF16 48.4 instead of 49.9, of 2048 17.6 and 18.2).
+// Gates beyond 128, where e^-g is 0, have 128's exponent, as t of the largest would be infinite and r with it; a
+// minimum of their bits as integers leaves negative numbers alone (t is infinite for the largest of those, too, and
+// 2^t with it).
 __device__ __forceinline__ float gate_of(float g) {
-  const float t = g * -1.44269502f;
-  const float r = __builtin_fmaf(g, -1.92596299e-8f, __builtin_fmaf(g, -1.44269502f, -t));
-  const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, 0.693147181f, 1.0f);
-  return g * __builtin_amdgcn_rcpf(1.0f + e);
+  const float x = bitsf(min((int32_t)fbits(g), 0x43000000)), t = x * -1.44269502f;
+  const float r = __builtin_fmaf(x, -1.92596299e-8f, __builtin_fmaf(x, -1.44269502f, -t));
+  return g * __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(t), __builtin_fmaf(r, 0.693147181f, 1.0f), 1.0f));
 }
 
 // kLanes threads a row, kPieces pieces of 16 bytes a thread. Where a wave is a row it goes on to others, the next
 // one's pieces asked for under the current one's arithmetic and the norm's weights kept in registers. Sixteen waves
 // have 128 registers a thread and 64 values in them: what does not fit beside those is asked for piece by piece, the
 // weights behind the sum of squares. Held as in the other widths it went to scratch memory: 4096 rows of 12288
-// channels normed with residual 167 us instead of 86 (F32 393, 145), gated F32 132 instead of 93.
+// channels normed with residual 167 us instead of 86 (F32 393, 145), gated F32 132 instead of 93. Gated rows of BF16
+// in a wave each are asked to fit in 96 registers, five waves a SIMD: 97 without, and 18.7 us instead of 18.2 for 8192
+// rows of 2048.
 template <typename T, RowSource kSource, int kLanes, int kPieces>
-__global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void k_int8_rows(RowArgs a) {
+__global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes, kLanes == 64 && kSource == RowSource::kGated && sizeof(T) == 2 ? 5 : 1) void k_int8_rows(RowArgs a) {
   typedef RowPiece<T> P;
   constexpr int E = P::kValues, kThreads = kLanes < 256 ? 256 : kLanes, kWaves = kLanes / 64, kRows = kThreads / kLanes;
   // registers for a row's pieces and the weights at once, beside its values

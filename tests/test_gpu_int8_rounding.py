@@ -95,3 +95,25 @@ def test_norm_of_tiny_rows(channels, dtype):
     q = ops().norm_quantize(x, w, eps=1e-6)
     off = q.scale.cpu().double() * 127 / (tiny.cpu().double() * 2 / (tiny.cpu().double() ** 2 + 1e-6).sqrt()) - 1
     assert off[:5].abs().max() < 8 * 2.0 ** -24 and float(q.scale[5]) == 0  # eps, mean and root, division, two products, the scale
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("channels", [16, 2064, 9008])
+def test_gates_at_the_ends_of_the_range(channels, dtype):
+    """Gates whose exponent passes F32's range, to the largest number: the product is the gate, or 0."""
+    say("largest gates", channels, dtype)
+    top = torch.finfo(dtype).max
+    gate = torch.tensor([200.0, 2.0 ** 24, 1e30, 1e38, 2.3e38, 2.4e38, 3e38, top], dtype=torch.float64).to(dtype)
+    gate = torch.cat([gate, -gate])
+    rows = gate[:, None].expand(-1, channels).contiguous().cuda()
+    q = ops().gated_quantize(rows, torch.ones_like(rows))
+    n = len(gate) // 2
+    # the reciprocal of 1 is within a step, the scale rounds
+    off = (q.scale[:n].cpu().double() * 127 / gate[:n].double() - 1).abs() / 2.0 ** -24
+    assert off.max() <= 3.1, off
+    assert bool((q.data[:n] == 127).all())
+    assert q.scale[n:].tolist() == [0.0] * n and bool((q.data[n:] == 0).all())
+    for x in (float("inf"), float("-inf"), float("nan")):
+        rows[1, channels - 1] = x
+        q = ops().gated_quantize(rows, torch.ones_like(rows))
+        assert bool(torch.isnan(q.scale[1])) and bool((q.data[1] == 0).all())
